@@ -94,6 +94,30 @@ _SIGS = {
     "kvs_gpu_of": [_vp, C.c_longlong, _ip],
     "kvs_load": [_vp, C.c_int, C.POINTER(C.c_longlong), _ip],
 }
+
+
+class _W4Matrix(C.Structure):
+    _fields_ = [("device", C.c_int), ("n", C.c_int), ("k", C.c_int), ("group", C.c_int), ("codes", _vp),
+                ("scales", _vp), ("zeros", _vp)]
+
+
+class _LogitsCall(C.Structure):
+    _fields_ = [("device", C.c_int), ("rows", C.c_int), ("vocab", C.c_int), ("dtype", C.c_int), ("logits", _vp),
+                ("ld_logits", C.c_longlong), ("out", _vp), ("ld_out", C.c_longlong), ("pick", _vp), ("hist", _vp),
+                ("hist_off", _vp), ("gen_from", _vp), ("hist_n", C.c_longlong), ("repetition", _vp),
+                ("presence", _vp), ("frequency", _vp), ("bias_ids", _vp), ("bias", _vp), ("bias_off", _vp),
+                ("bias_n", C.c_longlong), ("mask", _vp), ("ld_mask", C.c_longlong)]
+
+
+_w4p = C.POINTER(_W4Matrix)
+_SIGS.update({
+    "w4_sizes": [C.c_int, C.c_int, C.c_int] + [C.POINTER(C.c_size_t)] * 3,
+    "w4_quantize": [_w4p, _vp, C.c_int, C.c_longlong, _vp],
+    "w4_dequantize": [_w4p, _vp, C.c_longlong, _vp],
+    "w4_linear": [_w4p, _vp, C.c_int, C.c_int, C.c_longlong, _vp, _vp, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp],
+    "w4_gated": [_w4p, _w4p, _vp, C.c_int, C.c_int, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp],
+    "logits_adjust": [C.POINTER(_LogitsCall), _vp],
+})
 _RESTYPE = {"kv_last_error": C.c_char_p, "kv_status_str": C.c_char_p, "kv_version": C.c_char_p}
 
 _lib = None
@@ -398,6 +422,181 @@ def combine_lse_packed(packed, rows, out, stream=None) -> None:
     G = packed.shape[0]
     dim = packed.shape[1] // rows - 2
     call("attn_combine_lse_packed", G, rows, dim, _ptr(packed), _ptr(out), _stream(stream))
+
+
+# ---------------------------------------------------------------- step_ops.h
+STEP_F16, STEP_BF16, STEP_F32 = 0, 1, 2
+_step_types = {}  # torch dtype -> STEP_*
+
+
+def _step_dtype(t, what: str) -> int:
+    if not _step_types:
+        import torch
+        _step_types.update({torch.float16: STEP_F16, torch.bfloat16: STEP_BF16, torch.float32: STEP_F32})
+    d = _step_types.get(t.dtype)
+    if d is None:
+        raise ValueError(f"{what}: unsupported element type {t.dtype}")
+    return d
+
+
+def _rows(t, device: int, what: str, rows=None, cols=None) -> int:
+    """A 2-D device tensor with contiguous rows: the elements from row to row."""
+    if t.dim() != 2 or t.get_device() != device:
+        raise ValueError(f"{what}: a 2-D tensor on cuda:{device} is expected")
+    m, n = t.shape
+    if (rows is not None and m != rows) or (cols is not None and n != cols):
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected ({rows}, {cols})")
+    ld, inner = t.stride()
+    if inner != 1 and n > 1:
+        raise ValueError(f"{what}: the elements of a row must be adjacent")
+    return ld if m > 1 else n
+
+
+def _words(t, device: int, what: str, dtype, n=None):
+    """The address of a contiguous 1-D device tensor of 4-byte values (None: NULL)."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.get_device() != device or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous 1-D {dtype} tensor on cuda:{device} is expected")
+    if n is not None and t.shape[0] != n:
+        raise ValueError(f"{what}: {t.shape[0]} values, expected {n}")
+    return t.data_ptr()
+
+
+def _stream_on(stream, device: int):
+    if stream is None:
+        import torch
+        return torch.cuda.current_stream(device).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+class W4:
+    """A matrix [n, k] in 4 bits (w4_matrix of include/step_ops.h, which gives
+    the layout): codes int32 [T, S, 2, 32, 4], scales fp16 [T, Q, 8, 2] and
+    zero points uint8 of that shape or None, with T = ceil(n / 16), S = ceil(k /
+    128), Q = ceil(k / group).  Made by w4_quantize, or from such tensors."""
+
+    def __init__(self, codes, scales, zeros, n: int, k: int, group: int):
+        import torch
+        load()
+        sizes = [C.c_size_t() for _ in range(3)]
+        call("w4_sizes", n, k, group, *[C.byref(x) for x in sizes])
+        dev = codes.get_device()
+        if dev < 0:
+            raise ValueError("codes: a device tensor is expected")
+        for t, size, dtype, what in ((codes, sizes[0], torch.int32, "codes"), (scales, sizes[1], torch.float16, "scales"),
+                                     (zeros, sizes[2], torch.uint8, "zeros")):
+            if t is None and what == "zeros":
+                continue
+            if t.dtype != dtype or t.get_device() != dev or not t.is_contiguous() or t.nbytes != size.value:
+                raise ValueError(f"{what}: {size.value} contiguous bytes of {dtype} on cuda:{dev} are expected")
+        self.codes, self.scales, self.zeros = codes, scales, zeros
+        self.n, self.k, self.group, self.device = n, k, group, dev
+        self._c = _W4Matrix(dev, n, k, group, codes.data_ptr(), scales.data_ptr(),
+                            zeros.data_ptr() if zeros is not None else None)
+
+    def dequantize(self, out=None, stream=None):
+        """The matrix's values, fp32 [n, k]."""
+        import torch
+        if out is None:
+            out = torch.empty(self.n, self.k, dtype=torch.float32, device=self.codes.device)
+        elif out.dtype != torch.float32:
+            raise ValueError("out: fp32 is expected")
+        ld = _rows(out, self.device, "out", self.n, self.k)
+        call("w4_dequantize", C.byref(self._c), out.data_ptr(), ld, _stream_on(stream, self.device))
+        return out
+
+
+def w4_quantize(w, group: int = 128, zero_points: bool = False, stream=None) -> W4:
+    """w [n, k] fp16 or bf16 -> W4 (w4_quantize of include/step_ops.h)."""
+    import torch
+    n, k = w.shape
+    if not (n > 0 and k > 0 and group in (32, 64, 128)):
+        raise ValueError(f"a 4-bit matrix of {n} x {k} in groups of {group}: groups of 32, 64 or 128 are supported")
+    T, S, Q = (n + 15) // 16, (k + 127) // 128, (k + group - 1) // group
+    m = W4(torch.empty((T, S, 2, 32, 4), dtype=torch.int32, device=w.device),
+           torch.empty((T, Q, 8, 2), dtype=torch.float16, device=w.device),
+           torch.empty((T, Q, 8, 2), dtype=torch.uint8, device=w.device) if zero_points else None, n, k, group)
+    ld = _rows(w, m.device, "w")
+    call("w4_quantize", C.byref(m._c), w.data_ptr(), _step_dtype(w, "w"), ld, _stream_on(stream, m.device))
+    return m
+
+
+def w4_linear(w: W4, x, out, bias=None, residual=None, stream=None) -> None:
+    """out [m, n] = x [m, k] W^T (+ bias [n] fp32) (+ residual [m, n], of out's
+    type; may be out).  x and out fp16, bf16 or fp32, rows any distance apart."""
+    dev = w.device
+    m = x.shape[0]
+    ldx = _rows(x, dev, "x", None, w.k)
+    ldo = _rows(out, dev, "out", m, w.n)
+    b = r = None
+    ldr = 0
+    if bias is not None:
+        import torch
+        b = _words(bias, dev, "bias", torch.float32, w.n)
+    if residual is not None:
+        ldr = _rows(residual, dev, "residual", m, w.n)
+        if residual.dtype != out.dtype:
+            raise ValueError("residual: out's element type is expected")
+        r = residual.data_ptr()
+    rc = _lib.w4_linear(w._c, x.data_ptr(), _step_dtype(x, "x"), m, ldx, b, r, ldr, out.data_ptr(),
+                        _step_dtype(out, "out"), ldo, _stream_on(stream, dev))
+    if rc:
+        _check(rc, "w4_linear")
+
+
+def w4_gated(gate: W4, up: W4, x, out, stream=None) -> None:
+    """out [m, n] = silu(x Wg^T) * (x Wu^T), types as w4_linear."""
+    dev = gate.device
+    m = x.shape[0]
+    ldx = _rows(x, dev, "x", None, gate.k)
+    ldo = _rows(out, dev, "out", m, gate.n)
+    rc = _lib.w4_gated(gate._c, up._c, x.data_ptr(), _step_dtype(x, "x"), m, ldx, out.data_ptr(),
+                       _step_dtype(out, "out"), ldo, _stream_on(stream, dev))
+    if rc:
+        _check(rc, "w4_gated")
+
+
+def logits_adjust(logits, out, pick=None, hist=None, hist_off=None, gen_from=None, repetition=None, presence=None,
+                  frequency=None, bias_ids=None, bias=None, bias_off=None, mask=None, stream=None) -> None:
+    """Penalties, biases and a mask on logits [rows, vocab] (fp32, fp16 or
+    bf16) into out (may be logits), and the greedy choice of each row into
+    pick [rows] int32 (-1: nothing is left): logits_adjust of
+    include/step_ops.h.  hist / bias_ids are int32 lists cut by hist_off /
+    bias_off [rows + 1]; gen_from int32 and the penalties fp32 have one value
+    per row; mask is int32 [rows, >= ceil(vocab / 32)], a set bit allows."""
+    import torch
+    i32, f32 = torch.int32, torch.float32
+    load()
+    dev = logits.get_device()
+    ld_in = _rows(logits, dev, "logits")
+    rows, vocab = logits.shape
+    ld_out = _rows(out, dev, "out", rows, vocab)
+    if out.dtype != logits.dtype:
+        raise ValueError("out: the logits' element type is expected")
+    mask_ptr, ld_mask = None, 0
+    if mask is not None:
+        if mask.dtype != i32:
+            raise ValueError("mask: int32 words are expected")
+        ld_mask = _rows(mask, dev, "mask", rows)
+        if mask.shape[1] < (vocab + 31) // 32:
+            raise ValueError(f"mask: {mask.shape[1]} words per row for {vocab} tokens")
+        mask_ptr = mask.data_ptr()
+    if (hist is None) != (hist_off is None) or not ((bias is None) == (bias_ids is None) == (bias_off is None)):
+        raise ValueError("hist and hist_off, and bias_ids, bias and bias_off, come together")
+    if gen_from is not None and hist is None:
+        raise ValueError("gen_from needs a history")
+    bias_n = bias_ids.shape[0] if bias_ids is not None else 0
+    c = _LogitsCall(dev, rows, vocab, _step_dtype(logits, "logits"), logits.data_ptr(), ld_in, out.data_ptr(), ld_out,
+                    _words(pick, dev, "pick", i32, rows), _words(hist, dev, "hist", i32),
+                    _words(hist_off, dev, "hist_off", i32, rows + 1), _words(gen_from, dev, "gen_from", i32, rows),
+                    hist.shape[0] if hist is not None else 0, _words(repetition, dev, "repetition", f32, rows),
+                    _words(presence, dev, "presence", f32, rows), _words(frequency, dev, "frequency", f32, rows),
+                    _words(bias_ids, dev, "bias_ids", i32), _words(bias, dev, "bias", f32, bias_n),
+                    _words(bias_off, dev, "bias_off", i32, rows + 1), bias_n, mask_ptr, ld_mask)
+    rc = _lib.logits_adjust(C.byref(c), _stream_on(stream, dev))
+    if rc:
+        _check(rc, "logits_adjust")
 
 
 class Scheduler:

@@ -1,0 +1,89 @@
+// w4_internal.h -- the 4-bit projections' arguments and launch plan, shared by
+// the kernels, the C ABI (step_ops.cu) and the model (qwen2_engine.cu).
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "kvattn_internal.h"
+#include "step_ops.h"
+
+namespace kvattn {
+
+// What x is: 16-bit codes of the operand type; fp32 kept whole (three bf16
+// parts); the model's fp32 rows rounded through the reference's fp16, plain or
+// after an RMSNorm.
+enum { W4_X_16 = 0, W4_X_F32 = 1, W4_X_ROUND = 2, W4_X_NORM = 3 };
+// Epilogues: the model's call sites (GemvArgs) and the public operators.
+enum { W4_QKV = 0, W4_RESID = 1, W4_GATE_UP = 2, W4_LOGITS = 3, W4_LINEAR = 4, W4_GATED = 5 };
+
+struct W4Args {
+    const uint32_t* codes[2] = {};
+    const __half* scales[2] = {};
+    const uint8_t* zeros[2] = {};
+    int N = 0, K = 0, M = 0;
+    int T = 0, S = 0, Q = 0;  // tiles of 16 rows, spans of 128 inputs, groups per row
+    const void* x = nullptr;
+    long long ldx = 0;
+    int in = W4_X_16, mode = W4_LINEAR;
+    int pieces = 1;           // operand rows per x row (3 for W4_X_F32)
+    int out_dtype = STEP_F32;
+    const float* bias = nullptr;
+    const void* residual = nullptr;
+    long long ldr = 0;
+    void* out = nullptr;
+    long long ldo = 0;
+    GemvArgs g;               // the model's epilogues and norm
+    // the launch plan
+    int rows = 0;             // x rows per pass
+    int ks = 1, cs = 1;       // a tile's spans over ks warps and cs CTAs
+    int chunk = 0;            // spans of x staged at a time
+};
+
+constexpr int kSms = 148;
+constexpr int kW4MaxSmem = 227 * 1024;
+// Spans in flight per warp (64 rows leave the ring less shared memory).
+constexpr int w4_depth(int nw, int nt) { return nw == 2 ? 4 : nt == 8 ? 5 : 6; }
+
+struct W4Plan {
+    int nt, rows, passes, ks, cs, chunk, gx, smem;
+};
+
+inline W4Plan w4_plan(int M, int T, int S, int pieces, int nw, int sms) {
+    W4Plan p{};
+    const int nt_max = nw == 2 ? 4 : 8;
+    const int most = nt_max * 8 / pieces;
+    p.passes = (M + most - 1) / most;
+    p.rows = (M + p.passes - 1) / p.passes;
+    const int vr = p.rows * pieces;
+    p.nt = vr <= 8 ? 1 : vr <= 16 ? 2 : vr <= 32 ? 4 : 8;
+    // warps that share a tile's spans: as many as keep every warp of two
+    // CTAs per SM busy, no more than there are spans
+    const int share = std::max(1, std::min(S, sms * 16 / std::max(1, T * p.passes)));
+    p.ks = share >= 8 ? 8 : share >= 4 ? 4 : share >= 2 ? 2 : 1;
+    p.cs = share >= 64 ? 8 : share >= 32 ? 4 : share >= 16 ? 2 : 1;
+    const int fixed = 8 * (w4_depth(nw, p.nt) * nw * 1216 + nw * p.nt * 8 * 20 * 4);
+    const int spans = (S + p.cs - 1) / p.cs;
+    // staged spans: all of the CTA's, or a multiple of ks that fits
+    const int fit = ((kW4MaxSmem - fixed) / (vr * 2) - 32) / 128;
+    while (p.ks > fit) p.ks /= 2;
+    p.chunk = spans <= fit ? (spans + p.ks - 1) / p.ks * p.ks : fit / p.ks * p.ks;
+    if (p.chunk > fit) p.chunk = spans;
+    p.smem = fixed + vr * (p.chunk * 128 + 32) * 2;
+    const int groups = (T + 8 / p.ks - 1) / (8 / p.ks);
+    const int per_sm = p.smem <= 113 * 1024 ? 2 : 1;
+    const int cap = std::max(1, sms * per_sm / (p.passes * p.cs));
+    const int rounds = (groups + cap - 1) / cap;
+    p.gx = (groups + rounds - 1) / rounds;
+    return p;
+}
+
+cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, bool pdl, cudaStream_t st);
+cudaError_t launch_w4_quantize(const w4_matrix& m, const void* w, int dtype, long long ldw, cudaStream_t st);
+cudaError_t launch_w4_dequantize(const w4_matrix& m, float* out, long long ldo, cudaStream_t st);
+cudaError_t launch_logits(const logits_call& c, cudaStream_t st);
+
+}  // namespace kvattn

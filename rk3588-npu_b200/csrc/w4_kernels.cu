@@ -1,0 +1,589 @@
+// w4_kernels.cu -- projections with 4-bit weights (w4_matrix of step_ops.h):
+// the product, the gated feed-forward block on two of them, and the kernels
+// that bring a matrix to 4 bits and back.
+//
+// Product: y^T = W x^T as mma.sync m16n8k16 tiles, W the A operand (16 weight
+// rows x 16 inputs), up to 64 rows of x the B operand.  With
+//   y[m][n] = sum_g s[n][g] * (sum_{k in g} (q[n][k] - z[n][g]) x[m][k])
+// the integers q - z are exact in fp16 and in bf16, so the tensor core sums
+// exact products in fp32 within a group, and the group's scale multiplies
+// the fp32 sum: no weight is ever rounded.  What x is, is the only choice of
+// the operand type: fp16 as fp16, bf16 as bf16, and an fp32 row as three
+// bf16 rows (its first, second and third 8 significant bits) whose products
+// are added at the end, so one fp32 row costs no more than three of the 8
+// columns that a tile has anyway.
+//
+// A nibble becomes an operand without a conversion: or-ed under the exponent
+// of 1024 (fp16; 128 for bf16) it is 1024 + q, from which 1024 + z is
+// subtracted exactly; the nibble above it is 1024 + 16 q, brought back by one
+// fused multiply-add.  Two weights per instruction.
+//
+// Bound: the codes' bytes for few rows.  Each lane copies the 32 bytes of
+// codes that it will unpack itself to its own slots of a ring in shared memory
+// (cp.async, kDepth spans ahead, across tiles), so loads never wait for the
+// math and need no barrier; a warp's 16 rows x 128 inputs are one contiguous
+// KiB in memory.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "device_common.cuh"
+#include "kvattn.h"
+#include "kvattn_internal.h"
+#include "projection.cuh"
+#include "step_ops.h"
+#include "w4_internal.h"
+
+namespace kvattn {
+
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kSlot = 1024 + 128 + 64;  // a span of one tile: codes, up to 4 groups' scales and zero points
+constexpr int kRedLd = 20;              // floats per column of a reduced tile: 16 rows, padded against bank conflicts
+
+// ------------------------------------------------------------------ unpacking
+// The zero point z as the constants of unpack().
+template <int BF>
+__device__ __forceinline__ uint2 zero_consts(uint32_t z) {
+    if (BF) return make_uint2((0x4300u | z) * 0x10001u, 0u);
+    const __half2 h = __float2half2_rn(-(float)(64 + (int)z));
+    return make_uint2((0x6400u | z) * 0x10001u, *reinterpret_cast<const uint32_t*>(&h));
+}
+
+// Eight codes minus their zero point as four pairs of fp16 / bf16 values, in
+// input order.
+template <int BF>
+__device__ __forceinline__ void unpack(uint32_t w, uint2 zc, uint32_t (&p)[4]) {
+    if (BF) {
+        const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&zc.x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+            const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), z);
+            p[i] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+    } else {
+        const __half2 z = *reinterpret_cast<const __half2*>(&zc.x), z16 = *reinterpret_cast<const __half2*>(&zc.y);
+        const __half2 sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t u = w >> (8 * i);
+            const uint32_t lo = (u & 0x000F000Fu) | 0x64006400u, hi = (u & 0x00F000F0u) | 0x64006400u;
+            const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), z);
+            const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, z16);
+            p[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+            p[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+    }
+}
+
+// ------------------------------------------------------------------- staging
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// 4 bytes, zeros where !there (the source is not read then).
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The three bf16 parts of an fp32 value, each with the next 8 significant
+// bits (the third rounded; exact for any value whose third part is normal).
+// Infinity and NaN stay in the first part alone.
+__device__ __forceinline__ void split3(float x, uint16_t& a, uint16_t& b, uint16_t& c) {
+    const uint32_t u = __float_as_uint(x);
+    if ((u & 0x7F800000u) == 0x7F800000u) {
+        a = (u & 0x007FFFFFu) ? 0x7FFFu : (uint16_t)(u >> 16);
+        b = c = 0;
+        return;
+    }
+    a = (uint16_t)(u >> 16);
+    const float r = x - __uint_as_float(u & 0xFFFF0000u);  // exact
+    const uint32_t v = __float_as_uint(r);
+    b = (uint16_t)(v >> 16);
+    const __nv_bfloat16 t = __float2bfloat16_rn(r - __uint_as_float(v & 0xFFFF0000u));
+    c = *reinterpret_cast<const uint16_t*>(&t);
+}
+
+// One warp stages inputs [k0, k0 + len) of x row `row` (len a multiple of
+// 128; zeros from K on) into xs, as fp16 or bf16 codes: one row, or with
+// W4_X_F32 three rows `ld` halves apart.  `wide`: x rows are 16-byte aligned.
+__device__ __forceinline__ void stage(const W4Args& a, int row, int k0, int len, uint16_t* xs, int ld, bool wide) {
+    const int lane = threadIdx.x & 31, K = a.K;
+    if (a.in == W4_X_16) {
+        const uint16_t* src = static_cast<const uint16_t*>(a.x) + (size_t)row * a.ldx + k0;
+        for (int i = lane * 8; i < len; i += 256) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (wide && k0 + i + 8 <= K) {
+                v = __ldg(reinterpret_cast<const uint4*>(src + i));
+            } else {
+                uint32_t h[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[j] = k0 + i + j < K ? (uint32_t)__ldg(src + i + j) : 0u;
+                v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+            }
+            *reinterpret_cast<uint4*>(xs + i) = v;
+        }
+        return;
+    }
+    const float* xr = static_cast<const float*>(a.x) + (size_t)row * a.ldx;
+    float inv = 1.f;
+    if (a.in == W4_X_NORM) {
+        // 1 / rms of the whole row (op_rmsnorm.cpp:12-15)
+        float s = 0.f;
+        for (int i = lane * 4; i < K; i += 128) s = sum_sq4(s, __ldg(reinterpret_cast<const float4*>(xr + i)));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(s, (float)K), a.g.eps)));
+    }
+    for (int i = lane * 4; i < len; i += 128) {
+        float v[4];
+        if (wide && k0 + i + 4 <= K) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(xr + k0 + i));
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = k0 + i + j < K ? __ldg(xr + k0 + i + j) : 0.f;
+        }
+        if (a.in == W4_X_F32) {
+            uint16_t p[3][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) split3(v[j], p[0][j], p[1][j], p[2][j]);
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+                *reinterpret_cast<uint2*>(xs + q * ld + i) =
+                    make_uint2(p[q][0] | (uint32_t)p[q][1] << 16, p[q][2] | (uint32_t)p[q][3] << 16);
+        } else {
+            // the reference's fp16 (f32_to_f16 before every projection), after
+            // the norm (op_rmsnorm.cpp:17-18) where there is one
+            if (a.in == W4_X_NORM) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (k0 + i + j < K) v[j] = __fmul_rn(__fmul_rn(v[j], inv), __ldg(a.g.norm_w + k0 + i + j));
+            }
+            *reinterpret_cast<uint2*>(xs + i) =
+                make_uint2(enc_f16_trunc(v[0]) | (uint32_t)enc_f16_trunc(v[1]) << 16,
+                           enc_f16_trunc(v[2]) | (uint32_t)enc_f16_trunc(v[3]) << 16);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ epilogue
+__device__ __forceinline__ float load_as(const void* p, size_t i, int dtype) {
+    if (dtype == STEP_F32) return static_cast<const float*>(p)[i];
+    if (dtype == STEP_F16) return __half2float(static_cast<const __half*>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_as(void* p, size_t i, int dtype, float v) {
+    if (dtype == STEP_F32) static_cast<float*>(p)[i] = v;
+    else if (dtype == STEP_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ void epilogue(const W4Args& a, int row, int n, float y, float y2) {
+    switch (a.mode) {
+        case W4_QKV: gemv_epilogue<0>(a.g, row, n, y, y2); break;
+        case W4_RESID: gemv_epilogue<1>(a.g, row, n, y, y2); break;
+        case W4_GATE_UP: gemv_epilogue<2>(a.g, row, n, y, y2); break;
+        case W4_LOGITS: gemv_epilogue<3>(a.g, row, n, y, y2); break;
+        case W4_LINEAR:
+            if (a.bias) y += __ldg(a.bias + n);
+            if (a.residual) y += load_as(a.residual, (size_t)row * a.ldr + n, a.out_dtype);
+            store_as(a.out, (size_t)row * a.ldo + n, a.out_dtype, y);
+            break;
+        default:
+            store_as(a.out, (size_t)row * a.ldo + n, a.out_dtype, __fdiv_rn(y, 1.0f + expf(-y)) * y2);
+    }
+}
+
+// BF: bf16 operands (else fp16).  NT: n8 tiles of x rows per pass.  NW: 2 for
+// the gated block.  GP: groups per span (1, 2 or 4).
+//
+// CTA (cluster rank r of cs, pass blockIdx.y): spans [S r / cs, S (r + 1) / cs)
+// of kWarps / ks tiles at a time; warp w takes tile w / ks and every ks-th
+// span from w % ks on.  The warps' and the cluster's partial tiles are added
+// in a fixed order (through shared memory, other CTAs' by DSMEM), so results
+// do not depend on timing.
+template <int BF, int NT, int NW, int GP>
+__global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
+    w4_kernel(const __grid_constant__ W4Args a) {
+    constexpr int kDepth = w4_depth(NW, NT);
+    constexpr int kCols = NT * 8;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int ks = a.ks, tpc = kWarps / ks, sub = warp / ks, part = warp % ks;
+    const int cs = a.cs, rank = (int)blockIdx.x % cs;
+    const int m0 = blockIdx.y * a.rows, mrows = min(a.rows, a.M - m0), vr = mrows * a.pieces;
+    const int ldx = a.chunk * 128 + 32;  // halves per staged row: an odd number of 64-byte units
+    uint16_t* xs = reinterpret_cast<uint16_t*>(smem);
+    uint8_t* ring = smem + (size_t)a.rows * a.pieces * ldx * 2 + (size_t)warp * (kDepth * NW * kSlot);
+    float* red = reinterpret_cast<float*>(smem + (size_t)a.rows * a.pieces * ldx * 2 + kWarps * kDepth * NW * kSlot);
+
+    const int s0 = (int)((long long)a.S * rank / cs), s1 = (int)((long long)a.S * (rank + 1) / cs);
+    const int groups = (a.T + tpc - 1) / tpc;
+    const int rg0 = (int)blockIdx.x / cs, rstep = (int)gridDim.x / cs;
+    const int nmax = (s1 - s0 + ks - 1) / ks;                              // spans per warp, at most
+    const int nmine = s0 + part < s1 ? (s1 - s0 - part + ks - 1) / ks : 0;  // this warp's
+    const uint32_t ring_s = smem_u32(ring);
+
+    // the warp's (tile, span) sequence, kDepth - 1 ahead of the math
+    int pr = rg0, pi = 0, pslot = 0;
+    auto issue = [&]() {
+        if (nmine > 0 && pr < groups) {
+            const int tile = pr * tpc + sub;
+            if (tile < a.T) {
+                const int sp = s0 + part + pi * ks;
+#pragma unroll
+                for (int q = 0; q < NW; ++q) {
+                    const uint32_t dst = ring_s + (pslot * NW + q) * kSlot;
+                    const uint8_t* src = reinterpret_cast<const uint8_t*>(a.codes[q]) + ((size_t)tile * a.S + sp) * 1024;
+                    cp16(dst + lane * 16, src + lane * 16);
+                    cp16(dst + 512 + lane * 16, src + 512 + lane * 16);
+                    const int gi = sp * GP + (lane >> 3);
+                    if (lane < GP * 8)
+                        cp4(dst + 1024 + lane * 4,
+                            reinterpret_cast<const uint8_t*>(a.scales[q]) + ((size_t)tile * a.Q + min(gi, a.Q - 1)) * 32 + (lane & 7) * 4,
+                            gi < a.Q);
+                    if (a.zeros[q] && lane < GP * 4) {
+                        const int gz = sp * GP + (lane >> 2);
+                        cp4(dst + 1152 + lane * 4, a.zeros[q] + ((size_t)tile * a.Q + min(gz, a.Q - 1)) * 16 + (lane & 3) * 4, gz < a.Q);
+                    }
+                }
+            }
+            if (++pi == nmine) {
+                pi = 0;
+                pr += rstep;
+            }
+        }
+        cp_commit();
+        pslot = pslot + 1 == kDepth ? 0 : pslot + 1;
+    };
+
+    // Launched as a programmatic dependent in the model's chain: the weights,
+    // which no kernel of the chain writes, are fetched before the wait.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kDepth - 1; ++i) issue();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const bool wide = (reinterpret_cast<size_t>(a.x) & 15) == 0 && (a.ldx * (a.in == W4_X_16 ? 2 : 4)) % 16 == 0;
+    const int chunks = (s1 - s0 + a.chunk - 1) / a.chunk;
+    auto stage_chunk = [&](int ch) {
+        const int b = s0 + ch * a.chunk, e = min(b + a.chunk, s1);
+        for (int m = warp; m < mrows; m += kWarps)
+            stage(a, m0 + m, b * 128, (e - b) * 128, xs + (size_t)m * a.pieces * ldx, ldx, wide);
+    };
+    const int per_chunk = a.chunk / ks;  // steps of a warp per staged chunk (chunk is a multiple of ks, or holds every span)
+    if (chunks == 1) {
+        stage_chunk(0);
+        __syncthreads();
+    }
+
+    int slot = 0;
+#pragma unroll 1
+    for (int rg = rg0; rg < groups; rg += rstep) {
+        const bool live = rg * tpc + sub < a.T;
+        float acc[NW][NT][4];
+#pragma unroll
+        for (int q = 0; q < NW; ++q)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[q][t][0] = acc[q][t][1] = acc[q][t][2] = acc[q][t][3] = 0.f;
+#pragma unroll 1
+        for (int it = 0; it < nmax; ++it) {
+            if (chunks > 1 && it % per_chunk == 0) {
+                __syncthreads();
+                stage_chunk(it / per_chunk);
+                __syncthreads();
+            }
+            if (it >= nmine) continue;
+            cp_wait<kDepth - 2>();
+            __syncwarp();  // the span's scales came by other lanes; the slot refilled next was read by all of them
+            issue();
+            if (live) {
+                const int xo = (part + it * ks) % a.chunk * 128;  // the span within the staged chunk
+                uint32_t w[NW][8][4];  // A operands: steps of 16 inputs
+                float2 sc[NW][GP];     // scales of rows g and g + 8
+#pragma unroll
+                for (int q = 0; q < NW; ++q) {
+                    const uint8_t* sl = ring + (slot * NW + q) * kSlot;
+                    const uint4 lo4 = *reinterpret_cast<const uint4*>(sl + lane * 16);
+                    const uint4 hi4 = *reinterpret_cast<const uint4*>(sl + 512 + lane * 16);
+                    const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+                    uint2 zl, zh;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j % (4 / GP) == 0) {
+                            const int gq = j / (4 / GP);
+                            sc[q][gq] = __half22float2(*reinterpret_cast<const __half2*>(sl + 1024 + gq * 32 + g * 4));
+                            uint32_t z = 0x0808u;
+                            if (a.zeros[q]) z = *reinterpret_cast<const uint16_t*>(sl + 1152 + gq * 16 + g * 2);
+                            zl = zero_consts<BF>(z & 15u);
+                            zh = zero_consts<BF>((z >> 8) & 15u);
+                        }
+                        uint32_t p[4], r[4];
+                        unpack<BF>(lo[j], zl, p);
+                        unpack<BF>(hi[j], zh, r);
+                        w[q][2 * j][0] = p[0], w[q][2 * j][1] = r[0], w[q][2 * j][2] = p[1], w[q][2 * j][3] = r[1];
+                        w[q][2 * j + 1][0] = p[2], w[q][2 * j + 1][1] = r[2], w[q][2 * j + 1][2] = p[3], w[q][2 * j + 1][3] = r[3];
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if (t * 8 >= vr) break;
+                    // columns from vr on hold some row's values and are not read
+                    const uint16_t* xr = xs + (size_t)min(t * 8 + g, vr - 1) * ldx + xo + 8 * c;
+                    float d[NW][4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 b = *reinterpret_cast<const uint4*>(xr + 32 * j);
+#pragma unroll
+                        for (int q = 0; q < NW; ++q) {
+                            if (j % (4 / GP) == 0) d[q][0] = d[q][1] = d[q][2] = d[q][3] = 0.f;
+                            mma16816<BF>(d[q], w[q][2 * j][0], w[q][2 * j][1], w[q][2 * j][2], w[q][2 * j][3], b.x, b.y);
+                            mma16816<BF>(d[q], w[q][2 * j + 1][0], w[q][2 * j + 1][1], w[q][2 * j + 1][2], w[q][2 * j + 1][3], b.z, b.w);
+                            if ((j + 1) % (4 / GP) == 0) {
+                                const float2 s = sc[q][j / (4 / GP)];
+                                acc[q][t][0] = fmaf(s.x, d[q][0], acc[q][t][0]);
+                                acc[q][t][1] = fmaf(s.x, d[q][1], acc[q][t][1]);
+                                acc[q][t][2] = fmaf(s.y, d[q][2], acc[q][t][2]);
+                                acc[q][t][3] = fmaf(s.y, d[q][3], acc[q][t][3]);
+                            }
+                        }
+                    }
+                }
+            }
+            slot = slot + 1 == kDepth ? 0 : slot + 1;
+        }
+        // partial tiles of this warp: [matrix][column][row]
+        if (live) {
+#pragma unroll
+            for (int q = 0; q < NW; ++q)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        red[((warp * NW + q) * kCols + t * 8 + 2 * c + (i & 1)) * kRedLd + g + (i >> 1) * 8] = acc[q][t][i];
+        }
+        if (cs > 1) cluster_sync();
+        else __syncthreads();
+        const int total = tpc * mrows * 16;
+        for (int e = threadIdx.x + rank * kWarps * 32; e < total; e += cs * kWarps * 32) {
+            const int n16 = e & 15, m = (e >> 4) % mrows, ts = (e >> 4) / mrows;
+            const int n = (rg * tpc + ts) * 16 + n16;
+            if (n >= a.N) continue;
+            float y[2] = {0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < NW; ++q) {
+                for (int p = a.pieces - 1; p >= 0; --p) {  // the smallest parts first
+                    const int at = (q * kCols + m * a.pieces + p) * kRedLd + n16;
+                    for (int r = 0; r < cs; ++r) {
+                        const uint32_t base = cs > 1 ? cluster_map(smem_u32(red), r) : 0u;
+                        for (int u = 0; u < ks; ++u) {
+                            const int o = (ts * ks + u) * NW * kCols * kRedLd + at;
+                            y[q] += cs > 1 ? ld_cluster_f32(base + o * 4) : red[o];
+                        }
+                    }
+                }
+            }
+            epilogue(a, m0 + m, n, y[0], y[1]);
+        }
+        if (cs > 1) cluster_sync();  // red is written again, or this CTA ends, only when nobody reads it
+        else __syncthreads();
+    }
+    cp_wait<0>();
+}
+
+// ------------------------------------------------------- to 4 bits and back
+// One warp per (tile, span); lane (g, c) holds rows g and g + 8, inputs
+// 32 j + 8 c + i.  The group statistics are maxima, exact in any order.
+template <class T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <class T>
+__global__ void __launch_bounds__(256)
+    w4_quantize_kernel(const T* __restrict__ w, long long ldw, int N, int K, int T_, int S, int Q, int jg /* words per group */,
+                       uint32_t* __restrict__ codes, __half* __restrict__ scales, uint8_t* __restrict__ zeros) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (id >= (long long)T_ * S) return;
+    const int t = (int)(id / S), s = (int)(id % S);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int n = t * 16 + h * 8 + g;
+        float v[4][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int k = s * 128 + 32 * j + 8 * c + i;
+                v[j][i] = n < N && k < K ? to_f(w[(size_t)n * ldw + k]) : 0.f;
+            }
+        uint32_t word[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float lo = 0.f, hi = 0.f;
+            const int j0 = j / jg * jg;
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj)
+                if (jj >= j0 && jj < j0 + jg) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        lo = fminf(lo, v[jj][i]);
+                        hi = fmaxf(hi, v[jj][i]);
+                    }
+                }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+            const float span = zeros ? __fdiv_rn(__fsub_rn(hi, lo), 15.0f) : __fdiv_rn(fmaxf(-lo, hi), 7.0f);
+            const __half sh = __float2half_rn(span);
+            const float sc = __half2float(sh);
+            const bool some = sc > 0.f;
+            const float z = zeros && some ? fminf(fmaxf(rintf(__fdiv_rn(-lo, sc)), 0.f), 15.f) : 8.f;
+            uint32_t q = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float r = some ? __fadd_rn(rintf(__fdiv_rn(v[j][i], sc)), z) : z;
+                q |= (uint32_t)fminf(fmaxf(r, 0.f), 15.f) << (4 * ((i >> 1) + 4 * (i & 1)));
+            }
+            word[j] = q;
+            const int gi = s * (4 / jg) + j / jg;
+            if (j == j0 && c == 0 && gi < Q) {
+                const size_t at = (((size_t)t * Q + gi) * 8 + g) * 2 + h;
+                scales[at] = sh;
+                if (zeros) zeros[at] = (uint8_t)z;
+            }
+        }
+        reinterpret_cast<uint4*>(codes)[(id * 2 + h) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+    }
+}
+
+__global__ void __launch_bounds__(256)
+    w4_dequantize_kernel(const uint32_t* __restrict__ codes, const __half* __restrict__ scales,
+                         const uint8_t* __restrict__ zeros, int N, int K, int T_, int S, int Q, int jg,
+                         float* __restrict__ out, long long ldo) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (id >= (long long)T_ * S) return;
+    const int t = (int)(id / S), s = (int)(id % S);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int n = t * 16 + h * 8 + g;
+        const uint4 w4 = reinterpret_cast<const uint4*>(codes)[(id * 2 + h) * 32 + lane];
+        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        if (n >= N) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int gi = s * (4 / jg) + j / jg;
+            if (gi >= Q) continue;
+            const size_t at = (((size_t)t * Q + gi) * 8 + g) * 2 + h;
+            const float sc = __half2float(scales[at]), z = zeros ? (float)(zeros[at] & 15) : 8.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int k = s * 128 + 32 * j + 8 * c + i;
+                if (k < K)
+                    out[(size_t)n * ldo + k] = ((float)((w[j] >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) - z) * sc;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ launching
+template <int BF, int NT, int NW, int GP>
+cudaError_t launch_inst(const W4Args& a, int gx, int passes, int smem, bool pdl, cudaStream_t st) {
+    auto fn = w4_kernel<BF, NT, NW, GP>;
+    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kW4MaxSmem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(gx * a.cs), (unsigned)passes);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (a.cs > 1) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = (unsigned)a.cs;
+        attr[na].val.clusterDim.y = 1;
+        attr[na].val.clusterDim.z = 1;
+        ++na;
+    }
+    if (pdl) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na].val.programmaticStreamSerializationAllowed = 1;
+        ++na;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    return counted(cudaLaunchKernelEx(&cfg, fn, a));
+}
+
+template <int BF, int NT, int NW>
+cudaError_t launch_gp(const W4Args& a, int group, int gx, int passes, int smem, bool pdl, cudaStream_t st) {
+    if (group == 128) return launch_inst<BF, NT, NW, 1>(a, gx, passes, smem, pdl, st);
+    if (group == 64) return launch_inst<BF, NT, NW, 2>(a, gx, passes, smem, pdl, st);
+    return launch_inst<BF, NT, NW, 4>(a, gx, passes, smem, pdl, st);
+}
+
+template <int BF>
+cudaError_t launch_nt(const W4Args& a, int nt, int nw, int group, int gx, int passes, int smem, bool pdl, cudaStream_t st) {
+    if (nw == 2) {
+        if (nt == 1) return launch_gp<BF, 1, 2>(a, group, gx, passes, smem, pdl, st);
+        if (nt == 2) return launch_gp<BF, 2, 2>(a, group, gx, passes, smem, pdl, st);
+        return launch_gp<BF, 4, 2>(a, group, gx, passes, smem, pdl, st);
+    }
+    if (nt == 1) return launch_gp<BF, 1, 1>(a, group, gx, passes, smem, pdl, st);
+    if (nt == 2) return launch_gp<BF, 2, 1>(a, group, gx, passes, smem, pdl, st);
+    if (nt == 4) return launch_gp<BF, 4, 1>(a, group, gx, passes, smem, pdl, st);
+    return launch_gp<BF, 8, 1>(a, group, gx, passes, smem, pdl, st);
+}
+
+}  // namespace
+
+cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, bool pdl, cudaStream_t st) {
+    const W4Plan p = w4_plan(a.M, a.T, a.S, a.pieces, nw, kSms);
+    a.rows = p.rows;
+    a.ks = p.ks;
+    a.cs = p.cs;
+    a.chunk = p.chunk;
+    return bf ? launch_nt<1>(a, p.nt, nw, group, p.gx, p.passes, p.smem, pdl, st)
+              : launch_nt<0>(a, p.nt, nw, group, p.gx, p.passes, p.smem, pdl, st);
+}
+
+cudaError_t launch_w4_quantize(const w4_matrix& m, const void* w, int dtype, long long ldw, cudaStream_t st) {
+    const int T = (m.n + 15) / 16, S = (m.k + 127) / 128, Q = (m.k + m.group - 1) / m.group, jg = m.group / 32;
+    const long long blocks = ((long long)T * S + 7) / 8;
+    if (dtype == STEP_F16)
+        w4_quantize_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const __half*>(w), ldw, m.n, m.k, T, S, Q, jg,
+                                                             static_cast<uint32_t*>(m.codes), static_cast<__half*>(m.scales),
+                                                             static_cast<uint8_t*>(m.zeros));
+    else
+        w4_quantize_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(w), ldw, m.n, m.k, T, S, Q, jg,
+                                                             static_cast<uint32_t*>(m.codes), static_cast<__half*>(m.scales),
+                                                             static_cast<uint8_t*>(m.zeros));
+    return counted(cudaGetLastError());
+}
+
+cudaError_t launch_w4_dequantize(const w4_matrix& m, float* out, long long ldo, cudaStream_t st) {
+    const int T = (m.n + 15) / 16, S = (m.k + 127) / 128, Q = (m.k + m.group - 1) / m.group, jg = m.group / 32;
+    const long long blocks = ((long long)T * S + 7) / 8;
+    w4_dequantize_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const uint32_t*>(m.codes),
+                                                           static_cast<const __half*>(m.scales),
+                                                           static_cast<const uint8_t*>(m.zeros), m.n, m.k, T, S, Q, jg, out, ldo);
+    return counted(cudaGetLastError());
+}
+
+}  // namespace kvattn
