@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 struct kvx_exch;  // split-KV exchange object of the C ABI (xgpu_exchange.cu)
 struct kvn_comm;  // split-KV NCCL communicator of the C ABI (nccl_split.cu)
 struct kvp_pool;  // paged pool of the C ABI (kvattn_host.cu)
@@ -308,9 +310,26 @@ struct DeviceGuard {
         if (dev < 0) return;  // host-only object: no device calls
         if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
         if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
+        else prev = -1;  // nothing to restore
     }
     ~DeviceGuard() {
         if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+// Raises a kernel's dynamic shared memory limit once per device.
+struct SmemGrant {
+    static constexpr int kDevices = 64;
+    std::atomic<bool> done[kDevices];
+    cudaError_t raise(const void* fn, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev < 0 || dev >= kDevices) return cudaErrorInvalidDevice;
+        if (done[dev].load()) return cudaSuccess;
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done[dev].store(true);
+        return e;
     }
 };
 

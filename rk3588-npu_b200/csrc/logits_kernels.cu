@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(kThreads)
 template <class T>
 cudaError_t launch_t(const logits_call& c, cudaStream_t st) {
     const int smem = (c.hist ? kChunk * 4 : 0) + (c.bias_ids ? kChunk * 4 : 0);
-    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(logits_kernel<T>),
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kChunk * 4);
+    static SmemGrant grant;
+    const cudaError_t e = grant.raise(reinterpret_cast<const void*>(logits_kernel<T>), 2 * kChunk * 4);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(kCluster, (unsigned)c.rows);

@@ -163,7 +163,7 @@ int w4_linear(const w4_matrix* w, const void* x, int x_dtype, int m, long long l
     a.out = out;
     a.out_dtype = out_dtype;
     a.ldo = ldo;
-    return launched(launch_w4(a, w->group, x_dtype != STEP_F16, 1, false, static_cast<cudaStream_t>(stream)), "w4_linear");
+    return launched(launch_w4(a, w->group, x_dtype != STEP_F16, 1, static_cast<cudaStream_t>(stream)), "w4_linear");
 }
 
 int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dtype, int m, long long ldx, void* out,
@@ -185,7 +185,7 @@ int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dt
     a.out = out;
     a.out_dtype = out_dtype;
     a.ldo = ldo;
-    return launched(launch_w4(a, gate->group, x_dtype != STEP_F16, 2, false, static_cast<cudaStream_t>(stream)), "w4_gated");
+    return launched(launch_w4(a, gate->group, x_dtype != STEP_F16, 2, static_cast<cudaStream_t>(stream)), "w4_gated");
 }
 
 int logits_adjust(const logits_call* c, void* stream) {

@@ -41,12 +41,18 @@ struct W4Args {
     int rows = 0;             // x rows per pass
     int ks = 1, cs = 1;       // a tile's spans over ks warps and cs CTAs
     int chunk = 0;            // spans of x staged at a time
+    int last_groups = 0;      // groups of a row's last span
+    bool early = false;       // the weights may be read before the previous kernel of the stream ends
 };
 
 constexpr int kSms = 148;
 constexpr int kW4MaxSmem = 227 * 1024;
 // Spans in flight per warp (64 rows leave the ring less shared memory).
 constexpr int w4_depth(int nw, int nt) { return nw == 2 ? 4 : nt == 8 ? 5 : 6; }
+
+// Floats of a warp's partial tile: 20 per column (16 rows, padded against bank
+// conflicts), 4 more so that the warps' tiles start in different banks.
+constexpr int w4_red_floats(int nw, int nt) { return nw * nt * 8 * 20 + 4; }
 
 struct W4Plan {
     int nt, rows, passes, ks, cs, chunk, gx, smem;
@@ -65,7 +71,7 @@ inline W4Plan w4_plan(int M, int T, int S, int pieces, int nw, int sms) {
     const int share = std::max(1, std::min(S, sms * 16 / std::max(1, T * p.passes)));
     p.ks = share >= 8 ? 8 : share >= 4 ? 4 : share >= 2 ? 2 : 1;
     p.cs = share >= 64 ? 8 : share >= 32 ? 4 : share >= 16 ? 2 : 1;
-    const int fixed = 8 * (w4_depth(nw, p.nt) * nw * 1216 + nw * p.nt * 8 * 20 * 4);
+    const int fixed = 8 * (w4_depth(nw, p.nt) * nw * 1216 + w4_red_floats(nw, p.nt) * 4);
     const int spans = (S + p.cs - 1) / p.cs;
     // staged spans: all of the CTA's, or a multiple of ks that fits
     const int fit = ((kW4MaxSmem - fixed) / (vr * 2) - 32) / 128;
@@ -74,14 +80,12 @@ inline W4Plan w4_plan(int M, int T, int S, int pieces, int nw, int sms) {
     if (p.chunk > fit) p.chunk = spans;
     p.smem = fixed + vr * (p.chunk * 128 + 32) * 2;
     const int groups = (T + 8 / p.ks - 1) / (8 / p.ks);
-    const int per_sm = p.smem <= 113 * 1024 ? 2 : 1;
-    const int cap = std::max(1, sms * per_sm / (p.passes * p.cs));
-    const int rounds = (groups + cap - 1) / cap;
-    p.gx = (groups + rounds - 1) / rounds;
+    const int per_sm = p.smem <= 113 * 1024 && p.nt * nw <= 2 ? 2 : 1;
+    p.gx = std::min(groups, std::max(1, sms * per_sm / (p.passes * p.cs)));
     return p;
 }
 
-cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, bool pdl, cudaStream_t st);
+cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st);
 cudaError_t launch_w4_quantize(const w4_matrix& m, const void* w, int dtype, long long ldw, cudaStream_t st);
 cudaError_t launch_w4_dequantize(const w4_matrix& m, float* out, long long ldo, cudaStream_t st);
 cudaError_t launch_logits(const logits_call& c, cudaStream_t st);

@@ -83,9 +83,8 @@ __device__ __forceinline__ void unpack(uint32_t w, uint2 zc, uint32_t (&p)[4]) {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// 4 bytes, zeros where !there (the source is not read then).
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -111,65 +110,100 @@ __device__ __forceinline__ void split3(float x, uint16_t& a, uint16_t& b, uint16
     c = *reinterpret_cast<const uint16_t*>(&t);
 }
 
-// One warp stages inputs [k0, k0 + len) of x row `row` (len a multiple of
-// 128; zeros from K on) into xs, as fp16 or bf16 codes: one row, or with
-// W4_X_F32 three rows `ld` halves apart.  `wide`: x rows are 16-byte aligned.
-__device__ __forceinline__ void stage(const W4Args& a, int row, int k0, int len, uint16_t* xs, int ld, bool wide) {
-    const int lane = threadIdx.x & 31, K = a.K;
-    if (a.in == W4_X_16) {
-        const uint16_t* src = static_cast<const uint16_t*>(a.x) + (size_t)row * a.ldx + k0;
-        for (int i = lane * 8; i < len; i += 256) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (wide && k0 + i + 8 <= K) {
-                v = __ldg(reinterpret_cast<const uint4*>(src + i));
-            } else {
-                uint32_t h[8];
+// The x rows of a pass, inputs [k0, k0 + len) (len a multiple of 128; zeros
+// from K on), staged into xs as operand codes by the whole CTA: row m at m *
+// pieces * ld halves, an fp32 row as its three parts `ld` apart.  8 / mrows
+// warps share a row; a warp's loads of a batch are all issued before any is
+// used, and 16-bit rows go by cp.async (the caller waits).  `wide`: rows of x
+// are 16-byte aligned.
+__device__ __forceinline__ void stage_rows(const W4Args& a, int m0, int mrows, int k0, int len, uint16_t* xs, int ld,
+                                           bool wide) {
+    constexpr int kU = 4;  // 16-byte loads in flight per lane
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = a.K;
+    const int wpr = mrows >= 8 ? 1 : mrows > 4 ? 1 : mrows > 2 ? 2 : mrows > 1 ? 4 : 8;
+    const int first = (warp % wpr) * 32 + lane, step = wpr * 32;
+    for (int m = warp / wpr; m < mrows; m += kWarps / wpr) {
+        if (a.in == W4_X_16) {
+            const uint16_t* src = static_cast<const uint16_t*>(a.x) + (size_t)(m0 + m) * a.ldx + k0;
+            uint16_t* dst = xs + (size_t)m * ld;
+            for (int i = first * 8; i < len; i += step * 8) {
+                if (wide && k0 + i + 8 <= K) {
+                    cp16(smem_u32(dst + i), src + i);
+                } else {
+                    uint32_t h[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[j] = k0 + i + j < K ? (uint32_t)__ldg(src + i + j) : 0u;
-                v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                    for (int j = 0; j < 8; ++j) h[j] = k0 + i + j < K ? (uint32_t)__ldg(src + i + j) : 0u;
+                    *reinterpret_cast<uint4*>(dst + i) =
+                        make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                }
             }
-            *reinterpret_cast<uint4*>(xs + i) = v;
+            continue;
         }
-        return;
-    }
-    const float* xr = static_cast<const float*>(a.x) + (size_t)row * a.ldx;
-    float inv = 1.f;
-    if (a.in == W4_X_NORM) {
-        // 1 / rms of the whole row (op_rmsnorm.cpp:12-15)
-        float s = 0.f;
-        for (int i = lane * 4; i < K; i += 128) s = sum_sq4(s, __ldg(reinterpret_cast<const float4*>(xr + i)));
+        const float* xr = static_cast<const float*>(a.x) + (size_t)(m0 + m) * a.ldx;
+        uint16_t* dst = xs + (size_t)m * a.pieces * ld;
+        float inv = 1.f;
+        if (a.in == W4_X_NORM) {
+            // 1 / rms of the whole row (op_rmsnorm.cpp:12-15), by each of its warps
+            float s = 0.f;
+            for (int i = lane * 4; i < K; i += 128 * 6) {
+                float4 v[6];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(s, (float)K), a.g.eps)));
-    }
-    for (int i = lane * 4; i < len; i += 128) {
-        float v[4];
-        if (wide && k0 + i + 4 <= K) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(xr + k0 + i));
-            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-        } else {
+                for (int u = 0; u < 6; ++u)
+                    if (i + u * 128 < K) v[u] = __ldg(reinterpret_cast<const float4*>(xr + i + u * 128));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = k0 + i + j < K ? __ldg(xr + k0 + i + j) : 0.f;
-        }
-        if (a.in == W4_X_F32) {
-            uint16_t p[3][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) split3(v[j], p[0][j], p[1][j], p[2][j]);
-#pragma unroll
-            for (int q = 0; q < 3; ++q)
-                *reinterpret_cast<uint2*>(xs + q * ld + i) =
-                    make_uint2(p[q][0] | (uint32_t)p[q][1] << 16, p[q][2] | (uint32_t)p[q][3] << 16);
-        } else {
-            // the reference's fp16 (f32_to_f16 before every projection), after
-            // the norm (op_rmsnorm.cpp:17-18) where there is one
-            if (a.in == W4_X_NORM) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (k0 + i + j < K) v[j] = __fmul_rn(__fmul_rn(v[j], inv), __ldg(a.g.norm_w + k0 + i + j));
+                for (int u = 0; u < 6; ++u)
+                    if (i + u * 128 < K) s = sum_sq4(s, v[u]);
             }
-            *reinterpret_cast<uint2*>(xs + i) =
-                make_uint2(enc_f16_trunc(v[0]) | (uint32_t)enc_f16_trunc(v[1]) << 16,
-                           enc_f16_trunc(v[2]) | (uint32_t)enc_f16_trunc(v[3]) << 16);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(s, (float)K), a.g.eps)));
+        }
+        for (int i0 = first * 4; i0 < len; i0 += step * 4 * kU) {
+            float4 f[kU], nw[kU];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int i = i0 + u * step * 4;
+                f[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < len) {
+                    const int k = k0 + i;
+                    if (wide && k + 4 <= K) {
+                        f[u] = __ldg(reinterpret_cast<const float4*>(xr + k));
+                        if (a.in == W4_X_NORM) nw[u] = __ldg(reinterpret_cast<const float4*>(a.g.norm_w + k));
+                    } else {  // the model's rows are always wide and whole
+                        if (k < K) f[u].x = __ldg(xr + k);
+                        if (k + 1 < K) f[u].y = __ldg(xr + k + 1);
+                        if (k + 2 < K) f[u].z = __ldg(xr + k + 2);
+                        if (k + 3 < K) f[u].w = __ldg(xr + k + 3);
+                        nw[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int i = i0 + u * step * 4;
+                if (i >= len) break;
+                float v[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
+                if (a.in == W4_X_F32) {
+                    uint16_t p[3][4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) split3(v[j], p[0][j], p[1][j], p[2][j]);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        *reinterpret_cast<uint2*>(dst + q * ld + i) =
+                            make_uint2(p[q][0] | (uint32_t)p[q][1] << 16, p[q][2] | (uint32_t)p[q][3] << 16);
+                } else {
+                    // the reference's fp16 (f32_to_f16 before every projection),
+                    // after the norm (op_rmsnorm.cpp:17-18) where there is one
+                    if (a.in == W4_X_NORM) {
+                        const float w[4] = {nw[u].x, nw[u].y, nw[u].z, nw[u].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], inv), w[j]);
+                    }
+                    *reinterpret_cast<uint2*>(dst + i) =
+                        make_uint2(enc_f16_trunc(v[0]) | (uint32_t)enc_f16_trunc(v[1]) << 16,
+                                   enc_f16_trunc(v[2]) | (uint32_t)enc_f16_trunc(v[3]) << 16);
+                }
+            }
         }
     }
 }
@@ -205,20 +239,24 @@ __device__ __forceinline__ void epilogue(const W4Args& a, int row, int n, float 
 // BF: bf16 operands (else fp16).  NT: n8 tiles of x rows per pass.  NW: 2 for
 // the gated block.  GP: groups per span (1, 2 or 4).
 //
-// CTA (cluster rank r of cs, pass blockIdx.y): spans [S r / cs, S (r + 1) / cs)
-// of kWarps / ks tiles at a time; warp w takes tile w / ks and every ks-th
-// span from w % ks on.  The warps' and the cluster's partial tiles are added
-// in a fixed order (through shared memory, other CTAs' by DSMEM), so results
-// do not depend on timing.
+// Work: CTA b of gx (cluster rank r of cs, pass blockIdx.y) takes the tiles
+// (i kWarps / ks + w / ks) gx + b, i = 0, 1, .., of its warps w, and of those
+// the spans [S r / cs, S (r + 1) / cs), warp w every ks-th from w % ks on.  So
+// what does not divide evenly is spread over different SMs.  The partial
+// tiles of ks warps and cs CTAs are added in a fixed order (shared memory,
+// other CTAs' by DSMEM): results do not depend on timing.  With ks = cs = 1
+// warps never wait for one another.
 template <int BF, int NT, int NW, int GP>
 __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     w4_kernel(const __grid_constant__ W4Args a) {
     constexpr int kDepth = w4_depth(NW, NT);
     constexpr int kCols = NT * 8;
+    constexpr int kRedWarp = w4_red_floats(NW, NT);
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int ks = a.ks, tpc = kWarps / ks, sub = warp / ks, part = warp % ks;
     const int cs = a.cs, rank = (int)blockIdx.x % cs;
+    const int bx = (int)blockIdx.x / cs, gx = (int)gridDim.x / cs;
     const int m0 = blockIdx.y * a.rows, mrows = min(a.rows, a.M - m0), vr = mrows * a.pieces;
     const int ldx = a.chunk * 128 + 32;  // halves per staged row: an odd number of 64-byte units
     uint16_t* xs = reinterpret_cast<uint16_t*>(smem);
@@ -226,58 +264,72 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     float* red = reinterpret_cast<float*>(smem + (size_t)a.rows * a.pieces * ldx * 2 + kWarps * kDepth * NW * kSlot);
 
     const int s0 = (int)((long long)a.S * rank / cs), s1 = (int)((long long)a.S * (rank + 1) / cs);
-    const int groups = (a.T + tpc - 1) / tpc;
-    const int rg0 = (int)blockIdx.x / cs, rstep = (int)gridDim.x / cs;
-    const int nmax = (s1 - s0 + ks - 1) / ks;                              // spans per warp, at most
+    const int rounds = (a.T + tpc * gx - 1) / (tpc * gx);
+    const int nmax = (s1 - s0 + ks - 1) / ks;                               // spans per warp, at most
     const int nmine = s0 + part < s1 ? (s1 - s0 - part + ks - 1) / ks : 0;  // this warp's
-    const uint32_t ring_s = smem_u32(ring);
+    const int tile0 = sub * gx + bx, tstep = tpc * gx;
 
-    // the warp's (tile, span) sequence, kDepth - 1 ahead of the math
-    int pr = rg0, pi = 0, pslot = 0;
+    // The warp's (tile, span) sequence, kDepth - 1 ahead of the math: pointers
+    // that advance by constants.
+    int ptiles = nmine > 0 && tile0 < a.T ? (a.T - tile0 + tstep - 1) / tstep : 0, pleft = nmine;
+    int pgroup = (s0 + part) * GP;  // the next span's first group
+    const uint8_t *pc[NW], *ps[NW], *pz[NW];
+#pragma unroll
+    for (int q = 0; q < NW; ++q) {
+        pc[q] = reinterpret_cast<const uint8_t*>(a.codes[q]) + ((size_t)tile0 * a.S + s0 + part) * 1024 + lane * 16;
+        ps[q] = reinterpret_cast<const uint8_t*>(a.scales[q]) + ((size_t)tile0 * a.Q + pgroup) * 32 + lane * 4;
+        pz[q] = a.zeros[q] ? a.zeros[q] + ((size_t)tile0 * a.Q + pgroup) * 16 + lane * 4 : nullptr;
+    }
+    const size_t cjump = ((size_t)tstep * a.S - (size_t)nmine * ks) * 1024;
+    const long long gjump = (long long)tstep * a.Q - (long long)nmine * ks * GP;
+    const uint32_t ring_s = smem_u32(ring);
+    uint32_t poff = 0;
     auto issue = [&]() {
-        if (nmine > 0 && pr < groups) {
-            const int tile = pr * tpc + sub;
-            if (tile < a.T) {
-                const int sp = s0 + part + pi * ks;
+        if (ptiles > 0) {
+#pragma unroll
+            for (int q = 0; q < NW; ++q) {
+                const uint32_t dst = ring_s + poff + q * kSlot;
+                cp16(dst + lane * 16, pc[q]);
+                cp16(dst + 512 + lane * 16, pc[q] + 512);
+                // 32 bytes of scales and 16 of zero points per group; a row's last span may have fewer groups
+                if (lane < GP * 8 && (GP == 1 || pgroup + (lane >> 3) < a.Q)) cp4(dst + 1024 + lane * 4, ps[q]);
+                if (pz[q] && lane < GP * 4 && (GP == 1 || pgroup + (lane >> 2) < a.Q)) cp4(dst + 1152 + lane * 4, pz[q]);
+                pc[q] += ks * 1024;
+                ps[q] += ks * GP * 32;
+                if (pz[q]) pz[q] += ks * GP * 16;
+            }
+            pgroup += ks * GP;
+            if (--pleft == 0) {
+                pleft = nmine;
+                --ptiles;
+                pgroup -= nmine * ks * GP;
 #pragma unroll
                 for (int q = 0; q < NW; ++q) {
-                    const uint32_t dst = ring_s + (pslot * NW + q) * kSlot;
-                    const uint8_t* src = reinterpret_cast<const uint8_t*>(a.codes[q]) + ((size_t)tile * a.S + sp) * 1024;
-                    cp16(dst + lane * 16, src + lane * 16);
-                    cp16(dst + 512 + lane * 16, src + 512 + lane * 16);
-                    const int gi = sp * GP + (lane >> 3);
-                    if (lane < GP * 8)
-                        cp4(dst + 1024 + lane * 4,
-                            reinterpret_cast<const uint8_t*>(a.scales[q]) + ((size_t)tile * a.Q + min(gi, a.Q - 1)) * 32 + (lane & 7) * 4,
-                            gi < a.Q);
-                    if (a.zeros[q] && lane < GP * 4) {
-                        const int gz = sp * GP + (lane >> 2);
-                        cp4(dst + 1152 + lane * 4, a.zeros[q] + ((size_t)tile * a.Q + min(gz, a.Q - 1)) * 16 + (lane & 3) * 4, gz < a.Q);
-                    }
+                    pc[q] += cjump;
+                    ps[q] += gjump * 32;
+                    if (pz[q]) pz[q] += gjump * 16;
                 }
-            }
-            if (++pi == nmine) {
-                pi = 0;
-                pr += rstep;
             }
         }
         cp_commit();
-        pslot = pslot + 1 == kDepth ? 0 : pslot + 1;
+        poff = poff == (kDepth - 1) * NW * kSlot ? 0 : poff + NW * kSlot;
     };
 
-    // Launched as a programmatic dependent in the model's chain: the weights,
-    // which no kernel of the chain writes, are fetched before the wait.
+    // In the model's chain (a.early) the weights, which no kernel of the chain
+    // writes, are fetched before the wait for the previous kernel.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (!a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < kDepth - 1; ++i) issue();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const bool wide = (reinterpret_cast<size_t>(a.x) & 15) == 0 && (a.ldx * (a.in == W4_X_16 ? 2 : 4)) % 16 == 0;
     const int chunks = (s1 - s0 + a.chunk - 1) / a.chunk;
     auto stage_chunk = [&](int ch) {
         const int b = s0 + ch * a.chunk, e = min(b + a.chunk, s1);
-        for (int m = warp; m < mrows; m += kWarps)
-            stage(a, m0 + m, b * 128, (e - b) * 128, xs + (size_t)m * a.pieces * ldx, ldx, wide);
+        stage_rows(a, m0, mrows, b * 128, (e - b) * 128, xs, ldx, wide);
+        cp_commit();
+        cp_wait<0>();
     };
     const int per_chunk = a.chunk / ks;  // steps of a warp per staged chunk (chunk is a multiple of ks, or holds every span)
     if (chunks == 1) {
@@ -285,80 +337,90 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
         __syncthreads();
     }
 
-    int slot = 0;
+    uint32_t slot = 0;
+    uint2 zl[NW], zh[NW];  // zero points of rows g and g + 8
+#pragma unroll
+    for (int q = 0; q < NW; ++q) zl[q] = zh[q] = zero_consts<BF>(8u);
+    int xrow[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) xrow[t] = min(t * 8 + g, vr - 1) * ldx;
 #pragma unroll 1
-    for (int rg = rg0; rg < groups; rg += rstep) {
-        const bool live = rg * tpc + sub < a.T;
+    for (int rd = 0; rd < rounds; ++rd) {
+        const int tile = tile0 + rd * tstep;
+        const bool live = tile < a.T;
         float acc[NW][NT][4];
 #pragma unroll
         for (int q = 0; q < NW; ++q)
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[q][t][0] = acc[q][t][1] = acc[q][t][2] = acc[q][t][3] = 0.f;
+        const uint16_t* xp = xs + part * 128 + 8 * c;
+        int left = s1 - s0 - part;  // spans from this one to the range's end
 #pragma unroll 1
         for (int it = 0; it < nmax; ++it) {
             if (chunks > 1 && it % per_chunk == 0) {
                 __syncthreads();
                 stage_chunk(it / per_chunk);
                 __syncthreads();
+                xp = xs + part * 128 + 8 * c;
             }
-            if (it >= nmine) continue;
+            if (it >= nmine || !live) continue;
             cp_wait<kDepth - 2>();
             __syncwarp();  // the span's scales came by other lanes; the slot refilled next was read by all of them
             issue();
-            if (live) {
-                const int xo = (part + it * ks) % a.chunk * 128;  // the span within the staged chunk
-                uint32_t w[NW][8][4];  // A operands: steps of 16 inputs
-                float2 sc[NW][GP];     // scales of rows g and g + 8
+            uint32_t lo[NW][4], hi[NW][4];  // codes of rows g and g + 8, 8 inputs a word
+#pragma unroll
+            for (int q = 0; q < NW; ++q) {
+                const uint8_t* sl = ring + slot + q * kSlot + lane * 16;
+                const uint4 a4 = *reinterpret_cast<const uint4*>(sl), b4 = *reinterpret_cast<const uint4*>(sl + 512);
+                lo[q][0] = a4.x, lo[q][1] = a4.y, lo[q][2] = a4.z, lo[q][3] = a4.w;
+                hi[q][0] = b4.x, hi[q][1] = b4.y, hi[q][2] = b4.z, hi[q][3] = b4.w;
+            }
+            float d[NW][NT][4];  // this group's sums
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t p[NW][4], r[NW][4];
 #pragma unroll
                 for (int q = 0; q < NW; ++q) {
-                    const uint8_t* sl = ring + (slot * NW + q) * kSlot;
-                    const uint4 lo4 = *reinterpret_cast<const uint4*>(sl + lane * 16);
-                    const uint4 hi4 = *reinterpret_cast<const uint4*>(sl + 512 + lane * 16);
-                    const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
-                    uint2 zl, zh;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j % (4 / GP) == 0) {
-                            const int gq = j / (4 / GP);
-                            sc[q][gq] = __half22float2(*reinterpret_cast<const __half2*>(sl + 1024 + gq * 32 + g * 4));
-                            uint32_t z = 0x0808u;
-                            if (a.zeros[q]) z = *reinterpret_cast<const uint16_t*>(sl + 1152 + gq * 16 + g * 2);
-                            zl = zero_consts<BF>(z & 15u);
-                            zh = zero_consts<BF>((z >> 8) & 15u);
-                        }
-                        uint32_t p[4], r[4];
-                        unpack<BF>(lo[j], zl, p);
-                        unpack<BF>(hi[j], zh, r);
-                        w[q][2 * j][0] = p[0], w[q][2 * j][1] = r[0], w[q][2 * j][2] = p[1], w[q][2 * j][3] = r[1];
-                        w[q][2 * j + 1][0] = p[2], w[q][2 * j + 1][1] = r[2], w[q][2 * j + 1][2] = p[3], w[q][2 * j + 1][3] = r[3];
+                    if (j % (4 / GP) == 0 && a.zeros[q]) {
+                        const uint32_t z = *reinterpret_cast<const uint16_t*>(ring + slot + q * kSlot + 1152 + j / (4 / GP) * 16 + g * 2);
+                        zl[q] = zero_consts<BF>(z & 15u);
+                        zh[q] = zero_consts<BF>((z >> 8) & 15u);
                     }
+                    unpack<BF>(lo[q][j], zl[q], p[q]);
+                    unpack<BF>(hi[q][j], zh[q], r[q]);
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    if (t * 8 >= vr) break;
                     // columns from vr on hold some row's values and are not read
-                    const uint16_t* xr = xs + (size_t)min(t * 8 + g, vr - 1) * ldx + xo + 8 * c;
-                    float d[NW][4];
+                    const uint4 b = *reinterpret_cast<const uint4*>(xp + xrow[t] + 32 * j);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint4 b = *reinterpret_cast<const uint4*>(xr + 32 * j);
+                    for (int q = 0; q < NW; ++q) {
+                        if (j % (4 / GP) == 0) d[q][t][0] = d[q][t][1] = d[q][t][2] = d[q][t][3] = 0.f;
+                        mma16816<BF>(d[q][t], p[q][0], r[q][0], p[q][1], r[q][1], b.x, b.y);
+                        mma16816<BF>(d[q][t], p[q][2], r[q][2], p[q][3], r[q][3], b.z, b.w);
+                    }
+                }
+                if ((j + 1) % (4 / GP) == 0) {
+                    const int gq = j / (4 / GP);
+                    // a group that the row does not have: its x is zero, its slot's old bytes may be anything
+                    const bool none = GP > 1 && gq > 0 && left == 1 && s1 == a.S && gq >= a.last_groups;
 #pragma unroll
-                        for (int q = 0; q < NW; ++q) {
-                            if (j % (4 / GP) == 0) d[q][0] = d[q][1] = d[q][2] = d[q][3] = 0.f;
-                            mma16816<BF>(d[q], w[q][2 * j][0], w[q][2 * j][1], w[q][2 * j][2], w[q][2 * j][3], b.x, b.y);
-                            mma16816<BF>(d[q], w[q][2 * j + 1][0], w[q][2 * j + 1][1], w[q][2 * j + 1][2], w[q][2 * j + 1][3], b.z, b.w);
-                            if ((j + 1) % (4 / GP) == 0) {
-                                const float2 s = sc[q][j / (4 / GP)];
-                                acc[q][t][0] = fmaf(s.x, d[q][0], acc[q][t][0]);
-                                acc[q][t][1] = fmaf(s.x, d[q][1], acc[q][t][1]);
-                                acc[q][t][2] = fmaf(s.y, d[q][2], acc[q][t][2]);
-                                acc[q][t][3] = fmaf(s.y, d[q][3], acc[q][t][3]);
-                            }
+                    for (int q = 0; q < NW; ++q) {
+                        float2 sc = __half22float2(*reinterpret_cast<const __half2*>(ring + slot + q * kSlot + 1024 + gq * 32 + g * 4));
+                        if (none) sc = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            acc[q][t][0] = fmaf(sc.x, d[q][t][0], acc[q][t][0]);
+                            acc[q][t][1] = fmaf(sc.x, d[q][t][1], acc[q][t][1]);
+                            acc[q][t][2] = fmaf(sc.y, d[q][t][2], acc[q][t][2]);
+                            acc[q][t][3] = fmaf(sc.y, d[q][t][3], acc[q][t][3]);
                         }
                     }
                 }
             }
-            slot = slot + 1 == kDepth ? 0 : slot + 1;
+            xp += ks * 128;
+            left -= ks;
+            slot = slot == (kDepth - 1) * NW * kSlot ? 0 : slot + NW * kSlot;
         }
         // partial tiles of this warp: [matrix][column][row]
         if (live) {
@@ -368,30 +430,56 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        red[((warp * NW + q) * kCols + t * 8 + 2 * c + (i & 1)) * kRedLd + g + (i >> 1) * 8] = acc[q][t][i];
+                        red[warp * kRedWarp + (q * kCols + t * 8 + 2 * c + (i & 1)) * kRedLd + g + (i >> 1) * 8] = acc[q][t][i];
+        }
+        if (ks == 1 && cs == 1) {
+            __syncwarp();
+            if (live) {
+                for (int e = lane; e < 16 * mrows; e += 32) {
+                    const int n = tile * 16 + (e & 15), m = e >> 4;
+                    if (n >= a.N) continue;
+                    float y[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int q = 0; q < NW; ++q) {
+                        const float* at = red + warp * kRedWarp + (q * kCols + m * a.pieces) * kRedLd + (e & 15);
+                        for (int p = a.pieces - 1; p >= 0; --p) y[q] += at[p * kRedLd];  // the smallest parts first
+                    }
+                    epilogue(a, m0 + m, n, y[0], y[1]);
+                }
+            }
+            __syncwarp();
+            continue;
         }
         if (cs > 1) cluster_sync();
         else __syncthreads();
-        const int total = tpc * mrows * 16;
-        for (int e = threadIdx.x + rank * kWarps * 32; e < total; e += cs * kWarps * 32) {
+        // ks lanes per output, one per warp that has a part of it
+        const int total = tpc * mrows * 16, per = kWarps * 32 / ks, u = threadIdx.x % ks;
+        for (int e0 = rank * per; e0 < total; e0 += cs * per) {
+            const int e = e0 + threadIdx.x / ks;
+            const bool some = e < total;
             const int n16 = e & 15, m = (e >> 4) % mrows, ts = (e >> 4) / mrows;
-            const int n = (rg * tpc + ts) * 16 + n16;
-            if (n >= a.N) continue;
             float y[2] = {0.f, 0.f};
+            if (some) {
+                for (int p = a.pieces - 1; p >= 0; --p)  // the smallest parts first
 #pragma unroll
-            for (int q = 0; q < NW; ++q) {
-                for (int p = a.pieces - 1; p >= 0; --p) {  // the smallest parts first
-                    const int at = (q * kCols + m * a.pieces + p) * kRedLd + n16;
-                    for (int r = 0; r < cs; ++r) {
-                        const uint32_t base = cs > 1 ? cluster_map(smem_u32(red), r) : 0u;
-                        for (int u = 0; u < ks; ++u) {
-                            const int o = (ts * ks + u) * NW * kCols * kRedLd + at;
-                            y[q] += cs > 1 ? ld_cluster_f32(base + o * 4) : red[o];
+                    for (int q = 0; q < NW; ++q) {
+                        const int o = (ts * ks + u) * kRedWarp + (q * kCols + m * a.pieces + p) * kRedLd + n16;
+                        if (cs == 1) {
+                            y[q] += red[o];
+                        } else {
+                            float v[8];
+#pragma unroll
+                            for (int r = 0; r < 8; ++r) v[r] = r < cs ? ld_cluster_f32(cluster_map(smem_u32(red + o), r)) : 0.f;
+#pragma unroll
+                            for (int r = 0; r < 8; ++r) y[q] += v[r];
                         }
                     }
-                }
             }
-            epilogue(a, m0 + m, n, y[0], y[1]);
+            for (int o = 1; o < ks; o <<= 1)
+#pragma unroll
+                for (int q = 0; q < NW; ++q) y[q] += __shfl_xor_sync(0xffffffffu, y[q], o);
+            const int n = (tile0 - sub * gx + (ts + rd * tpc) * gx) * 16 + n16;
+            if (some && u == 0 && n < a.N) epilogue(a, m0 + m, n, y[0], y[1]);
         }
         if (cs > 1) cluster_sync();  // red is written again, or this CTA ends, only when nobody reads it
         else __syncthreads();
@@ -502,10 +590,10 @@ __global__ void __launch_bounds__(256)
 
 // ------------------------------------------------------------------ launching
 template <int BF, int NT, int NW, int GP>
-cudaError_t launch_inst(const W4Args& a, int gx, int passes, int smem, bool pdl, cudaStream_t st) {
+cudaError_t launch_inst(const W4Args& a, int gx, int passes, int smem, cudaStream_t st) {
     auto fn = w4_kernel<BF, NT, NW, GP>;
-    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kW4MaxSmem);
+    static SmemGrant grant;
+    cudaError_t e = grant.raise(reinterpret_cast<const void*>(fn), kW4MaxSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(gx * a.cs), (unsigned)passes);
@@ -521,46 +609,47 @@ cudaError_t launch_inst(const W4Args& a, int gx, int passes, int smem, bool pdl,
         attr[na].val.clusterDim.z = 1;
         ++na;
     }
-    if (pdl) {
-        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[na].val.programmaticStreamSerializationAllowed = 1;
-        ++na;
-    }
+    // may start while the previous kernel of the stream ends: it waits for
+    // that kernel before it reads anything (a.early: but weights)
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
     cfg.attrs = attr;
     cfg.numAttrs = na;
     return counted(cudaLaunchKernelEx(&cfg, fn, a));
 }
 
 template <int BF, int NT, int NW>
-cudaError_t launch_gp(const W4Args& a, int group, int gx, int passes, int smem, bool pdl, cudaStream_t st) {
-    if (group == 128) return launch_inst<BF, NT, NW, 1>(a, gx, passes, smem, pdl, st);
-    if (group == 64) return launch_inst<BF, NT, NW, 2>(a, gx, passes, smem, pdl, st);
-    return launch_inst<BF, NT, NW, 4>(a, gx, passes, smem, pdl, st);
+cudaError_t launch_gp(const W4Args& a, int group, int gx, int passes, int smem, cudaStream_t st) {
+    if (group == 128) return launch_inst<BF, NT, NW, 1>(a, gx, passes, smem, st);
+    if (group == 64) return launch_inst<BF, NT, NW, 2>(a, gx, passes, smem, st);
+    return launch_inst<BF, NT, NW, 4>(a, gx, passes, smem, st);
 }
 
 template <int BF>
-cudaError_t launch_nt(const W4Args& a, int nt, int nw, int group, int gx, int passes, int smem, bool pdl, cudaStream_t st) {
+cudaError_t launch_nt(const W4Args& a, int nt, int nw, int group, int gx, int passes, int smem, cudaStream_t st) {
     if (nw == 2) {
-        if (nt == 1) return launch_gp<BF, 1, 2>(a, group, gx, passes, smem, pdl, st);
-        if (nt == 2) return launch_gp<BF, 2, 2>(a, group, gx, passes, smem, pdl, st);
-        return launch_gp<BF, 4, 2>(a, group, gx, passes, smem, pdl, st);
+        if (nt == 1) return launch_gp<BF, 1, 2>(a, group, gx, passes, smem, st);
+        if (nt == 2) return launch_gp<BF, 2, 2>(a, group, gx, passes, smem, st);
+        return launch_gp<BF, 4, 2>(a, group, gx, passes, smem, st);
     }
-    if (nt == 1) return launch_gp<BF, 1, 1>(a, group, gx, passes, smem, pdl, st);
-    if (nt == 2) return launch_gp<BF, 2, 1>(a, group, gx, passes, smem, pdl, st);
-    if (nt == 4) return launch_gp<BF, 4, 1>(a, group, gx, passes, smem, pdl, st);
-    return launch_gp<BF, 8, 1>(a, group, gx, passes, smem, pdl, st);
+    if (nt == 1) return launch_gp<BF, 1, 1>(a, group, gx, passes, smem, st);
+    if (nt == 2) return launch_gp<BF, 2, 1>(a, group, gx, passes, smem, st);
+    if (nt == 4) return launch_gp<BF, 4, 1>(a, group, gx, passes, smem, st);
+    return launch_gp<BF, 8, 1>(a, group, gx, passes, smem, st);
 }
 
 }  // namespace
 
-cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, bool pdl, cudaStream_t st) {
+cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st) {
     const W4Plan p = w4_plan(a.M, a.T, a.S, a.pieces, nw, kSms);
     a.rows = p.rows;
     a.ks = p.ks;
     a.cs = p.cs;
     a.chunk = p.chunk;
-    return bf ? launch_nt<1>(a, p.nt, nw, group, p.gx, p.passes, p.smem, pdl, st)
-              : launch_nt<0>(a, p.nt, nw, group, p.gx, p.passes, p.smem, pdl, st);
+    a.last_groups = a.Q - (a.S - 1) * (128 / group);
+    return bf ? launch_nt<1>(a, p.nt, nw, group, p.gx, p.passes, p.smem, st)
+              : launch_nt<0>(a, p.nt, nw, group, p.gx, p.passes, p.smem, st);
 }
 
 cudaError_t launch_w4_quantize(const w4_matrix& m, const void* w, int dtype, long long ldw, cudaStream_t st) {
