@@ -47,9 +47,8 @@ struct W4Args {
 
 constexpr int kSms = 148;
 constexpr int kW4MaxSmem = 227 * 1024;
-// Spans in flight per warp (64 rows leave the ring less shared memory).
-constexpr int w4_depth(int nw, int nt) { return nw == 2 ? 4 : nt == 8 ? 5 : 6; }
-
+// Spans that a warp copies at a time (two such batches in shared memory).
+constexpr int w4_batch(int nw, int nt) { return nw == 2 || nt >= 4 ? 2 : 4; }
 // Floats of a warp's partial tile: 20 per column (16 rows, padded against bank
 // conflicts), 4 more so that the warps' tiles start in different banks.
 constexpr int w4_red_floats(int nw, int nt) { return nw * nt * 8 * 20 + 4; }
@@ -71,13 +70,13 @@ inline W4Plan w4_plan(int M, int T, int S, int pieces, int nw, int sms) {
     const int share = std::max(1, std::min(S, sms * 16 / std::max(1, T * p.passes)));
     p.ks = share >= 8 ? 8 : share >= 4 ? 4 : share >= 2 ? 2 : 1;
     p.cs = share >= 64 ? 8 : share >= 32 ? 4 : share >= 16 ? 2 : 1;
-    const int fixed = 8 * (w4_depth(nw, p.nt) * nw * 1216 + w4_red_floats(nw, p.nt) * 4);
+    const int fixed = 8 * (2 * w4_batch(nw, p.nt) * nw * 1216 + w4_red_floats(nw, p.nt) * 4);
     const int spans = (S + p.cs - 1) / p.cs;
-    // staged spans: all of the CTA's, or a multiple of ks that fits
+    // staged spans: all of the CTA's, or as many batches of its warps as fit
     const int fit = ((kW4MaxSmem - fixed) / (vr * 2) - 32) / 128;
-    while (p.ks > fit) p.ks /= 2;
-    p.chunk = spans <= fit ? (spans + p.ks - 1) / p.ks * p.ks : fit / p.ks * p.ks;
-    if (p.chunk > fit) p.chunk = spans;
+    const int unit = w4_batch(nw, p.nt);
+    while (p.ks > 1 && p.ks * unit > fit) p.ks /= 2;
+    p.chunk = spans <= fit ? spans : fit / (p.ks * unit) * (p.ks * unit);
     p.smem = fixed + vr * (p.chunk * 128 + 32) * 2;
     const int groups = (T + 8 / p.ks - 1) / (8 / p.ks);
     const int per_sm = p.smem <= 113 * 1024 && p.nt * nw <= 2 ? 2 : 1;

@@ -20,7 +20,7 @@
 //
 // Bound: the codes' bytes for few rows.  Each lane copies the 32 bytes of
 // codes that it will unpack itself to its own slots of a ring in shared memory
-// (cp.async, kDepth spans ahead, across tiles), so loads never wait for the
+// (cp.async, a batch of spans ahead, across tiles), so loads never wait for the
 // math and need no barrier; a warp's 16 rows x 128 inputs are one contiguous
 // KiB in memory.
 #include <cuda_bf16.h>
@@ -48,8 +48,7 @@ constexpr int kRedLd = 20;              // floats per column of a reduced tile: 
 template <int BF>
 __device__ __forceinline__ uint2 zero_consts(uint32_t z) {
     if (BF) return make_uint2((0x4300u | z) * 0x10001u, 0u);
-    const __half2 h = __float2half2_rn(-(float)(64 + (int)z));
-    return make_uint2((0x6400u | z) * 0x10001u, *reinterpret_cast<const uint32_t*>(&h));
+    return make_uint2((0x6400u | z) * 0x10001u, (0xD400u | z << 4) * 0x10001u);  // 1024 + z, -(64 + z)
 }
 
 // Eight codes minus their zero point as four pairs of fp16 / bf16 values, in
@@ -77,6 +76,20 @@ __device__ __forceinline__ void unpack(uint32_t w, uint2 zc, uint32_t (&p)[4]) {
             p[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
         }
     }
+}
+
+// mma16816 into fresh sums.
+template <int BF>
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+    if (BF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // ------------------------------------------------------------------- staging
@@ -249,7 +262,8 @@ __device__ __forceinline__ void epilogue(const W4Args& a, int row, int n, float 
 template <int BF, int NT, int NW, int GP>
 __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     w4_kernel(const __grid_constant__ W4Args a) {
-    constexpr int kDepth = w4_depth(NW, NT);
+    constexpr int kU = w4_batch(NW, NT);        // spans per batch
+    constexpr int kBatch = kU * NW * kSlot;     // bytes; two batches per warp: one in flight, one in use
     constexpr int kCols = NT * 8;
     constexpr int kRedWarp = w4_red_floats(NW, NT);
     extern __shared__ __align__(16) uint8_t smem[];
@@ -260,8 +274,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     const int m0 = blockIdx.y * a.rows, mrows = min(a.rows, a.M - m0), vr = mrows * a.pieces;
     const int ldx = a.chunk * 128 + 32;  // halves per staged row: an odd number of 64-byte units
     uint16_t* xs = reinterpret_cast<uint16_t*>(smem);
-    uint8_t* ring = smem + (size_t)a.rows * a.pieces * ldx * 2 + (size_t)warp * (kDepth * NW * kSlot);
-    float* red = reinterpret_cast<float*>(smem + (size_t)a.rows * a.pieces * ldx * 2 + kWarps * kDepth * NW * kSlot);
+    uint8_t* ring = smem + (size_t)a.rows * a.pieces * ldx * 2 + (size_t)warp * (2 * kBatch);
+    float* red = reinterpret_cast<float*>(smem + (size_t)a.rows * a.pieces * ldx * 2 + kWarps * 2 * kBatch);
 
     const int s0 = (int)((long long)a.S * rank / cs), s1 = (int)((long long)a.S * (rank + 1) / cs);
     const int rounds = (a.T + tpc * gx - 1) / (tpc * gx);
@@ -269,8 +283,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     const int nmine = s0 + part < s1 ? (s1 - s0 - part + ks - 1) / ks : 0;  // this warp's
     const int tile0 = sub * gx + bx, tstep = tpc * gx;
 
-    // The warp's (tile, span) sequence, kDepth - 1 ahead of the math: pointers
-    // that advance by constants.
+    // The warp's (tile, span) sequence, a batch ahead of the math: pointers that
+    // advance by constants; a batch ends with its tile.
     int ptiles = nmine > 0 && tile0 < a.T ? (a.T - tile0 + tstep - 1) / tstep : 0, pleft = nmine;
     int pgroup = (s0 + part) * GP;  // the next span's first group
     const uint8_t *pc[NW], *ps[NW], *pz[NW];
@@ -286,20 +300,26 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     uint32_t poff = 0;
     auto issue = [&]() {
         if (ptiles > 0) {
+            const int n = min(kU, pleft);
 #pragma unroll
-            for (int q = 0; q < NW; ++q) {
-                const uint32_t dst = ring_s + poff + q * kSlot;
-                cp16(dst + lane * 16, pc[q]);
-                cp16(dst + 512 + lane * 16, pc[q] + 512);
-                // 32 bytes of scales and 16 of zero points per group; a row's last span may have fewer groups
-                if (lane < GP * 8 && (GP == 1 || pgroup + (lane >> 3) < a.Q)) cp4(dst + 1024 + lane * 4, ps[q]);
-                if (pz[q] && lane < GP * 4 && (GP == 1 || pgroup + (lane >> 2) < a.Q)) cp4(dst + 1152 + lane * 4, pz[q]);
-                pc[q] += ks * 1024;
-                ps[q] += ks * GP * 32;
-                if (pz[q]) pz[q] += ks * GP * 16;
+            for (int u = 0; u < kU; ++u) {
+                if (u >= n) break;
+#pragma unroll
+                for (int q = 0; q < NW; ++q) {
+                    const uint32_t dst = ring_s + poff + (u * NW + q) * kSlot;
+                    cp16(dst + lane * 16, pc[q]);
+                    cp16(dst + 512 + lane * 16, pc[q] + 512);
+                    // 32 bytes of scales and 16 of zero points per group; a row's last span may have fewer groups
+                    if (lane < GP * 8 && (GP == 1 || pgroup + (lane >> 3) < a.Q)) cp4(dst + 1024 + lane * 4, ps[q]);
+                    if (pz[q] && lane < GP * 4 && (GP == 1 || pgroup + (lane >> 2) < a.Q)) cp4(dst + 1152 + lane * 4, pz[q]);
+                    pc[q] += ks * 1024;
+                    ps[q] += ks * GP * 32;
+                    if (pz[q]) pz[q] += ks * GP * 16;
+                }
+                pgroup += ks * GP;
             }
-            pgroup += ks * GP;
-            if (--pleft == 0) {
+            pleft -= n;
+            if (pleft == 0) {
                 pleft = nmine;
                 --ptiles;
                 pgroup -= nmine * ks * GP;
@@ -312,15 +332,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
             }
         }
         cp_commit();
-        poff = poff == (kDepth - 1) * NW * kSlot ? 0 : poff + NW * kSlot;
+        poff ^= kBatch;
     };
 
     // In the model's chain (a.early) the weights, which no kernel of the chain
     // writes, are fetched before the wait for the previous kernel.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (!a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < kDepth - 1; ++i) issue();
+    issue();
     if (a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const bool wide = (reinterpret_cast<size_t>(a.x) & 15) == 0 && (a.ldx * (a.in == W4_X_16 ? 2 : 4)) % 16 == 0;
@@ -331,7 +350,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
         cp_commit();
         cp_wait<0>();
     };
-    const int per_chunk = a.chunk / ks;  // steps of a warp per staged chunk (chunk is a multiple of ks, or holds every span)
+    const int per_chunk = a.chunk / ks;  // a warp's spans per staged chunk (whole batches, or chunk holds every span)
     if (chunks == 1) {
         stage_chunk(0);
         __syncthreads();
@@ -356,7 +375,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
         const uint16_t* xp = xs + part * 128 + 8 * c;
         int left = s1 - s0 - part;  // spans from this one to the range's end
 #pragma unroll 1
-        for (int it = 0; it < nmax; ++it) {
+        for (int it = 0; it < nmax; it += kU) {
             if (chunks > 1 && it % per_chunk == 0) {
                 __syncthreads();
                 stage_chunk(it / per_chunk);
@@ -364,13 +383,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
                 xp = xs + part * 128 + 8 * c;
             }
             if (it >= nmine || !live) continue;
-            cp_wait<kDepth - 2>();
-            __syncwarp();  // the span's scales came by other lanes; the slot refilled next was read by all of them
+            cp_wait<0>();
+            __syncwarp();  // scales came by other lanes; the batch refilled next was read by all of them
             issue();
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+            if (it + u >= nmine) break;
+            const uint8_t* const sl0 = ring + slot + u * NW * kSlot;
             uint32_t lo[NW][4], hi[NW][4];  // codes of rows g and g + 8, 8 inputs a word
 #pragma unroll
             for (int q = 0; q < NW; ++q) {
-                const uint8_t* sl = ring + slot + q * kSlot + lane * 16;
+                const uint8_t* sl = sl0 + q * kSlot + lane * 16;
                 const uint4 a4 = *reinterpret_cast<const uint4*>(sl), b4 = *reinterpret_cast<const uint4*>(sl + 512);
                 lo[q][0] = a4.x, lo[q][1] = a4.y, lo[q][2] = a4.z, lo[q][3] = a4.w;
                 hi[q][0] = b4.x, hi[q][1] = b4.y, hi[q][2] = b4.z, hi[q][3] = b4.w;
@@ -382,7 +405,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
 #pragma unroll
                 for (int q = 0; q < NW; ++q) {
                     if (j % (4 / GP) == 0 && a.zeros[q]) {
-                        const uint32_t z = *reinterpret_cast<const uint16_t*>(ring + slot + q * kSlot + 1152 + j / (4 / GP) * 16 + g * 2);
+                        const uint32_t z = *reinterpret_cast<const uint16_t*>(sl0 + q * kSlot + 1152 + j / (4 / GP) * 16 + g * 2);
                         zl[q] = zero_consts<BF>(z & 15u);
                         zh[q] = zero_consts<BF>((z >> 8) & 15u);
                     }
@@ -395,8 +418,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
                     const uint4 b = *reinterpret_cast<const uint4*>(xp + xrow[t] + 32 * j);
 #pragma unroll
                     for (int q = 0; q < NW; ++q) {
-                        if (j % (4 / GP) == 0) d[q][t][0] = d[q][t][1] = d[q][t][2] = d[q][t][3] = 0.f;
-                        mma16816<BF>(d[q][t], p[q][0], r[q][0], p[q][1], r[q][1], b.x, b.y);
+                        if (j % (4 / GP) == 0) mma16816_first<BF>(d[q][t], p[q][0], r[q][0], p[q][1], r[q][1], b.x, b.y);
+                        else mma16816<BF>(d[q][t], p[q][0], r[q][0], p[q][1], r[q][1], b.x, b.y);
                         mma16816<BF>(d[q][t], p[q][2], r[q][2], p[q][3], r[q][3], b.z, b.w);
                     }
                 }
@@ -406,7 +429,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
                     const bool none = GP > 1 && gq > 0 && left == 1 && s1 == a.S && gq >= a.last_groups;
 #pragma unroll
                     for (int q = 0; q < NW; ++q) {
-                        float2 sc = __half22float2(*reinterpret_cast<const __half2*>(ring + slot + q * kSlot + 1024 + gq * 32 + g * 4));
+                        float2 sc = __half22float2(*reinterpret_cast<const __half2*>(sl0 + q * kSlot + 1024 + gq * 32 + g * 4));
                         if (none) sc = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
@@ -420,7 +443,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
             }
             xp += ks * 128;
             left -= ks;
-            slot = slot == (kDepth - 1) * NW * kSlot ? 0 : slot + NW * kSlot;
+            }
+            slot ^= kBatch;
         }
         // partial tiles of this warp: [matrix][column][row]
         if (live) {
@@ -452,34 +476,34 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
         }
         if (cs > 1) cluster_sync();
         else __syncthreads();
-        // ks lanes per output, one per warp that has a part of it
-        const int total = tpc * mrows * 16, per = kWarps * 32 / ks, u = threadIdx.x % ks;
-        for (int e0 = rank * per; e0 < total; e0 += cs * per) {
-            const int e = e0 + threadIdx.x / ks;
-            const bool some = e < total;
-            const int n16 = e & 15, m = (e >> 4) % mrows, ts = (e >> 4) / mrows;
+        const int lone = tpc * mrows * 16 * ks <= kWarps * 32 ? ks : 1;  // lanes that share an output: its parts, where that fits
+        const int per = lone > 1 ? 1 : ks;                               // parts per lane
+        const int lu = threadIdx.x % lone, e0 = threadIdx.x / lone, n16 = e0 & 15, mstep = lone > 1 ? mrows * tpc : kWarps * 2;
+        for (int i = (e0 >> 4) + rank * mstep; i - (e0 >> 4) < mrows * tpc; i += cs * mstep) {
+            const int ts = mrows == 1 ? i : i / mrows, m = i - ts * mrows;
+            const bool some = ts < tpc;
             float y[2] = {0.f, 0.f};
             if (some) {
                 for (int p = a.pieces - 1; p >= 0; --p)  // the smallest parts first
 #pragma unroll
                     for (int q = 0; q < NW; ++q) {
-                        const int o = (ts * ks + u) * kRedWarp + (q * kCols + m * a.pieces + p) * kRedLd + n16;
-                        if (cs == 1) {
-                            y[q] += red[o];
-                        } else {
-                            float v[8];
+                        const float* at = red + (ts * ks + lu) * kRedWarp + (q * kCols + m * a.pieces + p) * kRedLd + n16;
+                        for (int r = 0; r < cs; ++r) {
+                            const uint32_t far = cs > 1 ? cluster_map(smem_u32(at), r) : 0u;
+                            float v[kWarps];
 #pragma unroll
-                            for (int r = 0; r < 8; ++r) v[r] = r < cs ? ld_cluster_f32(cluster_map(smem_u32(red + o), r)) : 0.f;
+                            for (int u = 0; u < kWarps; ++u)
+                                v[u] = u >= per ? 0.f : cs > 1 ? ld_cluster_f32(far + u * kRedWarp * 4) : at[u * kRedWarp];
 #pragma unroll
-                            for (int r = 0; r < 8; ++r) y[q] += v[r];
+                            for (int u = 0; u < kWarps; ++u) y[q] += v[u];
                         }
                     }
             }
-            for (int o = 1; o < ks; o <<= 1)
+            for (int o = 1; o < lone; o <<= 1)
 #pragma unroll
                 for (int q = 0; q < NW; ++q) y[q] += __shfl_xor_sync(0xffffffffu, y[q], o);
-            const int n = (tile0 - sub * gx + (ts + rd * tpc) * gx) * 16 + n16;
-            if (some && u == 0 && n < a.N) epilogue(a, m0 + m, n, y[0], y[1]);
+            const int n = (bx + (ts + rd * tpc) * gx) * 16 + n16;
+            if (some && lu == 0 && n < a.N) epilogue(a, m0 + m, n, y[0], y[1]);
         }
         if (cs > 1) cluster_sync();  // red is written again, or this CTA ends, only when nobody reads it
         else __syncthreads();
