@@ -51,6 +51,13 @@ __device__ __forceinline__ uint2 zero_consts(uint32_t z) {
     return make_uint2((0x6400u | z) * 0x10001u, (0xD400u | z << 4) * 0x10001u);  // 1024 + z, -(64 + z)
 }
 
+// (a & b) | c in one instruction (only one of b and c may be an immediate).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
 // Eight codes minus their zero point as four pairs of fp16 / bf16 values, in
 // input order.
 template <int BF>
@@ -59,7 +66,7 @@ __device__ __forceinline__ void unpack(uint32_t w, uint2 zc, uint32_t (&p)[4]) {
         const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&zc.x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t v = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+            const uint32_t v = and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
             const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), z);
             p[i] = *reinterpret_cast<const uint32_t*>(&r);
         }
@@ -69,7 +76,7 @@ __device__ __forceinline__ void unpack(uint32_t w, uint2 zc, uint32_t (&p)[4]) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t u = w >> (8 * i);
-            const uint32_t lo = (u & 0x000F000Fu) | 0x64006400u, hi = (u & 0x00F000F0u) | 0x64006400u;
+            const uint32_t lo = and_or(u, 0x000F000Fu, 0x64006400u), hi = and_or(u, 0x00F000F0u, 0x64006400u);
             const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), z);
             const __half2 b = __hfma2(*reinterpret_cast<const __half2*>(&hi), sixteenth, z16);
             p[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
@@ -513,7 +520,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
 
 // ------------------------------------------------------- to 4 bits and back
 // One warp per (tile, span); lane (g, c) holds rows g and g + 8, inputs
-// 32 j + 8 c + i.  The group statistics are maxima, exact in any order.
+// 32 j + 8 c + i: the words that it writes or reads.  A matrix's rows are
+// read (or written) as units of W bytes, the widest that the addresses and the
+// row length allow, all of a lane's at once.  The group statistics are maxima, exact in any order.
+// Bound: the bytes of the wide side.
 template <class T>
 __device__ __forceinline__ float to_f(T v);
 template <>
@@ -521,79 +531,104 @@ __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
 template <>
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-template <class T>
+template <int W>
+struct Unit;
+template <>
+struct Unit<16> { using type = uint4; };
+template <>
+struct Unit<8> { using type = uint2; };
+template <>
+struct Unit<4> { using type = uint32_t; };
+template <>
+struct Unit<2> { using type = uint16_t; };
+
+template <class T, int W, int JG /* words per group */, bool ZP>
 __global__ void __launch_bounds__(256)
-    w4_quantize_kernel(const T* __restrict__ w, long long ldw, int N, int K, int T_, int S, int Q, int jg /* words per group */,
+    w4_quantize_kernel(const T* __restrict__ w, long long ldw, int N, int K, int S, int Q,
                        uint32_t* __restrict__ codes, __half* __restrict__ scales, uint8_t* __restrict__ zeros) {
+    using U = typename Unit<W>::type;
+    constexpr int kE = W / 2;  // elements per unit
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (id >= (long long)T_ * S) return;
-    const int t = (int)(id / S), s = (int)(id % S);
+    const int s = blockIdx.x * 8 + (threadIdx.x >> 5), t = blockIdx.y;
+    if (s >= S) return;
+    T v[2][4][8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int n = t * 16 + h * 8 + g;
-        float v[4][8];
+        const T* row = w + (size_t)min(n, N - 1) * ldw;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 8; i += kE) {
                 const int k = s * 128 + 32 * j + 8 * c + i;
-                v[j][i] = n < N && k < K ? to_f(w[(size_t)n * ldw + k]) : 0.f;
+                if (k + kE <= K) {
+                    *reinterpret_cast<U*>(&v[h][j][i]) = __ldg(reinterpret_cast<const U*>(row + k));
+                } else {
+#pragma unroll
+                    for (int ii = 0; ii < kE; ++ii) {
+                        const uint16_t zero = 0;
+                        v[h][j][i + ii] = k + ii < K ? row[k + ii] : *reinterpret_cast<const T*>(&zero);
+                    }
+                }
             }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
         uint32_t word[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j0 = 0; j0 < 4; j0 += JG) {
             float lo = 0.f, hi = 0.f;
-            const int j0 = j / jg * jg;
 #pragma unroll
-            for (int jj = 0; jj < 4; ++jj)
-                if (jj >= j0 && jj < j0 + jg) {
+            for (int j = j0; j < j0 + JG; ++j)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        lo = fminf(lo, v[jj][i]);
-                        hi = fmaxf(hi, v[jj][i]);
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    lo = fminf(lo, to_f(v[h][j][i]));
+                    hi = fmaxf(hi, to_f(v[h][j][i]));
                 }
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) {
                 lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
                 hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
             }
-            const float span = zeros ? __fdiv_rn(__fsub_rn(hi, lo), 15.0f) : __fdiv_rn(fmaxf(-lo, hi), 7.0f);
-            const __half sh = __float2half_rn(span);
+            const __half sh = __float2half_rn(ZP ? __fdiv_rn(__fsub_rn(hi, lo), 15.0f) : __fdiv_rn(fmaxf(-lo, hi), 7.0f));
             const float sc = __half2float(sh);
             const bool some = sc > 0.f;
-            const float z = zeros && some ? fminf(fmaxf(rintf(__fdiv_rn(-lo, sc)), 0.f), 15.f) : 8.f;
-            uint32_t q = 0;
+            const float z = ZP && some ? fminf(fmaxf(rintf(__fdiv_rn(-lo, sc)), 0.f), 15.f) : 8.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float r = some ? __fadd_rn(rintf(__fdiv_rn(v[j][i], sc)), z) : z;
-                q |= (uint32_t)fminf(fmaxf(r, 0.f), 15.f) << (4 * ((i >> 1) + 4 * (i & 1)));
+            for (int j = j0; j < j0 + JG; ++j) {
+                uint32_t q = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float r = some ? __fadd_rn(rintf(__fdiv_rn(to_f(v[h][j][i]), sc)), z) : z;
+                    q |= (uint32_t)fminf(fmaxf(r, 0.f), 15.f) << (4 * ((i >> 1) + 4 * (i & 1)));
+                }
+                word[j] = q;
             }
-            word[j] = q;
-            const int gi = s * (4 / jg) + j / jg;
-            if (j == j0 && c == 0 && gi < Q) {
+            const int gi = s * (4 / JG) + j0 / JG;
+            if (c == 0 && gi < Q) {
                 const size_t at = (((size_t)t * Q + gi) * 8 + g) * 2 + h;
                 scales[at] = sh;
-                if (zeros) zeros[at] = (uint8_t)z;
+                if (ZP) zeros[at] = (uint8_t)z;
             }
         }
-        reinterpret_cast<uint4*>(codes)[(id * 2 + h) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+        reinterpret_cast<uint4*>(codes)[(((size_t)t * S + s) * 2 + h) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
     }
 }
 
+template <int W>
 __global__ void __launch_bounds__(256)
     w4_dequantize_kernel(const uint32_t* __restrict__ codes, const __half* __restrict__ scales,
-                         const uint8_t* __restrict__ zeros, int N, int K, int T_, int S, int Q, int jg,
-                         float* __restrict__ out, long long ldo) {
+                         const uint8_t* __restrict__ zeros, int N, int K, int S, int Q, int jg, float* __restrict__ out,
+                         long long ldo) {
+    using U = typename Unit<W>::type;
+    constexpr int kE = W / 4;
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (id >= (long long)T_ * S) return;
-    const int t = (int)(id / S), s = (int)(id % S);
+    const int s = blockIdx.x * 8 + (threadIdx.x >> 5), t = blockIdx.y;
+    if (s >= S) return;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int n = t * 16 + h * 8 + g;
-        const uint4 w4 = reinterpret_cast<const uint4*>(codes)[(id * 2 + h) * 32 + lane];
+        const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(codes) + (((size_t)t * S + s) * 2 + h) * 32 + lane);
         const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
         if (n >= N) continue;
 #pragma unroll
@@ -602,11 +637,20 @@ __global__ void __launch_bounds__(256)
             if (gi >= Q) continue;
             const size_t at = (((size_t)t * Q + gi) * 8 + g) * 2 + h;
             const float sc = __half2float(scales[at]), z = zeros ? (float)(zeros[at] & 15) : 8.f;
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int k = s * 128 + 32 * j + 8 * c + i;
-                if (k < K)
-                    out[(size_t)n * ldo + k] = ((float)((w[j] >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) - z) * sc;
+            for (int i = 0; i < 8; ++i) v[i] = ((float)((w[j] >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) - z) * sc;
+            const int k = s * 128 + 32 * j + 8 * c;
+            float* to = out + (size_t)n * ldo + k;
+#pragma unroll
+            for (int i = 0; i < 8; i += kE) {
+                if (k + i + kE <= K) {
+                    *reinterpret_cast<U*>(to + i) = *reinterpret_cast<const U*>(v + i);
+                } else {
+#pragma unroll
+                    for (int ii = 0; ii < kE; ++ii)
+                        if (k + i + ii < K) to[i + ii] = v[i + ii];
+                }
             }
         }
     }
@@ -676,27 +720,74 @@ cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st) {
               : launch_nt<0>(a, p.nt, nw, group, p.gx, p.passes, p.smem, st);
 }
 
-cudaError_t launch_w4_quantize(const w4_matrix& m, const void* w, int dtype, long long ldw, cudaStream_t st) {
-    const int T = (m.n + 15) / 16, S = (m.k + 127) / 128, Q = (m.k + m.group - 1) / m.group, jg = m.group / 32;
-    const long long blocks = ((long long)T * S + 7) / 8;
-    if (dtype == STEP_F16)
-        w4_quantize_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const __half*>(w), ldw, m.n, m.k, T, S, Q, jg,
-                                                             static_cast<uint32_t*>(m.codes), static_cast<__half*>(m.scales),
-                                                             static_cast<uint8_t*>(m.zeros));
+namespace {
+
+// The widest power of two up to `most` bytes that an address and a row stride share.
+int unit_bytes(const void* p, long long ld_bytes, int most) {
+    int w = most;
+    while (reinterpret_cast<size_t>(p) % w || ld_bytes % w) w /= 2;
+    return w;
+}
+
+template <class T, int W, int JG>
+void quantize_zp(const w4_matrix& m, const void* w, long long ldw, dim3 grid, int S, int Q, int tile0, cudaStream_t st) {
+    const T* src = static_cast<const T*>(w) + (size_t)tile0 * 16 * ldw;
+    uint32_t* codes = static_cast<uint32_t*>(m.codes) + (size_t)tile0 * S * 256;
+    __half* scales = static_cast<__half*>(m.scales) + (size_t)tile0 * Q * 16;
+    uint8_t* zeros = static_cast<uint8_t*>(m.zeros);
+    const int N = m.n - tile0 * 16;
+    if (zeros)
+        w4_quantize_kernel<T, W, JG, true><<<grid, 256, 0, st>>>(src, ldw, N, m.k, S, Q, codes, scales, zeros + (size_t)tile0 * Q * 16);
     else
-        w4_quantize_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(w), ldw, m.n, m.k, T, S, Q, jg,
-                                                             static_cast<uint32_t*>(m.codes), static_cast<__half*>(m.scales),
-                                                             static_cast<uint8_t*>(m.zeros));
-    return counted(cudaGetLastError());
+        w4_quantize_kernel<T, W, JG, false><<<grid, 256, 0, st>>>(src, ldw, N, m.k, S, Q, codes, scales, nullptr);
+}
+
+template <class T, int W>
+void quantize_jg(const w4_matrix& m, const void* w, long long ldw, dim3 grid, int S, int Q, int tile0, cudaStream_t st) {
+    if (m.group == 128) quantize_zp<T, W, 4>(m, w, ldw, grid, S, Q, tile0, st);
+    else if (m.group == 64) quantize_zp<T, W, 2>(m, w, ldw, grid, S, Q, tile0, st);
+    else quantize_zp<T, W, 1>(m, w, ldw, grid, S, Q, tile0, st);
+}
+
+template <class T>
+void quantize_w(const w4_matrix& m, const void* w, long long ldw, dim3 grid, int S, int Q, int tile0, cudaStream_t st) {
+    const int u = unit_bytes(w, ldw * 2, 16);
+    if (u == 16) quantize_jg<T, 16>(m, w, ldw, grid, S, Q, tile0, st);
+    else if (u >= 4) quantize_jg<T, 4>(m, w, ldw, grid, S, Q, tile0, st);
+    else quantize_jg<T, 2>(m, w, ldw, grid, S, Q, tile0, st);
+}
+
+constexpr int kMaxGridY = 65535;  // tiles per launch
+
+}  // namespace
+
+cudaError_t launch_w4_quantize(const w4_matrix& m, const void* w, int dtype, long long ldw, cudaStream_t st) {
+    const int T = (m.n + 15) / 16, S = (m.k + 127) / 128, Q = (m.k + m.group - 1) / m.group;
+    for (int t0 = 0; t0 < T; t0 += kMaxGridY) {
+        const dim3 grid((unsigned)((S + 7) / 8), (unsigned)(T - t0 < kMaxGridY ? T - t0 : kMaxGridY));
+        if (dtype == STEP_F16) quantize_w<__half>(m, w, ldw, grid, S, Q, t0, st);
+        else quantize_w<__nv_bfloat16>(m, w, ldw, grid, S, Q, t0, st);
+        const cudaError_t e = counted(cudaGetLastError());
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 cudaError_t launch_w4_dequantize(const w4_matrix& m, float* out, long long ldo, cudaStream_t st) {
     const int T = (m.n + 15) / 16, S = (m.k + 127) / 128, Q = (m.k + m.group - 1) / m.group, jg = m.group / 32;
-    const long long blocks = ((long long)T * S + 7) / 8;
-    w4_dequantize_kernel<<<(unsigned)blocks, 256, 0, st>>>(static_cast<const uint32_t*>(m.codes),
-                                                           static_cast<const __half*>(m.scales),
-                                                           static_cast<const uint8_t*>(m.zeros), m.n, m.k, T, S, Q, jg, out, ldo);
-    return counted(cudaGetLastError());
+    const int u = unit_bytes(out, ldo * 4, 16);
+    auto fn = u == 16 ? w4_dequantize_kernel<16> : u == 8 ? w4_dequantize_kernel<8> : w4_dequantize_kernel<4>;
+    for (int t0 = 0; t0 < T; t0 += kMaxGridY) {
+        const dim3 grid((unsigned)((S + 7) / 8), (unsigned)(T - t0 < kMaxGridY ? T - t0 : kMaxGridY));
+        const uint8_t* zeros = static_cast<const uint8_t*>(m.zeros);
+        fn<<<grid, 256, 0, st>>>(static_cast<const uint32_t*>(m.codes) + (size_t)t0 * S * 256,
+                                 static_cast<const __half*>(m.scales) + (size_t)t0 * Q * 16,
+                                 zeros ? zeros + (size_t)t0 * Q * 16 : nullptr, m.n - t0 * 16, m.k, S, Q, jg,
+                                 out + (size_t)t0 * 16 * ldo, ldo);
+        const cudaError_t e = counted(cudaGetLastError());
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace kvattn
