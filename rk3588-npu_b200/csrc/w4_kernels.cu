@@ -519,11 +519,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
 }
 
 // ------------------------------------------------------- to 4 bits and back
-// One warp per (tile, span); lane (g, c) holds rows g and g + 8, inputs
-// 32 j + 8 c + i: the words that it writes or reads.  A matrix's rows are
-// read (or written) as units of W bytes, the widest that the addresses and the
-// row length allow, all of a lane's at once.  The group statistics are maxima, exact in any order.
-// Bound: the bytes of the wide side.
+// One warp per (tile, span), row by row: lane l holds inputs 4 l .. 4 l + 3, so
+// a row's 128 inputs are one contiguous access and half a code word is a
+// lane's own.  The 16 rows' loads are issued together, in units of W bytes,
+// the widest that the addresses allow.  Group statistics are maxima, exact in
+// any order.  Bound: the bytes of the 16- or 32-bit side.
 template <class T>
 __device__ __forceinline__ float to_f(T v);
 template <>
@@ -542,118 +542,138 @@ struct Unit<4> { using type = uint32_t; };
 template <>
 struct Unit<2> { using type = uint16_t; };
 
-template <class T, int W, int JG /* words per group */, bool ZP>
+// rint(v / s), v and s of at most 11 significant bits, inv = 1 / s correctly
+// rounded: one correction by the exact residual leaves the quotient within an
+// ulp, and exact where fp32 holds it (ties among those); no other quotient of
+// such values is nearer than 2^-13 to a half.  Adding 1.5 * 2^23 rounds it
+// to a whole number, ties to even, in the low bits.
+__device__ __forceinline__ int round_quotient(float v, float s, float inv) {
+    const float q = v * inv;
+    const float r = fmaf(fmaf(-q, s, v), inv, q);
+    return __float_as_int(__fadd_rn(r, 12582912.f)) - 0x4B400000;
+}
+
+template <class T, int W, int GL /* lanes per group */, bool ZP>
 __global__ void __launch_bounds__(256)
     w4_quantize_kernel(const T* __restrict__ w, long long ldw, int N, int K, int S, int Q,
                        uint32_t* __restrict__ codes, __half* __restrict__ scales, uint8_t* __restrict__ zeros) {
     using U = typename Unit<W>::type;
     constexpr int kE = W / 2;  // elements per unit
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int lane = threadIdx.x & 31;
     const int s = blockIdx.x * 8 + (threadIdx.x >> 5), t = blockIdx.y;
     if (s >= S) return;
-    T v[2][4][8];
+    const int k0 = s * 128 + lane * 4;
+    union Four {
+        U u[4 / kE];
+        T e[4];
+        uint2 bits;
+    };
+    Four v[16];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int n = t * 16 + h * 8 + g;
-        const T* row = w + (size_t)min(n, N - 1) * ldw;
+    for (int r = 0; r < 16; ++r) {
+        const T* row = w + (size_t)min(t * 16 + r, N - 1) * ldw + k0;
+        v[r].bits = make_uint2(0u, 0u);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int i = 0; i < 4; i += kE) {
+            if (k0 + i + kE <= K) {
+                v[r].u[i / kE] = __ldg(reinterpret_cast<const U*>(row + i));
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; i += kE) {
-                const int k = s * 128 + 32 * j + 8 * c + i;
-                if (k + kE <= K) {
-                    *reinterpret_cast<U*>(&v[h][j][i]) = __ldg(reinterpret_cast<const U*>(row + k));
-                } else {
-#pragma unroll
-                    for (int ii = 0; ii < kE; ++ii) {
-                        const uint16_t zero = 0;
-                        v[h][j][i + ii] = k + ii < K ? row[k + ii] : *reinterpret_cast<const T*>(&zero);
-                    }
-                }
+                for (int ii = 0; ii < kE; ++ii)
+                    if (k0 + i + ii < K) v[r].e[i + ii] = row[i + ii];
             }
+        }
     }
+    const int gi = s * (32 / GL) + lane / GL;
+    uint32_t* word = codes + ((size_t)t * S + s) * 256 + ((lane >> 1) & 3) * 4 + (lane >> 3);  // + [h][4 g][.]
+    const size_t note = ((size_t)t * Q + gi) * 16;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t word[4];
+    for (int r = 0; r < 16; ++r) {
+        const int h = r >> 3, g = r & 7;
+        float f[4];
 #pragma unroll
-        for (int j0 = 0; j0 < 4; j0 += JG) {
-            float lo = 0.f, hi = 0.f;
+        for (int i = 0; i < 4; ++i) f[i] = to_f(v[r].e[i]);
+        float sc, z = 8.f;
+        __half sh;
+        if (ZP) {
+            float lo = fminf(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), 0.f);
+            float hi = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), 0.f);
 #pragma unroll
-            for (int j = j0; j < j0 + JG; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    lo = fminf(lo, to_f(v[h][j][i]));
-                    hi = fmaxf(hi, to_f(v[h][j][i]));
-                }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
+            for (int o = 1; o < GL; o <<= 1) {
                 lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
                 hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
             }
-            const __half sh = __float2half_rn(ZP ? __fdiv_rn(__fsub_rn(hi, lo), 15.0f) : __fdiv_rn(fmaxf(-lo, hi), 7.0f));
-            const float sc = __half2float(sh);
-            const bool some = sc > 0.f;
-            const float z = ZP && some ? fminf(fmaxf(rintf(__fdiv_rn(-lo, sc)), 0.f), 15.f) : 8.f;
+            sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
+            sc = __half2float(sh);
+            if (sc > 0.f) z = fminf(fmaxf(rintf(__fdiv_rn(-lo, sc)), 0.f), 15.f);
+        } else {
+            float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
 #pragma unroll
-            for (int j = j0; j < j0 + JG; ++j) {
-                uint32_t q = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float r = some ? __fadd_rn(rintf(__fdiv_rn(to_f(v[h][j][i]), sc)), z) : z;
-                    q |= (uint32_t)fminf(fmaxf(r, 0.f), 15.f) << (4 * ((i >> 1) + 4 * (i & 1)));
-                }
-                word[j] = q;
-            }
-            const int gi = s * (4 / JG) + j0 / JG;
-            if (c == 0 && gi < Q) {
-                const size_t at = (((size_t)t * Q + gi) * 8 + g) * 2 + h;
-                scales[at] = sh;
-                if (ZP) zeros[at] = (uint8_t)z;
-            }
+            for (int o = 1; o < GL; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            sh = __float2half_rn(__fdiv_rn(top, 7.0f));
+            sc = __half2float(sh);
         }
-        reinterpret_cast<uint4*>(codes)[(((size_t)t * S + s) * 2 + h) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
+        const float inv = sc > 0.f ? __frcp_rn(sc) : 0.f;  // no scale: every code is the zero point
+        const int zi = (int)z;
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = (uint32_t)min(max(round_quotient(sc > 0.f ? f[i] : 0.f, sc, inv) + zi, 0), 15);
+        // inputs 0..3 of a word stand at 0, 4, 1, 5 (times four bits), 4..7 at 2, 6, 3, 7
+        uint32_t part = q[0] | q[1] << 16 | q[2] << 4 | q[3] << 20;
+        part = (lane & 1) ? part << 8 : part;
+        part |= __shfl_xor_sync(0xffffffffu, part, 1);
+        if (!(lane & 1)) word[h * 128 + g * 16] = part;
+        if (lane % GL == 0 && gi < Q) {
+            scales[note + g * 2 + h] = sh;
+            if (ZP) zeros[note + g * 2 + h] = (uint8_t)zi;
+        }
     }
 }
 
+// Lane l writes inputs (W / 4) l .. of each block of 8 W inputs.
 template <int W>
 __global__ void __launch_bounds__(256)
     w4_dequantize_kernel(const uint32_t* __restrict__ codes, const __half* __restrict__ scales,
-                         const uint8_t* __restrict__ zeros, int N, int K, int S, int Q, int jg, float* __restrict__ out,
-                         long long ldo) {
+                         const uint8_t* __restrict__ zeros, int N, int K, int S, int Q, int lg /* log2 group */,
+                         float* __restrict__ out, long long ldo) {
     using U = typename Unit<W>::type;
-    constexpr int kE = W / 4;
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    constexpr int kE = W / 4, kB = 4 / kE;  // values per unit, units per lane and row
+    const int lane = threadIdx.x & 31;
     const int s = blockIdx.x * 8 + (threadIdx.x >> 5), t = blockIdx.y;
     if (s >= S) return;
+    const uint32_t* span = codes + ((size_t)t * S + s) * 256;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int n = t * 16 + h * 8 + g;
-        const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(codes) + (((size_t)t * S + s) * 2 + h) * 32 + lane);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-        if (n >= N) continue;
+    for (int h = 0; h < 2; ++h)
+#pragma unroll 4
+        for (int g = 0; g < 8; ++g) {
+            const int n = t * 16 + h * 8 + g;
+            if (n >= N) break;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int gi = s * (4 / jg) + j / jg;
-            if (gi >= Q) continue;
-            const size_t at = (((size_t)t * Q + gi) * 8 + g) * 2 + h;
-            const float sc = __half2float(scales[at]), z = zeros ? (float)(zeros[at] & 15) : 8.f;
-            float v[8];
+            for (int b = 0; b < kB; ++b) {
+                const int kk = b * 32 * kE + lane * kE, k = s * 128 + kk;  // inside the span, inside the row
+                if (k >= K) continue;
+                const uint32_t w = __ldg(span + h * 128 + (g * 4 + ((kk >> 3) & 3)) * 4 + (kk >> 5));
+                const size_t at = ((size_t)t * Q + (k >> lg)) * 16 + g * 2 + h;
+                const float sc = __half2float(scales[at]), z = zeros ? (float)(zeros[at] & 15) : 8.f;
+                union {
+                    U u;
+                    float f[kE];
+                } v;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = ((float)((w[j] >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) - z) * sc;
-            const int k = s * 128 + 32 * j + 8 * c;
-            float* to = out + (size_t)n * ldo + k;
-#pragma unroll
-            for (int i = 0; i < 8; i += kE) {
-                if (k + i + kE <= K) {
-                    *reinterpret_cast<U*>(to + i) = *reinterpret_cast<const U*>(v + i);
+                for (int i = 0; i < kE; ++i) {
+                    const int ii = (kk & 7) + i;
+                    v.f[i] = ((float)((w >> (4 * ((ii >> 1) + 4 * (ii & 1)))) & 15u) - z) * sc;
+                }
+                float* to = out + (size_t)n * ldo + k;
+                if (k + kE <= K) {
+                    *reinterpret_cast<U*>(to) = v.u;
                 } else {
 #pragma unroll
-                    for (int ii = 0; ii < kE; ++ii)
-                        if (k + i + ii < K) to[i + ii] = v[i + ii];
+                    for (int i = 0; i < kE; ++i)
+                        if (k + i < K) to[i] = v.f[i];
                 }
             }
         }
-    }
 }
 
 // ------------------------------------------------------------------ launching
@@ -729,7 +749,7 @@ int unit_bytes(const void* p, long long ld_bytes, int most) {
     return w;
 }
 
-template <class T, int W, int JG>
+template <class T, int W, int GL>
 void quantize_zp(const w4_matrix& m, const void* w, long long ldw, dim3 grid, int S, int Q, int tile0, cudaStream_t st) {
     const T* src = static_cast<const T*>(w) + (size_t)tile0 * 16 * ldw;
     uint32_t* codes = static_cast<uint32_t*>(m.codes) + (size_t)tile0 * S * 256;
@@ -737,24 +757,24 @@ void quantize_zp(const w4_matrix& m, const void* w, long long ldw, dim3 grid, in
     uint8_t* zeros = static_cast<uint8_t*>(m.zeros);
     const int N = m.n - tile0 * 16;
     if (zeros)
-        w4_quantize_kernel<T, W, JG, true><<<grid, 256, 0, st>>>(src, ldw, N, m.k, S, Q, codes, scales, zeros + (size_t)tile0 * Q * 16);
+        w4_quantize_kernel<T, W, GL, true><<<grid, 256, 0, st>>>(src, ldw, N, m.k, S, Q, codes, scales, zeros + (size_t)tile0 * Q * 16);
     else
-        w4_quantize_kernel<T, W, JG, false><<<grid, 256, 0, st>>>(src, ldw, N, m.k, S, Q, codes, scales, nullptr);
+        w4_quantize_kernel<T, W, GL, false><<<grid, 256, 0, st>>>(src, ldw, N, m.k, S, Q, codes, scales, nullptr);
 }
 
 template <class T, int W>
-void quantize_jg(const w4_matrix& m, const void* w, long long ldw, dim3 grid, int S, int Q, int tile0, cudaStream_t st) {
-    if (m.group == 128) quantize_zp<T, W, 4>(m, w, ldw, grid, S, Q, tile0, st);
-    else if (m.group == 64) quantize_zp<T, W, 2>(m, w, ldw, grid, S, Q, tile0, st);
-    else quantize_zp<T, W, 1>(m, w, ldw, grid, S, Q, tile0, st);
+void quantize_group(const w4_matrix& m, const void* w, long long ldw, dim3 grid, int S, int Q, int tile0, cudaStream_t st) {
+    if (m.group == 128) quantize_zp<T, W, 32>(m, w, ldw, grid, S, Q, tile0, st);
+    else if (m.group == 64) quantize_zp<T, W, 16>(m, w, ldw, grid, S, Q, tile0, st);
+    else quantize_zp<T, W, 8>(m, w, ldw, grid, S, Q, tile0, st);
 }
 
 template <class T>
 void quantize_w(const w4_matrix& m, const void* w, long long ldw, dim3 grid, int S, int Q, int tile0, cudaStream_t st) {
-    const int u = unit_bytes(w, ldw * 2, 16);
-    if (u == 16) quantize_jg<T, 16>(m, w, ldw, grid, S, Q, tile0, st);
-    else if (u >= 4) quantize_jg<T, 4>(m, w, ldw, grid, S, Q, tile0, st);
-    else quantize_jg<T, 2>(m, w, ldw, grid, S, Q, tile0, st);
+    const int u = unit_bytes(w, ldw * 2, 8);
+    if (u == 8) quantize_group<T, 8>(m, w, ldw, grid, S, Q, tile0, st);
+    else if (u >= 4) quantize_group<T, 4>(m, w, ldw, grid, S, Q, tile0, st);
+    else quantize_group<T, 2>(m, w, ldw, grid, S, Q, tile0, st);
 }
 
 constexpr int kMaxGridY = 65535;  // tiles per launch
@@ -774,7 +794,8 @@ cudaError_t launch_w4_quantize(const w4_matrix& m, const void* w, int dtype, lon
 }
 
 cudaError_t launch_w4_dequantize(const w4_matrix& m, float* out, long long ldo, cudaStream_t st) {
-    const int T = (m.n + 15) / 16, S = (m.k + 127) / 128, Q = (m.k + m.group - 1) / m.group, jg = m.group / 32;
+    const int T = (m.n + 15) / 16, S = (m.k + 127) / 128, Q = (m.k + m.group - 1) / m.group;
+    const int lg = m.group == 128 ? 7 : m.group == 64 ? 6 : 5;
     const int u = unit_bytes(out, ldo * 4, 16);
     auto fn = u == 16 ? w4_dequantize_kernel<16> : u == 8 ? w4_dequantize_kernel<8> : w4_dequantize_kernel<4>;
     for (int t0 = 0; t0 < T; t0 += kMaxGridY) {
@@ -782,7 +803,7 @@ cudaError_t launch_w4_dequantize(const w4_matrix& m, float* out, long long ldo, 
         const uint8_t* zeros = static_cast<const uint8_t*>(m.zeros);
         fn<<<grid, 256, 0, st>>>(static_cast<const uint32_t*>(m.codes) + (size_t)t0 * S * 256,
                                  static_cast<const __half*>(m.scales) + (size_t)t0 * Q * 16,
-                                 zeros ? zeros + (size_t)t0 * Q * 16 : nullptr, m.n - t0 * 16, m.k, S, Q, jg,
+                                 zeros ? zeros + (size_t)t0 * Q * 16 : nullptr, m.n - t0 * 16, m.k, S, Q, lg,
                                  out + (size_t)t0 * 16 * ldo, ldo);
         const cudaError_t e = counted(cudaGetLastError());
         if (e != cudaSuccess) return e;
