@@ -202,6 +202,49 @@ int qw2_submit(qw2_model* m, const qw2_request* request, int* job);
 int qw2_wait(qw2_model* m, int job, int timeout_ms, int* out_ids, int out_cap, qw2_result* result);
 int qw2_cancel(qw2_model* m, int session);
 
+/* ------------------------------------------------------- 4-bit weights
+ * Every projection and lm_head brought to 4 bits (w4_quantize of step_ops.h,
+ * group 32, 64 or 128, with zero points where asked), once all tensors are
+ * set; the fp16 matrices but the embedding are freed.  From then on forwards
+ * multiply the 4-bit values with the same fp16 inputs, fp32 sums and
+ * epilogues.  KV_ERR_STATE while a request runs, a second time, or together
+ * with qw2_set_exact; matrices cannot be set afterwards.  On failure (no
+ * memory) the model is unchanged. */
+int qw2_quantize_weights(qw2_model* m, int group, int zero_points);
+
+/* ------------------------------------------------------------ controls
+ * Called on the host before each choice of a session that has it: `ids` are
+ * the n_ids ids in the session's cache (from gen_from on: generated), `allowed`
+ * the mask to fill (n_words words, bit t % 32 of word t / 32, all set on
+ * entry).  Return 1 to use it, 0 for no mask at this step, < 0 to fail the
+ * session's request (its token is in the cache by then).  It runs under the model's lock and must not call the model. */
+typedef int (*qw2_mask_cb)(void* user, int session, const int* ids, int n_ids, int gen_from, uint32_t* allowed,
+                           int n_words);
+
+/* What a session's choices go through before the largest logit is taken, in
+ * the order and arithmetic of logits_adjust (step_ops.h).  The history is the
+ * ids in the session's cache; its generated part is the running request's
+ * output (for qw2_forward: the ids forwarded one at a time since the last
+ * longer forward). */
+typedef struct qw2_controls {
+    float repetition_penalty; /* > 0, 1: none */
+    float presence_penalty;   /* 0: none */
+    float frequency_penalty;  /* 0: none */
+    int n_bias;
+    const int* bias_ids;
+    const float* bias;
+    const uint32_t* allowed;  /* ceil(vocab / 32) words, or NULL: every token */
+    qw2_mask_cb mask_cb;      /* or NULL; joined with `allowed` */
+    void* user;
+} qw2_controls;
+
+/* Give `session` controls (copied), or none (NULL).  They hold for
+ * qw2_forward*, generate and async calls until changed or the session is
+ * destroyed.  Logits read back stay the model's own; only the choice (argmax)
+ * changes.  Where a mask leaves nothing, the choice is -1 and a generation
+ * ends as at a stop token (hit_stop). */
+int qw2_set_controls(qw2_model* m, int session, const qw2_controls* controls);
+
 /* Bytes of weights one decode step reads (all projections + lm_head). */
 int qw2_weight_bytes(const qw2_model* m, long long* bytes);
 

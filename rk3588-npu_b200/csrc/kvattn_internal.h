@@ -317,17 +317,19 @@ struct DeviceGuard {
     }
 };
 
-// Raises a kernel's dynamic shared memory limit once per device.
+// Raises a kernel's dynamic shared memory limit (and allows clusters of 16)
+// once per device.
 struct SmemGrant {
     static constexpr int kDevices = 64;
     std::atomic<bool> done[kDevices];
-    cudaError_t raise(const void* fn, int bytes) {
+    cudaError_t raise(const void* fn, int bytes, bool cluster16 = false) {
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
         if (dev < 0 || dev >= kDevices) return cudaErrorInvalidDevice;
         if (done[dev].load()) return cudaSuccess;
         e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && cluster16) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e == cudaSuccess) done[dev].store(true);
         return e;
     }

@@ -37,6 +37,8 @@
 #include "kvattn.h"
 #include "kvattn_internal.h"
 #include "qwen2_engine.h"
+#include "step_ops.h"
+#include "w4_internal.h"
 
 using namespace kvattn;
 
@@ -101,7 +103,8 @@ struct Job {
     qw2_token_cb cb = nullptr;
     void* user = nullptr;
     std::vector<int> out;
-    int next = 0;                 // greedy choice of the last forward
+    int next = 0;                 // the choice of the last forward (-1: a mask left nothing)
+    int gen_from = 0;             // this request's generated ids start here in the session's history
     int step = 0;                 // decode step (loop counter of the reference)
     bool prefilled = false;
     bool decoding = false;        // `next` is pushed and waits for its forward
@@ -112,6 +115,16 @@ struct Job {
 };
 
 }  // namespace
+
+// A session's controls (qw2_set_controls), owned copies.
+struct Controls {
+    float repetition = 1.f, presence = 0.f, frequency = 0.f;
+    std::vector<int> bias_ids;
+    std::vector<float> bias;
+    std::vector<uint32_t> allowed;  // empty: no fixed mask
+    qw2_mask_cb mask_cb = nullptr;
+    void* user = nullptr;
+};
 
 struct qw2_model {
     int device = 0;
@@ -125,6 +138,13 @@ struct qw2_model {
     int rows_cap = 0;              // rows of one forward (activation buffers)
     std::vector<int> session_seq;  // session -> pool sequence id, -1 = free
     std::vector<char> session_busy;  // an async request runs on it
+    std::vector<std::vector<int>> session_ids;  // the ids in its cache, in order
+    std::vector<int> session_gen;    // ids from here on came one at a time (taken as generated)
+    std::vector<std::unique_ptr<Controls>> controls;  // per session, NULL: none
+    float* adjusted = nullptr;       // [S][V] logits after the controls, allocated with the first of them
+    int* pick = nullptr;             // [S]
+    void* ctl_dev = nullptr;         // the controls' lists of one step, on the device
+    size_t ctl_cap = 0;
 
     // async engine
     std::mutex mu;                 // one model operation at a time
@@ -146,12 +166,16 @@ struct qw2_model {
         uint16_t* wg = nullptr;    // [IS][H]
         uint16_t* wu = nullptr;    // [IS][H]
         uint16_t* wd = nullptr;    // [H][IS]
+        // the same in 4 bits (qw2_quantize_weights), in place of those
+        w4_matrix qqkv{}, qo{}, qg{}, qu{}, qd{};
         bool have[F_COUNT] = {};
     };
     std::vector<Layer> L;
     uint16_t* embed = nullptr;  // [V][H], also lm_head
     float* norm = nullptr;
     bool have_embed = false, have_norm = false;
+    int w4_group = 0;           // > 0: the projections are in 4 bits
+    w4_matrix qhead{};          // lm_head in 4 bits (the lookup keeps the fp16 embedding)
 
     // activations, up to max_position rows
     float* hidden = nullptr;  // [R][H]
@@ -189,6 +213,12 @@ struct qw2_model {
     template <class T>
     int alloc_n(T** p, size_t n) {
         return alloc(reinterpret_cast<void**>(p), n * sizeof(T));
+    }
+    void drop(void* p) {
+        auto it = std::find(allocs.begin(), allocs.end(), p);
+        if (it == allocs.end()) return;
+        cudaFree(p);
+        allocs.erase(it);
     }
     void release() {
         for (void* p : allocs) cudaFree(p);
@@ -428,7 +458,157 @@ struct Group {
     int n = 0;
     float* logits_host = nullptr;  // [vocab] or NULL
     int argmax = 0;
+    bool choose = true;            // the choice is used (the last chunk of a prompt, a decode step)
+    int gen_from = -1;             // history index of the first generated id, -1: the session's own rule
+    int status = KV_OK;            // the choice's own failure (a mask callback's)
 };
+
+// The body of a call with host allocations: no exception leaves it.
+template <class F>
+int guarded(F f) {
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        return qfail(KV_ERR_OOM, "host memory: %s", e.what());
+    }
+}
+
+// After a forward: the groups' ids join their sessions' histories.
+void note_ids(qw2_model* m, const std::vector<Group>& gs) {
+    for (const Group& g : gs) {
+        std::vector<int>& h = m->session_ids[g.session];
+        h.insert(h.end(), g.tokens, g.tokens + g.n);
+        if (g.n > 1) m->session_gen[g.session] = (int)h.size();
+    }
+}
+
+// The choices of the groups whose session has controls, in place of the plain
+// argmax: row i of m->logits belongs to gs[order[i]].  The histories include
+// this forward's ids.  Returns after the stream's work on them.
+int choose_controlled(qw2_model* m, std::vector<Group>& gs, const std::vector<int>& order) {
+    std::vector<int> rows;  // rows of m->logits with controls
+    for (int i = 0; i < (int)order.size(); ++i)
+        if (gs[order[i]].choose && m->controls[gs[order[i]].session]) rows.push_back(i);
+    if (rows.empty()) return KV_OK;
+    const int V = m->c.vocab, words = (V + 31) / 32, R = (int)rows.size();
+    std::vector<int> hist, hist_off(1, 0), gen_from, bias_ids, bias_off(1, 0);
+    std::vector<float> rep, pres, freq, bias;
+    std::vector<uint32_t> mask;
+    bool any_mask = false;
+    for (int i : rows) {
+        const Group& g = gs[order[i]];
+        const Controls& c = *m->controls[g.session];
+        const std::vector<int>& ids = m->session_ids[g.session];
+        hist.insert(hist.end(), ids.begin(), ids.end());
+        hist_off.push_back((int)hist.size());
+        gen_from.push_back(g.gen_from >= 0 ? g.gen_from : m->session_gen[g.session]);
+        rep.push_back(c.repetition);
+        pres.push_back(c.presence);
+        freq.push_back(c.frequency);
+        bias_ids.insert(bias_ids.end(), c.bias_ids.begin(), c.bias_ids.end());
+        bias.insert(bias.end(), c.bias.begin(), c.bias.end());
+        bias_off.push_back((int)bias_ids.size());
+        const size_t at = mask.size();
+        mask.resize(at + words, 0xFFFFFFFFu);
+        if (!c.allowed.empty()) {
+            std::copy(c.allowed.begin(), c.allowed.end(), mask.begin() + at);
+            any_mask = true;
+        }
+        if (c.mask_cb) {
+            std::vector<uint32_t> step(words, 0xFFFFFFFFu);
+            const int rc = c.mask_cb(c.user, g.session, ids.data(), (int)ids.size(), gen_from.back(), step.data(), words);
+            if (rc < 0) gs[order[i]].status = qfail(KV_ERR_STATE, "mask callback of session %d failed (%d)", g.session, rc);
+            if (rc > 0) {
+                for (int w = 0; w < words; ++w) mask[at + w] &= step[w];
+                any_mask = true;
+            }
+        }
+    }
+    if (!any_mask) mask.clear();
+    // one upload of all lists
+    std::vector<uint8_t> up;
+    auto put = [&](const void* p, size_t bytes) {
+        const size_t at = (up.size() + 15) / 16 * 16;
+        up.resize(at + bytes);
+        if (bytes) memcpy(up.data() + at, p, bytes);
+        return at;
+    };
+    const size_t o_hist = put(hist.data(), hist.size() * 4), o_off = put(hist_off.data(), hist_off.size() * 4),
+                 o_gen = put(gen_from.data(), R * 4), o_rep = put(rep.data(), R * 4), o_pres = put(pres.data(), R * 4),
+                 o_freq = put(freq.data(), R * 4), o_bid = put(bias_ids.data(), bias_ids.size() * 4),
+                 o_bias = put(bias.data(), bias.size() * 4), o_boff = put(bias_off.data(), bias_off.size() * 4),
+                 o_mask = put(mask.data(), mask.size() * 4);
+    cudaStream_t st = m->st;
+    if (up.size() > m->ctl_cap) {
+        QW_CUDA(cudaStreamSynchronize(st));
+        if (m->ctl_dev) m->drop(m->ctl_dev);
+        m->ctl_dev = nullptr;
+        m->ctl_cap = 0;
+        const size_t cap = up.size() * 2;
+        QW_OK(m->alloc(&m->ctl_dev, cap));
+        m->ctl_cap = cap;
+    }
+    QW_CUDA(cudaMemcpyAsync(m->ctl_dev, up.data(), up.size(), cudaMemcpyHostToDevice, st));
+    const uint8_t* d = static_cast<const uint8_t*>(m->ctl_dev);
+    auto i32 = [&](size_t o) { return reinterpret_cast<const int*>(d + o); };
+    auto f32 = [&](size_t o) { return reinterpret_cast<const float*>(d + o); };
+    // runs of consecutive rows, usually one
+    for (int a = 0; a < R;) {
+        int b = a + 1;
+        while (b < R && rows[b] == rows[b - 1] + 1) ++b;
+        logits_call q{};
+        q.device = m->device;
+        q.rows = b - a;
+        q.vocab = V;
+        q.dtype = STEP_F32;
+        q.logits = m->logits + (size_t)rows[a] * V;
+        q.out = m->adjusted + (size_t)rows[a] * V;
+        q.ld_logits = q.ld_out = V;
+        q.pick = m->pick + rows[a];
+        q.hist = i32(o_hist);
+        q.hist_off = i32(o_off) + a;
+        q.hist_n = (long long)hist.size();
+        q.gen_from = i32(o_gen) + a;
+        q.repetition = f32(o_rep) + a;
+        q.presence = f32(o_pres) + a;
+        q.frequency = f32(o_freq) + a;
+        if (!bias.empty()) {
+            q.bias_ids = i32(o_bid);
+            q.bias = f32(o_bias);
+            q.bias_off = i32(o_boff) + a;
+            q.bias_n = (long long)bias.size();
+        }
+        if (any_mask) {
+            q.mask = reinterpret_cast<const uint32_t*>(d + o_mask) + (size_t)a * words;
+            q.ld_mask = words;
+        }
+        QW_OK(logits_adjust(&q, st));
+        a = b;
+    }
+    std::vector<int> pick(order.size());
+    QW_CUDA(cudaMemcpyAsync(pick.data(), m->pick, sizeof(int) * order.size(), cudaMemcpyDeviceToHost, st));
+    QW_CUDA(cudaStreamSynchronize(st));
+    for (int i : rows) gs[order[i]].argmax = pick[i];
+    return KV_OK;
+}
+
+// One projection of the forward: on the fp16 matrices of `a`, or on their
+// 4-bit forms.
+cudaError_t project(const qw2_model* m, int mode, int in, const GemvArgs& a, const w4_matrix& q, const w4_matrix* q2,
+                    cudaStream_t st) {
+    if (!m->w4_group) return launch_gemv(mode, in, a, st);
+    W4Args w;
+    w.set_matrix(0, q);
+    if (q2) w.set_matrix(1, *q2);
+    w.M = a.M;
+    w.x = a.x;
+    w.ldx = a.K;
+    w.in = in == 0 ? W4_X_16 : in == 1 ? W4_X_ROUND : W4_X_NORM;
+    w.mode = mode;  // the launch_gemv modes
+    w.g = a;
+    w.early = true;
+    return launch_w4(w, q.group, /*bf16*/ false, q2 ? 2 : 1, st);
+}
 
 // The float inputs where this process's C library expf (the exp the
 // reference's loops call) differs from the correctly rounded exponential --
@@ -559,7 +739,12 @@ int forward_exact(qw2_model* m, std::vector<Group>& gs) {
     if (status != 0) return status;
     for (int g = 0; g < G; ++g)
         gs[g].argmax = keys[g] ? (int)(0xFFFFFFFFu - (uint32_t)(keys[g] & 0xFFFFFFFFu)) : 0;
-    return KV_OK;
+    return guarded([&] {
+        note_ids(m, gs);
+        std::vector<int> order(G);
+        for (int g = 0; g < G; ++g) order[g] = g;
+        return choose_controlled(m, gs, order);
+    });
 }
 
 // Qwen2Model::forward (qwen2_model.cpp:131-274) over several sessions at
@@ -643,7 +828,7 @@ int forward_groups(qw2_model* m, std::vector<Group>& gs) {
         a.out2 = m->v;
         a.n0 = H;
         a.n1 = kvd;
-        QW_CUDA(launch_gemv(0, 2, a, st));
+        QW_CUDA(project(m, 0, 2, a, Ly.qqkv, nullptr, st));
         // 3-5: RoPE, KV append, attention
         if (nD) QW_OK(attn_decode_append(m->pool, li, m->q, m->k, m->v, m->attn, st));
         if (nD < G) {
@@ -661,7 +846,7 @@ int forward_groups(qw2_model* m, std::vector<Group>& gs) {
         o.M = rows;
         o.x = m->attn;
         o.resid = m->hidden;
-        QW_CUDA(launch_gemv(1, 1, o, st));
+        QW_CUDA(project(m, 1, 1, o, Ly.qo, nullptr, st));
         // 8-10: post-attention RMSNorm fused into gate/up (+ SiLU product), down + residual
         GemvArgs gu;
         gu.w = Ly.wg;
@@ -673,7 +858,7 @@ int forward_groups(qw2_model* m, std::vector<Group>& gs) {
         gu.norm_w = Ly.ln2;
         gu.eps = c.rms_eps;
         gu.out16 = m->h16;
-        QW_CUDA(launch_gemv(2, 2, gu, st));
+        QW_CUDA(project(m, 2, 2, gu, Ly.qg, &Ly.qu, st));
         GemvArgs d;
         d.w = Ly.wd;
         d.N = H;
@@ -681,7 +866,7 @@ int forward_groups(qw2_model* m, std::vector<Group>& gs) {
         d.M = rows;
         d.x = m->h16;
         d.resid = m->hidden;
-        QW_CUDA(launch_gemv(1, 0, d, st));
+        QW_CUDA(project(m, 1, 0, d, Ly.qd, nullptr, st));
     }
     if (nD) QW_OK(attn_decode_commit(m->pool));
     for (int i = nD; i < G; ++i) QW_OK(kvp_seq_set_len(m->pool, seq[order[i]], pos[order[i]] + gs[order[i]].n));
@@ -701,7 +886,7 @@ int forward_groups(qw2_model* m, std::vector<Group>& gs) {
     lm.norm_w = m->norm;
     lm.eps = c.rms_eps;
     lm.logits = m->logits;
-    QW_CUDA(launch_gemv(3, 2, lm, st));
+    QW_CUDA(project(m, 3, 2, lm, m->qhead, nullptr, st));
     QW_CUDA(launch_argmax(m->logits, c.vocab, G, m->best, st));
     std::vector<unsigned long long> keys(G);
     QW_CUDA(cudaMemcpyAsync(keys.data(), m->best, sizeof(unsigned long long) * G, cudaMemcpyDeviceToHost, st));
@@ -716,7 +901,10 @@ int forward_groups(qw2_model* m, std::vector<Group>& gs) {
         const unsigned long long key = keys[i];
         gs[order[i]].argmax = key ? (int)(0xFFFFFFFFu - (uint32_t)(key & 0xFFFFFFFFu)) : 0;
     }
-    return KV_OK;
+    return guarded([&] {
+        note_ids(m, gs);
+        return choose_controlled(m, gs, order);
+    });
 }
 
 using Clock = std::chrono::steady_clock;
@@ -739,6 +927,11 @@ void job_finish(Job& j, int status) {
 // forward is due.
 void job_advance(Job& j) {
     if (j.step >= j.max_new) {
+        job_finish(j, KV_OK);
+        return;
+    }
+    if (j.next < 0) {  // a mask left no token: the end of what it allows
+        j.res.hit_stop = 1;
         job_finish(j, KV_OK);
         return;
     }
@@ -780,6 +973,7 @@ int engine_step(qw2_model* m, std::vector<Job*>& jobs) {
             g.session = j->session;
             g.tokens = &j->out.back();
             g.n = 1;
+            g.gen_from = j->gen_from;
             gs.push_back(g);
             gj.push_back(j);
             ++rows;
@@ -794,6 +988,9 @@ int engine_step(qw2_model* m, std::vector<Job*>& jobs) {
         g.session = j->session;
         g.tokens = j->input.data();
         g.n = n;
+        g.choose = n == (int)j->input.size();
+        g.gen_from = (int)m->session_ids[j->session].size() + n;  // nothing generated yet
+        j->gen_from = g.gen_from;
         gs.push_back(g);
         gj.push_back(j);
         rows += n;
@@ -806,6 +1003,10 @@ int engine_step(qw2_model* m, std::vector<Job*>& jobs) {
     }
     for (size_t i = 0; i < gs.size(); ++i) {
         Job& j = *gj[i];
+        if (gs[i].status != KV_OK) {  // only its own request fails
+            job_finish(j, gs[i].status);
+            continue;
+        }
         j.next = gs[i].argmax;
         if (!j.prefilled) {
             j.input.erase(j.input.begin(), j.input.begin() + gs[i].n);
@@ -973,6 +1174,9 @@ int qw2_create_kv(int device, const qw2_config* cfg, int max_sessions, int kv_dt
     m->rows_cap = cfg->max_position + max_sessions;
     m->session_seq.assign(max_sessions, -1);
     m->session_busy.assign(max_sessions, 0);
+    m->session_ids.resize(max_sessions);
+    m->session_gen.assign(max_sessions, 0);
+    m->controls.resize(max_sessions);
     const size_t H = cfg->hidden, kvd = m->kvd, IS = cfg->intermediate, V = cfg->vocab, R = m->rows_cap,
                  S = max_sessions;
     int rc = KV_OK;
@@ -1038,6 +1242,8 @@ int qw2_create(int device, const qw2_config* cfg, qw2_model** out) {
 int qw2_set_exact(qw2_model* m, int on) {
     if (!m) return qfail(KV_ERR_INVAL, "NULL model");
     std::lock_guard<std::mutex> lk(m->mu);
+    if (on && m->w4_group)
+        return qfail(KV_ERR_STATE, "the reference-order forward needs the fp16 weights, which were brought to 4 bits");
     if (on && m->kv_dtype != KV_F16)
         return qfail(KV_ERR_INVAL, "the reference-order forward needs the fp16 KV cache (the reference's)");
     if (on && !m->ex_x16) {
@@ -1086,6 +1292,7 @@ int qw2_set_tensor(qw2_model* m, const char* name, int dtype, const int64_t* sha
     std::lock_guard<std::mutex> lk(m->mu);
     Target t;
     QW_OK(resolve(m, name, &t));
+    if (t.matrix && m->w4_group) return qfail(KV_ERR_STATE, "tensor '%s': the matrices were brought to 4 bits", name);
     const bool shape_ok = t.matrix ? (ndim == 2 && shape[0] == t.rows && shape[1] == t.cols)
                                    : (ndim == 1 && shape[0] == t.rows);
     if (!shape_ok)
@@ -1199,6 +1406,8 @@ int qw2_reset(qw2_model* m) {
         QW_OK(kvp_seq_free(m->pool, m->session_seq[0]));  // other sessions keep their blocks
     }
     QW_OK(kvp_seq_alloc(m->pool, &m->session_seq[0]));
+    m->session_ids[0].clear();
+    m->session_gen[0] = 0;
     QW_CUDA(cudaStreamSynchronize(m->st));
     return KV_OK;
 }
@@ -1211,6 +1420,9 @@ int qw2_session_create(qw2_model* m, int* session) {
     for (int s = 0; s < m->max_sessions; ++s)
         if (m->session_seq[s] < 0) {
             QW_OK(kvp_seq_alloc(m->pool, &m->session_seq[s]));
+            m->session_ids[s].clear();
+            m->session_gen[s] = 0;
+            m->controls[s].reset();
             *session = s;
             return KV_OK;
         }
@@ -1264,7 +1476,7 @@ int qw2_forward_session(qw2_model* m, int session, const int* tokens, int n, flo
     gs[0].logits_host = logits_host;
     QW_OK(forward_groups(m, gs));
     if (argmax) *argmax = gs[0].argmax;
-    return KV_OK;
+    return gs[0].status;
 }
 
 int qw2_forward(qw2_model* m, const int* tokens, int n, float* logits_host, int* argmax) {
@@ -1379,8 +1591,118 @@ int qw2_kv_pool(qw2_model* m, kvp_pool** pool) {
     return KV_OK;
 }
 
+int qw2_quantize_weights(qw2_model* m, int group, int zero_points) {
+    if (!m) return qfail(KV_ERR_INVAL, "NULL model");
+    std::lock_guard<std::mutex> lk(m->mu);
+    {
+        std::lock_guard<std::mutex> qk(m->qmu);
+        for (char b : m->session_busy)
+            if (b) return qfail(KV_ERR_STATE, "a session has a running request");
+    }
+    size_t bytes[3];
+    QW_OK(w4_sizes(m->c.hidden, m->c.hidden, group, &bytes[0], &bytes[1], &bytes[2]));  // checks the group
+    if (m->w4_group) return qfail(KV_ERR_STATE, "the weights are in 4 bits already");
+    if (m->exact) return qfail(KV_ERR_STATE, "the reference-order forward needs the fp16 weights");
+    QW_OK(qw2_ready(m));
+    DeviceGuard g(m->device);
+    const int H = m->c.hidden, kvd = m->kvd, IS = m->c.intermediate, V = m->c.vocab;
+    struct Item {
+        w4_matrix* q;
+        uint16_t** w;
+        int n, k;
+    };
+    std::vector<Item> items;
+    for (auto& Ly : m->L) {
+        items.push_back({&Ly.qqkv, &Ly.wqkv, H + 2 * kvd, H});
+        items.push_back({&Ly.qo, &Ly.wo, H, H});
+        items.push_back({&Ly.qg, &Ly.wg, IS, H});
+        items.push_back({&Ly.qu, &Ly.wu, IS, H});
+        items.push_back({&Ly.qd, &Ly.wd, H, IS});
+    }
+    items.push_back({&m->qhead, &m->embed, V, H});
+    // all of the 4-bit matrices first: without room for them nothing changes
+    const size_t before = m->allocs.size();
+    int rc = KV_OK;
+    for (Item& it : items) {
+        w4_matrix q{m->device, it.n, it.k, group, nullptr, nullptr, nullptr};
+        w4_sizes(it.n, it.k, group, &bytes[0], &bytes[1], &bytes[2]);
+        rc = m->alloc(&q.codes, bytes[0]);
+        if (rc == KV_OK) rc = m->alloc(&q.scales, bytes[1]);
+        if (rc == KV_OK && zero_points) rc = m->alloc(&q.zeros, bytes[2]);
+        if (rc == KV_OK) rc = w4_quantize(&q, *it.w, STEP_F16, it.k, m->st);
+        if (rc != KV_OK) break;
+        *it.q = q;
+    }
+    if (rc == KV_OK) {
+        const cudaError_t e = cudaStreamSynchronize(m->st);
+        if (e != cudaSuccess) rc = qfail(KV_ERR_CUDA, "quantising the weights: %s", cudaGetErrorString(e));
+    }
+    if (rc != KV_OK) {
+        cudaStreamSynchronize(m->st);
+        while (m->allocs.size() > before) {
+            cudaFree(m->allocs.back());
+            m->allocs.pop_back();
+        }
+        for (Item& it : items) *it.q = w4_matrix{};
+        return rc;
+    }
+    m->w4_group = group;
+    for (Item& it : items)
+        if (*it.w != m->embed) {
+            m->drop(*it.w);
+            *it.w = nullptr;
+        }
+    return KV_OK;
+}
+
+int qw2_set_controls(qw2_model* m, int session, const qw2_controls* c) {
+    if (!m) return qfail(KV_ERR_INVAL, "NULL model");
+    std::lock_guard<std::mutex> lk(m->mu);
+    QW_OK(session_check(m, session));
+    if (!c) {
+        m->controls[session].reset();
+        return KV_OK;
+    }
+    if (!(c->repetition_penalty > 0.f) || !std::isfinite(c->repetition_penalty) || !std::isfinite(c->presence_penalty) ||
+        !std::isfinite(c->frequency_penalty))
+        return qfail(KV_ERR_INVAL, "penalties have to be finite, the repetition penalty above 0");
+    if (c->n_bias < 0 || (c->n_bias > 0 && (!c->bias_ids || !c->bias))) return qfail(KV_ERR_INVAL, "malformed bias list");
+    std::unique_ptr<Controls> k;
+    QW_OK(guarded([&] {
+        k.reset(new Controls());
+        if (c->n_bias > 0) {
+            k->bias_ids.assign(c->bias_ids, c->bias_ids + c->n_bias);
+            k->bias.assign(c->bias, c->bias + c->n_bias);
+        }
+        if (c->allowed) k->allowed.assign(c->allowed, c->allowed + (m->c.vocab + 31) / 32);
+        return KV_OK;
+    }));
+    k->repetition = c->repetition_penalty;
+    k->presence = c->presence_penalty;
+    k->frequency = c->frequency_penalty;
+    k->mask_cb = c->mask_cb;
+    k->user = c->user;
+    if (!m->adjusted) {
+        DeviceGuard g(m->device);
+        if (!m->pick) QW_OK(m->alloc_n(&m->pick, m->max_sessions));
+        QW_OK(m->alloc_n(&m->adjusted, (size_t)m->max_sessions * m->c.vocab));
+    }
+    m->controls[session] = std::move(k);
+    return KV_OK;
+}
+
 int qw2_weight_bytes(const qw2_model* m, long long* bytes) {
     if (!m || !bytes) return qfail(KV_ERR_INVAL, "NULL argument");
+    if (m->w4_group) {
+        auto of = [](const w4_matrix& q) {
+            size_t b[3];
+            w4_sizes(q.n, q.k, q.group, &b[0], &b[1], &b[2]);
+            return (long long)(b[0] + b[1] + (q.zeros ? b[2] : 0));
+        };
+        *bytes = of(m->qhead);
+        for (const auto& Ly : m->L) *bytes += of(Ly.qqkv) + of(Ly.qo) + of(Ly.qg) + of(Ly.qu) + of(Ly.qd);
+        return KV_OK;
+    }
     const long long H = m->c.hidden, kvd = m->kvd, IS = m->c.intermediate, V = m->c.vocab;
     const long long per_layer = (H + 2 * kvd) * H + H * H + 3 * IS * H;
     *bytes = 2 * (per_layer * m->c.layers + V * H);

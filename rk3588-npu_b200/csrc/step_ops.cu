@@ -81,17 +81,6 @@ int check_rows(const w4_matrix& w, const void* x, int x_dtype, int m, long long 
     return KV_OK;
 }
 
-void set_matrix(W4Args& a, int i, const w4_matrix& w) {
-    a.codes[i] = static_cast<const uint32_t*>(w.codes);
-    a.scales[i] = static_cast<const __half*>(w.scales);
-    a.zeros[i] = static_cast<const uint8_t*>(w.zeros);
-    a.N = w.n;
-    a.K = w.k;
-    a.T = (w.n + 15) / 16;
-    a.S = (w.k + 127) / 128;
-    a.Q = (w.k + w.group - 1) / w.group;
-}
-
 void set_x(W4Args& a, const void* x, int x_dtype, int m, long long ldx) {
     a.x = x;
     a.ldx = ldx;
@@ -154,7 +143,7 @@ int w4_linear(const w4_matrix* w, const void* x, int x_dtype, int m, long long l
     DeviceGuard g(w->device);
     if (!g.ok) return sfail(KV_ERR_INVAL, "no CUDA device %d", w->device);
     W4Args a;
-    set_matrix(a, 0, *w);
+    a.set_matrix(0, *w);
     set_x(a, x, x_dtype, m, ldx);
     a.mode = W4_LINEAR;
     a.bias = bias;
@@ -178,8 +167,8 @@ int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dt
     DeviceGuard g(gate->device);
     if (!g.ok) return sfail(KV_ERR_INVAL, "no CUDA device %d", gate->device);
     W4Args a;
-    set_matrix(a, 0, *gate);
-    set_matrix(a, 1, *up);
+    a.set_matrix(0, *gate);
+    a.set_matrix(1, *up);
     set_x(a, x, x_dtype, m, ldx);
     a.mode = W4_GATED;
     a.out = out;

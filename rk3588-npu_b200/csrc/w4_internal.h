@@ -43,6 +43,17 @@ struct W4Args {
     int chunk = 0;            // spans of x staged at a time
     int last_groups = 0;      // groups of a row's last span
     bool early = false;       // the weights may be read before the previous kernel of the stream ends
+
+    void set_matrix(int i, const w4_matrix& w) {
+        codes[i] = static_cast<const uint32_t*>(w.codes);
+        scales[i] = static_cast<const __half*>(w.scales);
+        zeros[i] = static_cast<const uint8_t*>(w.zeros);
+        N = w.n;
+        K = w.k;
+        T = (w.n + 15) / 16;
+        S = (w.k + 127) / 128;
+        Q = (w.k + w.group - 1) / w.group;
+    }
 };
 
 constexpr int kSms = 148;

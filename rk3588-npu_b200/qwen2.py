@@ -137,6 +137,15 @@ class Qw2Request(C.Structure):
                 ("on_token", TOKEN_CB), ("user", C.c_void_p)]
 
 
+MASK_CB = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.POINTER(C.c_int), C.c_int, C.c_int, C.POINTER(C.c_uint32), C.c_int)
+
+
+class Qw2Controls(C.Structure):
+    _fields_ = [("repetition_penalty", C.c_float), ("presence_penalty", C.c_float), ("frequency_penalty", C.c_float),
+                ("n_bias", C.c_int), ("bias_ids", C.POINTER(C.c_int)), ("bias", C.POINTER(C.c_float)),
+                ("allowed", C.POINTER(C.c_uint32)), ("mask_cb", MASK_CB), ("user", C.c_void_p)]
+
+
 _SIGS = {
     "qw2_config_default": [C.POINTER(Qw2Config)],
     "qw2_create_sessions": [C.c_int, C.POINTER(Qw2Config), C.c_int, C.POINTER(C.c_void_p)],
@@ -167,6 +176,8 @@ _SIGS = {
     "qw2_weight_bytes": [C.c_void_p, C.POINTER(C.c_longlong)],
     "qw2_set_stream": [C.c_void_p, C.c_void_p],
     "qw2_set_exact": [C.c_void_p, C.c_int],
+    "qw2_quantize_weights": [C.c_void_p, C.c_int, C.c_int],
+    "qw2_set_controls": [C.c_void_p, C.c_int, C.POINTER(Qw2Controls)],
 }
 
 
@@ -200,6 +211,7 @@ class Model:
         self.h = h
         self.cfg = dict(cfg)
         self._keep = {}  # ctypes objects an async job still points at
+        self._callbacks = {}  # mask callbacks of the sessions' controls
 
     def close(self) -> None:
         if self.h:
@@ -344,6 +356,54 @@ class Model:
 
     def cancel(self, session: int) -> None:
         _check(self.L.qw2_cancel(self.h, session), "qw2_cancel")
+
+    def quantize_weights(self, group: int = 128, zero_points: bool = False) -> None:
+        """qw2_quantize_weights: every projection and lm_head in 4 bits from now on."""
+        _check(self.L.qw2_quantize_weights(self.h, group, int(zero_points)), "qw2_quantize_weights")
+
+    def set_controls(self, session: int = 0, repetition_penalty: float = 1.0, presence_penalty: float = 0.0,
+                     frequency_penalty: float = 0.0, bias: dict | None = None, allowed=None, mask=None) -> None:
+        """qw2_set_controls: penalties, {id: value} biases and a grammar mask on
+        the session's choices.  `allowed`: a bool array over the vocabulary (or
+        uint32 words of it); `mask(session, ids, gen_from)`: called before each
+        choice, returns such an array or None."""
+        bias = dict(bias or {})
+        ids = _ints(list(bias))
+        vals = (C.c_float * max(1, len(bias)))(*bias.values())
+        fixed = None if allowed is None else self._mask_words(allowed)
+
+        def call(user, s, tokens, n, gen_from, out, n_words):
+            try:
+                got = mask(s, [tokens[i] for i in range(n)], gen_from)
+                if got is None:
+                    return 0
+                C.memmove(out, self._mask_words(got).ctypes.data, n_words * 4)
+                return 1
+            except Exception:  # no exception may leave a C callback
+                return -1
+
+        cb = MASK_CB(call) if mask is not None else MASK_CB()
+        c = Qw2Controls(repetition_penalty, presence_penalty, frequency_penalty, len(bias), ids, vals,
+                        fixed.ctypes.data_as(C.POINTER(C.c_uint32)) if fixed is not None else None, cb, None)
+        _check(self.L.qw2_set_controls(self.h, session, C.byref(c)), "qw2_set_controls")
+        self._callbacks[session] = cb
+
+    def clear_controls(self, session: int = 0) -> None:
+        _check(self.L.qw2_set_controls(self.h, session, None), "qw2_set_controls")
+        self._callbacks.pop(session, None)
+
+    def _mask_words(self, allowed) -> np.ndarray:
+        a, vocab = np.asarray(allowed), self.cfg["vocab"]
+        words = (vocab + 31) // 32
+        if a.dtype == np.bool_:
+            if a.shape != (vocab,):
+                raise ValueError(f"allowed: {a.shape}, expected ({vocab},)")
+            bits = np.zeros(words * 32, np.uint8)
+            bits[:vocab] = a
+            return np.packbits(bits, bitorder="little").view(np.uint32)
+        if a.dtype != np.uint32 or a.shape != (words,):
+            raise ValueError(f"allowed: {words} uint32 words or {vocab} booleans are expected")
+        return np.ascontiguousarray(a)
 
     def weight_bytes(self) -> int:
         b = C.c_longlong()
