@@ -90,6 +90,11 @@ int w4_linear(const w4_matrix* w, const void* x, int x_dtype, int m, long long l
 int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dtype, int m, long long ldx, void* out,
              int out_dtype, long long ldo, void* stream);
 
+/* The waits inside the kernels for many rows are bounded (about a second):
+ * *status is KV_OK, or KV_ERR_TIMEOUT if one has run out on `device` since the
+ * last call (that launch's outputs are not written).  Synchronises the device. */
+int step_ops_status(int device, int* status);
+
 /* Penalties, biases, a mask and the greedy choice on `rows` rows of logits.
  * For row r and token t, in fp32, each step rounded by itself:
  *   l = logits[r][t]

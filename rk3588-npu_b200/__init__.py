@@ -117,6 +117,7 @@ _SIGS.update({
     "w4_linear": [_w4p, _vp, C.c_int, C.c_int, C.c_longlong, _vp, _vp, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp],
     "w4_gated": [_w4p, _w4p, _vp, C.c_int, C.c_int, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp],
     "logits_adjust": [C.POINTER(_LogitsCall), _vp],
+    "step_ops_status": [C.c_int, _ip],
 })
 _RESTYPE = {"kv_last_error": C.c_char_p, "kv_status_str": C.c_char_p, "kv_version": C.c_char_p}
 
@@ -555,6 +556,13 @@ def w4_gated(gate: W4, up: W4, x, out, stream=None) -> None:
                        _step_dtype(out, "out"), ldo, _stream_on(stream, dev))
     if rc:
         _check(rc, "w4_gated")
+
+
+def step_ops_status(device: int = 0) -> int:
+    """KV_OK, or KV_ERR_TIMEOUT if a bounded wait ran out since the last call (synchronises the device)."""
+    s = C.c_int()
+    call("step_ops_status", device, C.byref(s))
+    return s.value
 
 
 def logits_adjust(logits, out, pick=None, hist=None, hist_off=None, gen_from=None, repetition=None, presence=None,

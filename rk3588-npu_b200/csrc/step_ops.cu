@@ -177,6 +177,15 @@ int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dt
     return launched(launch_w4(a, gate->group, x_dtype != STEP_F16, 2, static_cast<cudaStream_t>(stream)), "w4_gated");
 }
 
+int step_ops_status(int device, int* status) {
+    if (!status || device < 0) return sfail(KV_ERR_INVAL, "NULL status or no device");
+    DeviceGuard g(device);
+    if (!g.ok) return sfail(KV_ERR_INVAL, "no CUDA device %d", device);
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = step_status(status);
+    return launched(e, "step_ops_status");
+}
+
 int logits_adjust(const logits_call* c, void* stream) {
     if (!c) return sfail(KV_ERR_INVAL, "NULL call");
     ST_OK(check_dtype(c->dtype, "logits"));

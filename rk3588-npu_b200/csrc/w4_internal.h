@@ -56,6 +56,7 @@ struct W4Args {
     }
 };
 
+constexpr int kW4TcRows = 64;
 constexpr int kSms = 148;
 constexpr int kW4MaxSmem = 227 * 1024;
 // Spans that a warp copies at a time (two such batches in shared memory).
@@ -95,7 +96,33 @@ inline W4Plan w4_plan(int M, int T, int S, int pieces, int nw, int sms) {
     return p;
 }
 
+// The tcgen05 form's plan: tiles of 128 weight rows (64 of each matrix of a
+// gated block) x nb operand rows of x.
+struct W4TcPlan {
+    int nb, rows, cs, gx, gy;
+};
+
+inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw, int sms) {
+    W4TcPlan p{};
+    auto rows_of = [&](int nb) { return pieces == 3 ? nb / 2 / 3 * 2 : nb; };
+    p.nb = M <= rows_of(64) ? 64 : 128;
+    p.rows = rows_of(p.nb);
+    p.gy = (M + p.rows - 1) / p.rows;
+    const int per = nw == 2 ? 4 : 8;
+    p.gx = (T + per - 1) / per;
+    // CTAs that share a tile's inputs: as the SMs allow, with four spans or more each
+    p.cs = std::max(1, std::min(std::min(8, S / 4), sms / std::max(1, p.gx * p.gy)));
+    return p;
+}
+
+// Rows from which the tcgen05 form is the faster one.
+inline bool w4_use_tc(int M, int pieces) { return M * pieces > kW4TcRows; }
+
 cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st);
+cudaError_t launch_w4_tc(W4Args a, int group, bool bf, int nw, cudaStream_t st);
+// The status of the waits in launch_w4_tc's kernels on the current device
+// (0, or KV_ERR_TIMEOUT), cleared by reading it.
+cudaError_t step_status(int* status);
 cudaError_t launch_w4_quantize(const w4_matrix& m, const void* w, int dtype, long long ldw, cudaStream_t st);
 cudaError_t launch_w4_dequantize(const w4_matrix& m, float* out, long long ldo, cudaStream_t st);
 cudaError_t launch_logits(const logits_call& c, cudaStream_t st);

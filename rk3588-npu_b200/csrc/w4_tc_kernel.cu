@@ -1,0 +1,450 @@
+// w4_tc_kernel.cu -- the 4-bit projections for many rows of x, on tcgen05.
+//
+// The same sums as w4_kernels.cu (integers q - z exact in the operand type,
+// a group's products summed in fp32, the scale applied to the sum), with the
+// roles of a tile spread over the warps of one CTA:
+//   warps 0-3   unpack codes into the A operand: 128 weight rows x 128 inputs
+//               in shared memory, 128-byte-swizzled K-major;
+//   warps 4-6   bring the B operand: kNB rows of x x 128 inputs, the same
+//               layout (16-bit rows by cp.async; fp32 rows rounded, or split
+//               into their three bf16 parts, on the way);
+//   warp 7      issues the MMAs: each group of inputs into a fresh sum in
+//               tensor memory, two of them in turn;
+//   warps 8-15  read a finished group (lane = weight row) and add it, times
+//               the row's scale, to fp32 sums in registers, while the next
+//               group is multiplied.
+// So the matrix instructions run back to back while the scaling, which they
+// cannot do, follows a group behind.  A gated block's tile is 64 gate rows and
+// the 64 up rows of the same outputs, which meet in shared memory at the end.
+// Few tiles: a cluster of CTAs shares a tile's inputs and adds its sums by
+// DSMEM in rank order.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "device_common.cuh"
+#include "kvattn.h"
+#include "kvattn_internal.h"
+#include "projection.cuh"
+#include "step_ops.h"
+#include "tcgen05.cuh"
+#include "w4_device.cuh"
+#include "w4_internal.h"
+
+namespace kvattn {
+
+namespace {
+
+constexpr int kStages = 3;
+constexpr int kThreads = 16 * 32;
+constexpr int kBWarps = 3, kMmaWarp = 7;
+constexpr int kHalfA = 128 * 128;  // 64 inputs of 128 rows
+constexpr long long kWaitLimit = 2000000000LL;  // SM clocks: about a second
+
+template <int NB>
+struct Smem {
+    static constexpr int kHalfB = NB * 128;
+    static constexpr int kStage = 2 * kHalfA + 2 * kHalfB;
+    static constexpr int kRed = NB * 128 * 4;  // [column][row] sums, over the stages
+    static constexpr int kBytes = 1024 + (kStages * kStage > kRed ? kStages * kStage : kRed);
+};
+
+struct Bars {
+    uint64_t full_a[kStages], full_b[kStages], empty[kStages], sum_full[2], sum_empty[2];
+    uint32_t tmem;
+    int failed;
+};
+
+__device__ int g_step_status;  // KV_ERR_TIMEOUT once a wait has run out
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Bars* b) {
+    if (mbar_wait_bounded(bar, parity, kWaitLimit)) return true;
+    atomicCAS(&g_step_status, 0, KV_ERR_TIMEOUT);
+    *reinterpret_cast<volatile int*>(&b->failed) = 1;
+    return false;
+}
+
+// The same for a whole warp: all of its lanes, or none, go on.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Bars* b) {
+    const bool ok = wait(bar, parity, b) && !*reinterpret_cast<volatile int*>(&b->failed);
+    return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// BF: bf16 operands (else fp16).  GP: groups per span.  NB: columns (operand
+// rows of x) of a tile.  GATED: two matrices.
+template <int BF, int GP, int NB, bool GATED>
+__global__ void __launch_bounds__(kThreads, 1)
+    w4_tc_kernel(const __grid_constant__ W4Args a) {
+    using SM = Smem<NB>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ Bars bars;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int cs = a.cs, rank = (int)blockIdx.x % cs;
+    const int tile0 = (int)blockIdx.x / cs * (GATED ? 4 : 8);  // first 16-row tile
+    const int m0 = blockIdx.y * a.rows, mrows = min(a.rows, a.M - m0);
+    const int s0 = (int)((long long)a.S * rank / cs), s1 = (int)((long long)a.S * (rank + 1) / cs);
+    // column of part p of row m: the three parts of an fp32 row stay in one half of the columns
+    const int per_half = a.pieces == 3 ? NB / 2 / 3 : NB / 2;  // rows per half
+    auto column = [&](int m, int p) { return m / per_half * (NB / 2) + m % per_half * a.pieces + p; };
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&bars.full_a[i], 4);
+            mbar_init(&bars.full_b[i], kBWarps);
+            mbar_init(&bars.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars.sum_full[i], 1);
+            mbar_init(&bars.sum_empty[i], 8);
+        }
+        bars.failed = 0;
+    }
+    fence_mbar_init();
+    if (warp == kMmaWarp) {
+        tmem_alloc(&bars.tmem, 2 * NB);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars.tmem;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    // tile i (0..7) of the CTA's rows
+    auto tile_of = [&](int i) { return min(tile0 + (GATED ? i & 3 : i), a.T - 1); };
+    auto mat_of = [&](int i) { return GATED ? i >> 2 : 0; };
+    auto flushes = [&](int sp) { return sp == a.S - 1 ? a.last_groups : GP; };
+
+    if (warp < 4) {
+        // ---------------------------------------------------- A: unpack codes
+        const int g = lane >> 2, c = lane & 3, odd = g & 1;
+        const uint8_t* src[2];
+        const uint8_t* zp[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int t = warp * 2 + i, q = mat_of(t);
+            src[i] = reinterpret_cast<const uint8_t*>(a.codes[q]) + ((size_t)tile_of(t) * a.S + s0) * 1024 + lane * 16;
+            zp[i] = a.zeros[q] ? a.zeros[q] + (size_t)tile_of(t) * a.Q * 16 + g * 2 : nullptr;
+        }
+        // odd rows take the words of a pair in the other order, so that eight
+        // lanes' stores fall into eight different 16-byte columns
+        const uint32_t row0 = (uint32_t)(warp * 32 + g) * 128;
+        const uint32_t chunk[2] = {(uint32_t)((odd * 4 + c) ^ g) << 4, (uint32_t)(((odd ^ 1) * 4 + c) ^ g) << 4};
+        uint4 next[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) next[i][h] = __ldg(reinterpret_cast<const uint4*>(src[i] + h * 512));
+        uint2 z[2] = {zero_consts<BF>(8u), zero_consts<BF>(8u)};
+        for (int sp = s0; sp < s1; ++sp) {
+            const int it = sp - s0, st = it % kStages;
+            uint4 w[2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    w[i][h] = next[i][h];
+                    src[i] += h * 1024;
+                    if (h == 1 && sp + 1 < s1) {
+                        next[i][0] = __ldg(reinterpret_cast<const uint4*>(src[i]));
+                        next[i][1] = __ldg(reinterpret_cast<const uint4*>(src[i] + 512));
+                    }
+                }
+            if (it >= kStages && !wait_warp(&bars.empty[st], (it / kStages - 1) & 1, &bars)) break;
+            uint8_t* dst = smem + st * SM::kStage + row0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t zz[GP];
+#pragma unroll
+                for (int q = 0; q < GP; ++q)
+                    zz[q] = zp[i] && sp * GP + q < a.Q ? *reinterpret_cast<const uint16_t*>(zp[i] + (size_t)(sp * GP + q) * 16) : 0x0808u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t v[4] = {odd ? w[i][h].y : w[i][h].x, odd ? w[i][h].x : w[i][h].y,
+                                           odd ? w[i][h].w : w[i][h].z, odd ? w[i][h].z : w[i][h].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        // word j of the lane is inputs 32 (j ^ odd) ..
+                        const int qa = j / (4 / GP), qb = (j ^ 1) / (4 / GP);
+                        if (j == 0 || GP == 4 || (GP == 2 && j == 2)) z[0] = zero_consts<BF>(((qa == qb || !odd ? zz[qa] : zz[qb]) >> (8 * h)) & 15u);
+                        uint32_t p[4];
+                        unpack<BF>(v[j], z[0], p);
+                        *reinterpret_cast<uint4*>(dst + (j >> 1) * kHalfA + (i * 16 + h * 8) * 128 + chunk[j & 1]) =
+                            make_uint4(p[0], p[1], p[2], p[3]);
+                    }
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.full_a[st]);
+        }
+    } else if (warp < 4 + kBWarps) {
+        // --------------------------------------------------------- B: rows of x
+        const int t = tid - 128;
+        const bool wide = (reinterpret_cast<size_t>(a.x) & 15) == 0 && (a.ldx * (a.in == W4_X_16 ? 2 : 4)) % 16 == 0;
+        int held = -1;  // a stage whose cp.async is in flight
+        auto release = [&](int st) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.full_b[st]);
+        };
+        for (int sp = s0; sp < s1; ++sp) {
+            const int it = sp - s0, st = it % kStages;
+            if (it >= kStages && !wait_warp(&bars.empty[st], (it / kStages - 1) & 1, &bars)) break;
+            uint8_t* dst = smem + st * SM::kStage + 2 * kHalfA;
+            const int k0 = sp * 128;
+            if (a.in == W4_X_16) {
+                const int c = t & 7;  // 16-byte column of both halves
+#pragma unroll 4
+                for (int r = t >> 3; r < NB; r += kBWarps * 4) {
+                    const uint16_t* row = static_cast<const uint16_t*>(a.x) + (size_t)(m0 + min(r, mrows - 1)) * a.ldx + k0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int k = h * 64 + c * 8;
+                        uint8_t* to = dst + h * SM::kHalfB + swz(r, c);
+                        if (wide && k0 + k + 8 <= a.K) {
+                            cp16(smem_u32(to), row + k);
+                        } else {
+                            uint32_t e[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) e[j] = k0 + k + j < a.K ? (uint32_t)__ldg(row + k + j) : 0u;
+                            *reinterpret_cast<uint4*>(to) = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+                        }
+                    }
+                }
+                cp_commit();
+                if (held >= 0) {
+                    cp_wait<1>();
+                    release(held);
+                }
+                held = st;
+                continue;
+            }
+            // fp32 rows: eight inputs at a time; rows past the last repeat it
+            const int units = (a.pieces == 3 ? 2 * per_half : NB) * 16;
+#pragma unroll 2
+            for (int u = t; u < units; u += kBWarps * 32) {
+                const int m = u >> 4, c = u & 15, k = c * 8;
+                const float* row = static_cast<const float*>(a.x) + (size_t)(m0 + min(m, mrows - 1)) * a.ldx + k0 + k;
+                float v[8];
+                if (wide && k0 + k + 8 <= a.K) {
+                    const float4 f = __ldg(reinterpret_cast<const float4*>(row)), e = __ldg(reinterpret_cast<const float4*>(row) + 1);
+                    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = e.x, v[5] = e.y, v[6] = e.z, v[7] = e.w;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = k0 + k + j < a.K ? __ldg(row + j) : 0.f;
+                }
+                uint8_t* half = dst + (c >> 3) * SM::kHalfB;
+                if (a.pieces == 3) {
+                    uint16_t p[3][8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) split3(v[j], p[0][j], p[1][j], p[2][j]);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q)
+                        *reinterpret_cast<uint4*>(half + swz(column(m, q), c & 7)) =
+                            make_uint4(p[q][0] | (uint32_t)p[q][1] << 16, p[q][2] | (uint32_t)p[q][3] << 16,
+                                       p[q][4] | (uint32_t)p[q][5] << 16, p[q][6] | (uint32_t)p[q][7] << 16);
+                } else {
+                    uint32_t e[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) e[j] = enc_f16_trunc(v[j]);
+                    *reinterpret_cast<uint4*>(half + swz(m, c & 7)) =
+                        make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+                }
+            }
+            release(st);
+        }
+        if (held >= 0) {
+            cp_wait<0>();
+            release(held);
+        }
+    } else if (warp == kMmaWarp) {
+        // ----------------------------------------------------------- MMA issue
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_f16(BF, 128, NB, 0);
+            int f = 0;  // groups so far
+            bool ok = true;
+            for (int sp = s0; ok && sp < s1; ++sp) {
+                const int it = sp - s0, st = it % kStages;
+                ok = wait(&bars.full_a[st], (it / kStages) & 1, &bars) && wait(&bars.full_b[st], (it / kStages) & 1, &bars);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t sa = smem_u32(smem + st * SM::kStage), sb = sa + 2 * kHalfA;
+                const int nf = flushes(sp);
+                for (int q = 0; ok && q < nf; ++q, ++f) {
+                    const int buf = f & 1;
+                    if (f >= 2) {
+                        ok = wait(&bars.sum_empty[buf], (f / 2 - 1) & 1, &bars);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8 / GP; ++i) {
+                        const int kk = q * (8 / GP) + i;  // 16 inputs
+                        const uint32_t at = (uint32_t)(kk & 3) * 32;
+                        mma_ss(tmem + buf * NB, sdesc(sa + (kk >> 2) * kHalfA + at, 16, 1024),
+                               sdesc(sb + (kk >> 2) * SM::kHalfB + at, 16, 1024), idesc, i != 0);
+                    }
+                    tc_commit(&bars.sum_full[buf]);
+                }
+                tc_commit(&bars.empty[st]);
+            }
+        }
+        __syncwarp();
+    } else {
+        // -------------------------------------------------- scale and accumulate
+        const int quarter = warp & 3, half = (warp - 8) >> 2;
+        const int r = quarter * 32 + lane;  // weight row of the CTA
+        const __half* sc = a.scales[mat_of(r >> 4)] + (size_t)tile_of(r >> 4) * a.Q * 16 + (r & 7) * 2 + ((r >> 3) & 1);
+        float acc[NB / 2];
+#pragma unroll
+        for (int i = 0; i < NB / 2; ++i) acc[i] = 0.f;
+        const int g0 = s0 * GP, g1 = min(s1 * GP, a.Q);
+        float s = __half2float(sc[(size_t)g0 * 16]);
+        bool ok = true;
+        for (int gi = g0; ok && gi < g1; ++gi) {
+            const int f = gi - g0, buf = f & 1;
+            const float s_next = gi + 1 < g1 ? __half2float(sc[(size_t)(gi + 1) * 16]) : 0.f;
+            ok = wait_warp(&bars.sum_full[buf], (f / 2) & 1, &bars);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * NB + half * (NB / 2));
+#pragma unroll
+            for (int b = 0; b < NB / 64; ++b) {
+                float d[32];
+                tmem_ld32(at + b * 32, d);
+                tc_wait_ld();
+                if (b == NB / 64 - 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.sum_empty[buf]);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[b * 32 + i] = fmaf(s, d[i], acc[b * 32 + i]);
+            }
+            s = s_next;
+        }
+        // every MMA has read its operands: the stages become the sums
+        float* red = reinterpret_cast<float*>(smem) + (size_t)half * (NB / 2) * 128 + r;
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the other half's last group too
+        if (ok)
+#pragma unroll
+            for (int i = 0; i < NB / 2; ++i) red[i * 128] = acc[i];
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const bool failed = *reinterpret_cast<volatile int*>(&bars.failed) != 0;
+    if (warp == kMmaWarp) {
+        if (failed && lane == 0) {  // MMAs in flight end before their memory goes
+            mbar_init(&bars.full_a[0], 1);
+            fence_mbar_init();
+            tc_commit(&bars.full_a[0]);
+            mbar_wait_bounded(&bars.full_a[0], 0, kWaitLimit);
+        }
+        __syncwarp();
+        tmem_dealloc(tmem, 2 * NB);
+    }
+    if (cs > 1) cluster_sync();
+    // finished outputs: rows of the tile fastest
+    constexpr int kN = GATED ? 64 : 128;
+    if (!failed) {
+        const float* red = reinterpret_cast<const float*>(smem);
+        const int i = tid % kN, n = tile0 * 16 + i;
+        constexpr int kStep = kThreads / kN;
+        if (n < a.N)
+            for (int m = tid / kN + rank * kStep; m < mrows; m += cs * kStep) {
+                float y[2] = {0.f, 0.f};
+#pragma unroll
+                for (int q = 0; q < (GATED ? 2 : 1); ++q)
+                    for (int p = a.pieces - 1; p >= 0; --p) {  // the smallest parts first
+                        const float* at = red + column(m, p) * 128 + q * 64 + i;
+                        if (cs == 1) {
+                            y[q] += *at;
+                        } else {
+                            float v[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) v[k] = k < cs ? ld_cluster_f32(cluster_map(smem_u32(at), k)) : 0.f;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) y[q] += v[k];
+                        }
+                    }
+                w4_epilogue(a, m0 + m, n, y[0], y[1]);
+            }
+    }
+    if (cs > 1) cluster_sync();  // nobody leaves while its sums are read
+}
+
+template <int BF, int GP, int NB, bool GATED>
+cudaError_t launch_inst(const W4Args& a, int gx, int gy, cudaStream_t st) {
+    auto fn = w4_tc_kernel<BF, GP, NB, GATED>;
+    static SmemGrant grant;
+    cudaError_t e = grant.raise(reinterpret_cast<const void*>(fn), Smem<NB>::kBytes);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(gx * a.cs), (unsigned)gy);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Smem<NB>::kBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.cs;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cs > 1 ? 2 : 1;
+    return counted(cudaLaunchKernelEx(&cfg, fn, a));
+}
+
+template <int BF, int GP, int NB>
+cudaError_t launch_gated(const W4Args& a, bool gated, int gx, int gy, cudaStream_t st) {
+    return gated ? launch_inst<BF, GP, NB, true>(a, gx, gy, st) : launch_inst<BF, GP, NB, false>(a, gx, gy, st);
+}
+
+template <int BF, int GP>
+cudaError_t launch_nb(const W4Args& a, int nb, bool gated, int gx, int gy, cudaStream_t st) {
+    return nb == 64 ? launch_gated<BF, GP, 64>(a, gated, gx, gy, st) : launch_gated<BF, GP, 128>(a, gated, gx, gy, st);
+}
+
+template <int BF>
+cudaError_t launch_group(const W4Args& a, int group, int nb, bool gated, int gx, int gy, cudaStream_t st) {
+    if (group == 128) return launch_nb<BF, 1>(a, nb, gated, gx, gy, st);
+    if (group == 64) return launch_nb<BF, 2>(a, nb, gated, gx, gy, st);
+    return launch_nb<BF, 4>(a, nb, gated, gx, gy, st);
+}
+
+}  // namespace
+
+cudaError_t launch_w4_tc(W4Args a, int group, bool bf, int nw, cudaStream_t st) {
+    const W4TcPlan p = w4_tc_plan(a.M, a.T, a.S, a.pieces, nw, kSms);
+    a.rows = p.rows;
+    a.cs = p.cs;
+    a.last_groups = a.Q - (a.S - 1) * (128 / group);
+    return bf ? launch_group<1>(a, group, p.nb, nw == 2, p.gx, p.gy, st)
+              : launch_group<0>(a, group, p.nb, nw == 2, p.gx, p.gy, st);
+}
+
+cudaError_t step_status(int* status) {
+    cudaError_t e = cudaMemcpyFromSymbol(status, g_step_status, sizeof(int));
+    if (e != cudaSuccess) return e;
+    const int zero = 0;
+    if (*status) e = cudaMemcpyToSymbol(g_step_status, &zero, sizeof(int));
+    return e;
+}
+
+}  // namespace kvattn

@@ -125,6 +125,7 @@ def test_linear(kv, case):
         tol = tol + half_step(np.abs(want) + tol, yd)
         assert np.all(np.abs(dbl(out) - want) <= tol), np.max(np.abs(dbl(out) - want) / tol)
         assert torch.all(buf[:32] == 77.0) and torch.all(buf[32 + m * n:] == 77.0)
+    assert kv.step_ops_status() == kv.KV_OK
 
 
 GATED = [
