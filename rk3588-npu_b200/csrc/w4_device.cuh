@@ -97,6 +97,9 @@ __device__ __forceinline__ void store_as(void* p, size_t i, int dtype, float v) 
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
+// silu(g) u
+__device__ __forceinline__ float gated(float g, float u) { return __fdiv_rn(g, 1.0f + expf(-g)) * u; }
+
 __device__ __forceinline__ void w4_epilogue(const W4Args& a, int row, int n, float y, float y2) {
     switch (a.mode) {
         case W4_QKV: gemv_epilogue<0>(a.g, row, n, y, y2); break;
@@ -109,7 +112,7 @@ __device__ __forceinline__ void w4_epilogue(const W4Args& a, int row, int n, flo
             store_as(a.out, (size_t)row * a.ldo + n, a.out_dtype, y);
             break;
         default:
-            store_as(a.out, (size_t)row * a.ldo + n, a.out_dtype, __fdiv_rn(y, 1.0f + expf(-y)) * y2);
+            store_as(a.out, (size_t)row * a.ldo + n, a.out_dtype, gated(y, y2));
     }
 }
 

@@ -102,7 +102,7 @@ struct W4TcPlan {
     int nb, rows, cs, gx, gy;
 };
 
-inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw, int sms) {
+inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw) {
     W4TcPlan p{};
     auto rows_of = [&](int nb) { return pieces == 3 ? nb / 2 / 3 * 2 : nb; };
     p.nb = M <= rows_of(64) ? 64 : 128;
@@ -110,8 +110,12 @@ inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw, int sms) {
     p.gy = (M + p.rows - 1) / p.rows;
     const int per = nw == 2 ? 4 : 8;
     p.gx = (T + per - 1) / per;
-    // CTAs that share a tile's inputs: as the SMs allow, with four spans or more each
-    p.cs = std::max(1, std::min(std::min(8, S / 4), sms / std::max(1, p.gx * p.gy)));
+    // CTAs that share a tile's inputs: as many as fit the SMs in clusters (which
+    // do not cross a GPC: 16 of 8, 34 of 4, 72 of 2), with four spans or more each
+    p.cs = 1;
+    const int tiles = p.gx * p.gy;
+    for (int c = 2, fit = 72; c <= 8; c *= 2, fit = c == 4 ? 34 : 16)
+        if (tiles <= fit && S / c >= 4) p.cs = c;
     return p;
 }
 

@@ -36,7 +36,9 @@ namespace kvattn {
 
 namespace {
 
-constexpr int kStages = 3;
+constexpr int kStagesA = 2;   // written from registers, so little waits in them
+constexpr int kStagesB = 4;   // copies in flight
+constexpr int kAhead = 3;     // spans of codes in registers
 constexpr int kThreads = 16 * 32;
 constexpr int kBWarps = 3, kMmaWarp = 7;
 constexpr int kHalfA = 128 * 128;  // 64 inputs of 128 rows
@@ -45,13 +47,14 @@ constexpr long long kWaitLimit = 2000000000LL;  // SM clocks: about a second
 template <int NB>
 struct Smem {
     static constexpr int kHalfB = NB * 128;
-    static constexpr int kStage = 2 * kHalfA + 2 * kHalfB;
-    static constexpr int kRed = NB * 128 * 4;  // [column][row] sums, over the stages
-    static constexpr int kBytes = 1024 + (kStages * kStage > kRed ? kStages * kStage : kRed);
+    static constexpr int kB = kStagesA * 2 * kHalfA;  // where the B stages start
+    static constexpr int kRed = NB * 128 * 4;         // [column][row] sums, over the stages
+    static constexpr int kAll = kB + kStagesB * 2 * kHalfB;
+    static constexpr int kBytes = 1024 + (kAll > kRed ? kAll : kRed);
 };
 
 struct Bars {
-    uint64_t full_a[kStages], full_b[kStages], empty[kStages], sum_full[2], sum_empty[2];
+    uint64_t full_a[kStagesA], empty_a[kStagesA], full_b[kStagesB], empty_b[kStagesB], sum_full[2], sum_empty[2];
     uint32_t tmem;
     int failed;
 };
@@ -71,11 +74,22 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Bars* 
     return __all_sync(0xffffffffu, ok);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// D (+)= A B by the warp's leader.  The whole warp runs the loop around it, so
+// that the operands are uniform: issued from a branch of one lane, each MMA
+// waited for its operands' way to uniform registers (134 clocks a piece,
+// whatever its size).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
+        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader) {
+    asm volatile(
+        "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
+        " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)),
+        "r"(leader)
         : "memory");
 }
 
@@ -101,10 +115,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
-        for (int i = 0; i < kStages; ++i) {
+        for (int i = 0; i < kStagesA; ++i) {
             mbar_init(&bars.full_a[i], 4);
+            mbar_init(&bars.empty_a[i], 1);
+        }
+        for (int i = 0; i < kStagesB; ++i) {
             mbar_init(&bars.full_b[i], kBWarps);
-            mbar_init(&bars.empty[i], 1);
+            mbar_init(&bars.empty_b[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars.sum_full[i], 1);
@@ -143,28 +160,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         // lanes' stores fall into eight different 16-byte columns
         const uint32_t row0 = (uint32_t)(warp * 32 + g) * 128;
         const uint32_t chunk[2] = {(uint32_t)((odd * 4 + c) ^ g) << 4, (uint32_t)(((odd ^ 1) * 4 + c) ^ g) << 4};
-        uint4 next[2][2];
+        uint4 ring[kAhead][2][2];  // [span][tile][rows g, g + 8]
+        auto fetch = [&](uint4 (&to)[2][2]) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) next[i][h] = __ldg(reinterpret_cast<const uint4*>(src[i] + h * 512));
+                for (int h = 0; h < 2; ++h) to[i][h] = __ldg(reinterpret_cast<const uint4*>(src[i] + h * 512));
+                src[i] += 1024;
+            }
+        };
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d)
+            if (s0 + d < s1) fetch(ring[d]);
         uint2 z[2] = {zero_consts<BF>(8u), zero_consts<BF>(8u)};
-        for (int sp = s0; sp < s1; ++sp) {
-            const int it = sp - s0, st = it % kStages;
+        bool alive = true;
+        for (int sp0 = s0; alive && sp0 < s1; sp0 += kAhead) {
+#pragma unroll
+          for (int d = 0; d < kAhead; ++d) {
+            const int sp = sp0 + d;
+            if (sp >= s1) break;
+            const int it = sp - s0, st = it % kStagesA;
             uint4 w[2][2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    w[i][h] = next[i][h];
-                    src[i] += h * 1024;
-                    if (h == 1 && sp + 1 < s1) {
-                        next[i][0] = __ldg(reinterpret_cast<const uint4*>(src[i]));
-                        next[i][1] = __ldg(reinterpret_cast<const uint4*>(src[i] + 512));
-                    }
-                }
-            if (it >= kStages && !wait_warp(&bars.empty[st], (it / kStages - 1) & 1, &bars)) break;
-            uint8_t* dst = smem + st * SM::kStage + row0;
+                for (int h = 0; h < 2; ++h) w[i][h] = ring[d][i][h];
+            if (sp + kAhead < s1) fetch(ring[d]);
+            if (it >= kStagesA && !wait_warp(&bars.empty_a[st], (it / kStagesA - 1) & 1, &bars)) {
+                alive = false;
+                break;
+            }
+            uint8_t* dst = smem + st * (2 * kHalfA) + row0;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 uint32_t zz[GP];
@@ -190,55 +216,70 @@ __global__ void __launch_bounds__(kThreads, 1)
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.full_a[st]);
+          }
         }
     } else if (warp < 4 + kBWarps) {
         // --------------------------------------------------------- B: rows of x
+        // (columns without a row keep what is there: a column's sums are its own)
         const int t = tid - 128;
         const bool wide = (reinterpret_cast<size_t>(a.x) & 15) == 0 && (a.ldx * (a.in == W4_X_16 ? 2 : 4)) % 16 == 0;
-        int held = -1;  // a stage whose cp.async is in flight
+        constexpr int kLag = kStagesB - 1;  // copies in flight behind the newest
         auto release = [&](int st) {
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.full_b[st]);
         };
-        for (int sp = s0; sp < s1; ++sp) {
-            const int it = sp - s0, st = it % kStages;
-            if (it >= kStages && !wait_warp(&bars.empty[st], (it / kStages - 1) & 1, &bars)) break;
-            uint8_t* dst = smem + st * SM::kStage + 2 * kHalfA;
+        // 16-bit rows: this thread's 16-byte column c of rows r0 + 12 i; 12 rows
+        // on, the swizzle of a column differs in its third bit
+        const int c = t & 7, r0 = t >> 3;
+        const uint32_t to0 = (uint32_t)r0 * 128 + ((c ^ (r0 & 7)) << 4);
+        const uint16_t* x16 = static_cast<const uint16_t*>(a.x) + (size_t)m0 * a.ldx + c * 8;
+        int it = 0;
+        for (int sp = s0; sp < s1; ++sp, ++it) {
+            const int st = it % kStagesB;
+            if (it >= kStagesB && !wait_warp(&bars.empty_b[st], (it / kStagesB - 1) & 1, &bars)) break;
+            uint8_t* dst = smem + SM::kB + st * (2 * SM::kHalfB);
             const int k0 = sp * 128;
             if (a.in == W4_X_16) {
-                const int c = t & 7;  // 16-byte column of both halves
-#pragma unroll 4
-                for (int r = t >> 3; r < NB; r += kBWarps * 4) {
-                    const uint16_t* row = static_cast<const uint16_t*>(a.x) + (size_t)(m0 + min(r, mrows - 1)) * a.ldx + k0;
+                if (wide && k0 + 128 <= a.K) {
+                    const uint32_t to = smem_u32(dst) + to0;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int k = h * 64 + c * 8;
-                        uint8_t* to = dst + h * SM::kHalfB + swz(r, c);
-                        if (wide && k0 + k + 8 <= a.K) {
-                            cp16(smem_u32(to), row + k);
-                        } else {
+                    for (int i = 0; i < (NB + kBWarps * 4 - 1) / (kBWarps * 4); ++i) {
+                        const int r = r0 + i * kBWarps * 4;
+                        if (r < mrows) {
+                            const uint16_t* row = x16 + (size_t)r * a.ldx + k0;
+                            const uint32_t at = (to ^ ((uint32_t)(i & 1) << 6)) + i * (kBWarps * 4 * 128);
+                            cp16(at, row);
+                            cp16(at + SM::kHalfB, row + 64);
+                        }
+                    }
+                } else {
+                    for (int r = r0; r < mrows; r += kBWarps * 4) {
+                        const uint16_t* row = x16 + (size_t)r * a.ldx + k0;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int k = k0 + h * 64 + c * 8;
                             uint32_t e[8];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) e[j] = k0 + k + j < a.K ? (uint32_t)__ldg(row + k + j) : 0u;
-                            *reinterpret_cast<uint4*>(to) = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+                            for (int j = 0; j < 8; ++j) e[j] = k + j < a.K ? (uint32_t)__ldg(row + h * 64 + j) : 0u;
+                            *reinterpret_cast<uint4*>(dst + h * SM::kHalfB + swz(r, c)) =
+                                make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
                         }
                     }
                 }
                 cp_commit();
-                if (held >= 0) {
-                    cp_wait<1>();
-                    release(held);
+                if (it >= kLag) {
+                    cp_wait<kLag>();
+                    release((it - kLag) % kStagesB);
                 }
-                held = st;
                 continue;
             }
-            // fp32 rows: eight inputs at a time; rows past the last repeat it
-            const int units = (a.pieces == 3 ? 2 * per_half : NB) * 16;
+            // fp32 rows: eight inputs at a time
+            const int units = mrows * 16;
 #pragma unroll 2
             for (int u = t; u < units; u += kBWarps * 32) {
                 const int m = u >> 4, c = u & 15, k = c * 8;
-                const float* row = static_cast<const float*>(a.x) + (size_t)(m0 + min(m, mrows - 1)) * a.ldx + k0 + k;
+                const float* row = static_cast<const float*>(a.x) + (size_t)(m0 + m) * a.ldx + k0 + k;
                 float v[8];
                 if (wide && k0 + k + 8 <= a.K) {
                     const float4 f = __ldg(reinterpret_cast<const float4*>(row)), e = __ldg(reinterpret_cast<const float4*>(row) + 1);
@@ -267,41 +308,45 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             release(st);
         }
-        if (held >= 0) {
+        if (a.in == W4_X_16) {
             cp_wait<0>();
-            release(held);
+            for (int i = max(it - kLag, 0); i < it; ++i) release(i % kStagesB);
         }
     } else if (warp == kMmaWarp) {
         // ----------------------------------------------------------- MMA issue
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_f16(BF, 128, NB, 0);
-            int f = 0;  // groups so far
-            bool ok = true;
-            for (int sp = s0; ok && sp < s1; ++sp) {
-                const int it = sp - s0, st = it % kStages;
-                ok = wait(&bars.full_a[st], (it / kStages) & 1, &bars) && wait(&bars.full_b[st], (it / kStages) & 1, &bars);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t sa = smem_u32(smem + st * SM::kStage), sb = sa + 2 * kHalfA;
-                const int nf = flushes(sp);
-                for (int q = 0; ok && q < nf; ++q, ++f) {
-                    const int buf = f & 1;
-                    if (f >= 2) {
-                        ok = wait(&bars.sum_empty[buf], (f / 2 - 1) & 1, &bars);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
+        constexpr uint32_t idesc = idesc_f16(BF, 128, NB, 0);
+        const uint32_t leader = lane == 0;
+        const uint32_t base = smem_u32(smem);
+        int f = 0, sta = 0, stb = 0, pha = 0, phb = 0;  // groups so far; stages and their phases
+        bool ok = true;
+        for (int sp = s0; ok && sp < s1; ++sp) {
+            ok = wait_warp(&bars.full_b[stb], phb, &bars) && wait_warp(&bars.full_a[sta], pha, &bars);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t da = sdesc(base + sta * (2 * kHalfA), 16, 1024), db = sdesc(base + SM::kB + stb * (2 * SM::kHalfB), 16, 1024);
+            const int nf = flushes(sp);
 #pragma unroll
-                    for (int i = 0; i < 8 / GP; ++i) {
-                        const int kk = q * (8 / GP) + i;  // 16 inputs
-                        const uint32_t at = (uint32_t)(kk & 3) * 32;
-                        mma_ss(tmem + buf * NB, sdesc(sa + (kk >> 2) * kHalfA + at, 16, 1024),
-                               sdesc(sb + (kk >> 2) * SM::kHalfB + at, 16, 1024), idesc, i != 0);
-                    }
-                    tc_commit(&bars.sum_full[buf]);
+            for (int q = 0; q < GP; ++q) {
+                if (q >= nf) break;
+                const int buf = f & 1;
+                if (f >= 2) {
+                    ok = wait_warp(&bars.sum_empty[buf], (f / 2 - 1) & 1, &bars);
+                    if (!ok) break;
+                    tc_fence_after();
                 }
-                tc_commit(&bars.empty[st]);
+#pragma unroll
+                for (int i = 0; i < 8 / GP; ++i) {
+                    const int kk = q * (8 / GP) + i;  // 16 inputs: 32 bytes on (the descriptors count 16)
+                    mma_ss(tmem + buf * NB, da + ((kk >> 2) * kHalfA + (kk & 3) * 32) / 16,
+                           db + ((kk >> 2) * SM::kHalfB + (kk & 3) * 32) / 16, idesc, i != 0, leader);
+                }
+                commit(&bars.sum_full[buf], leader);
+                ++f;
             }
+            commit(&bars.empty_a[sta], leader);
+            commit(&bars.empty_b[stb], leader);
+            if (++sta == kStagesA) sta = 0, pha ^= 1;
+            if (++stb == kStagesB) stb = 0, phb ^= 1;
         }
         __syncwarp();
     } else {
@@ -359,31 +404,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_dealloc(tmem, 2 * NB);
     }
     if (cs > 1) cluster_sync();
-    // finished outputs: rows of the tile fastest
-    constexpr int kN = GATED ? 64 : 128;
-    if (!failed) {
-        const float* red = reinterpret_cast<const float*>(smem);
-        const int i = tid % kN, n = tile0 * 16 + i;
-        constexpr int kStep = kThreads / kN;
-        if (n < a.N)
-            for (int m = tid / kN + rank * kStep; m < mrows; m += cs * kStep) {
-                float y[2] = {0.f, 0.f};
+    // finished outputs: a thread keeps its output n and walks the rows of x
+    constexpr int kN = GATED ? 64 : 128, kStep = kThreads / kN;
+    const int i = tid % kN, n = tile0 * 16 + i;
+    if (!failed && n < a.N) {
+        const float* red = reinterpret_cast<const float*>(smem) + i;
+        // the finished sum of row m: its parts', the smallest first, over the cluster in rank order
+        auto sum_at = [&](const float* at) {
+            if (cs == 1) return *at;
+            float v[8], y = 0.f;
 #pragma unroll
-                for (int q = 0; q < (GATED ? 2 : 1); ++q)
-                    for (int p = a.pieces - 1; p >= 0; --p) {  // the smallest parts first
-                        const float* at = red + column(m, p) * 128 + q * 64 + i;
-                        if (cs == 1) {
-                            y[q] += *at;
-                        } else {
-                            float v[8];
+            for (int k = 0; k < 8; ++k) v[k] = k < cs ? ld_cluster_f32(cluster_map(smem_u32(at), k)) : 0.f;
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) v[k] = k < cs ? ld_cluster_f32(cluster_map(smem_u32(at), k)) : 0.f;
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) y[q] += v[k];
-                        }
-                    }
-                w4_epilogue(a, m0 + m, n, y[0], y[1]);
+            for (int k = 0; k < 8; ++k) y += v[k];
+            return y;
+        };
+        auto sum = [&](int m, int q) {
+            if (a.pieces == 1) return sum_at(red + m * 128 + q * 64);
+            const float* at = red + column(m, 0) * 128 + q * 64;
+            return sum_at(at + 256) + sum_at(at + 128) + sum_at(at);
+        };
+        const int step = cs * kStep;
+        if (a.mode == W4_LINEAR) {
+            const float bias = a.bias ? __ldg(a.bias + n) : 0.f;
+#pragma unroll 4
+            for (int m = tid / kN + rank * kStep; m < mrows; m += step) {
+                float y = sum(m, 0) + bias;
+                if (a.residual) y += load_as(a.residual, (size_t)(m0 + m) * a.ldr + n, a.out_dtype);
+                store_as(a.out, (size_t)(m0 + m) * a.ldo + n, a.out_dtype, y);
             }
+        } else if (a.mode == W4_GATED) {
+#pragma unroll 2
+            for (int m = tid / kN + rank * kStep; m < mrows; m += step)
+                store_as(a.out, (size_t)(m0 + m) * a.ldo + n, a.out_dtype, gated(sum(m, 0), sum(m, GATED ? 1 : 0)));
+        } else {
+            for (int m = tid / kN + rank * kStep; m < mrows; m += step)
+                w4_epilogue(a, m0 + m, n, sum(m, 0), sum(m, GATED ? 1 : 0));
+        }
     }
     if (cs > 1) cluster_sync();  // nobody leaves while its sums are read
 }
@@ -431,7 +488,7 @@ cudaError_t launch_group(const W4Args& a, int group, int nb, bool gated, int gx,
 }  // namespace
 
 cudaError_t launch_w4_tc(W4Args a, int group, bool bf, int nw, cudaStream_t st) {
-    const W4TcPlan p = w4_tc_plan(a.M, a.T, a.S, a.pieces, nw, kSms);
+    const W4TcPlan p = w4_tc_plan(a.M, a.T, a.S, a.pieces, nw);
     a.rows = p.rows;
     a.cs = p.cs;
     a.last_groups = a.Q - (a.S - 1) * (128 / group);
