@@ -42,6 +42,7 @@ struct W4Args {
     int ks = 1, cs = 1;       // a tile's spans over ks warps and cs CTAs
     int chunk = 0;            // spans of x staged at a time
     int last_groups = 0;      // groups of a row's last span
+    bool tma = false;         // (tcgen05 form) x comes by TMA
     bool early = false;       // the weights may be read before the previous kernel of the stream ends
 
     void set_matrix(int i, const w4_matrix& w) {
@@ -105,7 +106,7 @@ struct W4TcPlan {
 inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw) {
     W4TcPlan p{};
     auto rows_of = [&](int nb) { return pieces == 3 ? nb / 2 / 3 * 2 : nb; };
-    p.nb = M <= rows_of(64) ? 64 : 128;
+    p.nb = M <= rows_of(64) ? 64 : M <= rows_of(128) ? 128 : 256;
     p.rows = rows_of(p.nb);
     p.gy = (M + p.rows - 1) / p.rows;
     const int per = nw == 2 ? 4 : 8;

@@ -5,9 +5,11 @@
 // roles of a tile spread over the warps of one CTA:
 //   warps 0-3   unpack codes into the A operand: 128 weight rows x 128 inputs
 //               in shared memory, 128-byte-swizzled K-major;
-//   warps 4-6   bring the B operand: kNB rows of x x 128 inputs, the same
-//               layout (16-bit rows by cp.async; fp32 rows rounded, or split
-//               into their three bf16 parts, on the way);
+//   warps 4-6   bring the B operand: NB rows of x x 128 inputs, the same
+//               layout (16-bit rows by TMA, which fills what lies outside x
+//               with zeros; rows that TMA cannot address element by element,
+//               fp32 rows rounded, or split into their three bf16 parts, on
+//               the way);
 //   warp 7      issues the MMAs: each group of inputs into a fresh sum in
 //               tensor memory, two of them in turn;
 //   warps 8-15  read a finished group (lane = weight row) and add it, times
@@ -18,6 +20,11 @@
 // the 64 up rows of the same outputs, which meet in shared memory at the end.
 // Few tiles: a cluster of CTAs shares a tile's inputs and adds its sums by
 // DSMEM in rank order.
+//
+// An M = 128, K = 16 MMA takes 107 to 135 clocks whatever its N up to 256, so a
+// tile has 256 columns where x has the rows for them; its sums then need 128
+// registers per scaling thread, which the unpacking and copying warps give up.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -37,7 +44,8 @@ namespace kvattn {
 namespace {
 
 constexpr int kStagesA = 2;   // written from registers, so little waits in them
-constexpr int kStagesB = 4;   // copies in flight
+template <int NB>
+constexpr int kStagesB = NB == 256 ? 2 : 4;  // copies in flight
 constexpr int kAhead = 3;     // spans of codes in registers
 constexpr int kThreads = 16 * 32;
 constexpr int kBWarps = 3, kMmaWarp = 7;
@@ -49,12 +57,12 @@ struct Smem {
     static constexpr int kHalfB = NB * 128;
     static constexpr int kB = kStagesA * 2 * kHalfA;  // where the B stages start
     static constexpr int kRed = NB * 128 * 4;         // [column][row] sums, over the stages
-    static constexpr int kAll = kB + kStagesB * 2 * kHalfB;
+    static constexpr int kAll = kB + kStagesB<NB> * 2 * kHalfB;
     static constexpr int kBytes = 1024 + (kAll > kRed ? kAll : kRed);
 };
 
 struct Bars {
-    uint64_t full_a[kStagesA], empty_a[kStagesA], full_b[kStagesB], empty_b[kStagesB], sum_full[2], sum_empty[2];
+    uint64_t full_a[kStagesA], empty_a[kStagesA], full_b[4], empty_b[4], sum_full[2], sum_empty[2];
     uint32_t tmem;
     int failed;
 };
@@ -97,9 +105,22 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 
 // BF: bf16 operands (else fp16).  GP: groups per span.  NB: columns (operand
 // rows of x) of a tile.  GATED: two matrices.
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// A box of 64 inputs x NB rows of x, zeros outside it.
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, int k, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(k), "r"(row), "r"(smem_u32(bar))
+        : "memory");
+}
+
 template <int BF, int GP, int NB, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
-    w4_tc_kernel(const __grid_constant__ W4Args a) {
+    w4_tc_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap xmap) {
     using SM = Smem<NB>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -119,8 +140,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bars.full_a[i], 4);
             mbar_init(&bars.empty_a[i], 1);
         }
-        for (int i = 0; i < kStagesB; ++i) {
-            mbar_init(&bars.full_b[i], kBWarps);
+        for (int i = 0; i < kStagesB<NB>; ++i) {
+            mbar_init(&bars.full_b[i], a.tma ? 1 : kBWarps);
             mbar_init(&bars.empty_b[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -147,6 +168,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp < 4) {
         // ---------------------------------------------------- A: unpack codes
+        // 512 threads of 128 registers: warpgroups of 104 + 56 + 2 x 176
+        if (NB == 256) regs_down<104>();
         const int g = lane >> 2, c = lane & 3, odd = g & 1;
         const uint8_t* src[2];
         const uint8_t* zp[2];
@@ -220,64 +243,47 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp < 4 + kBWarps) {
         // --------------------------------------------------------- B: rows of x
-        // (columns without a row keep what is there: a column's sums are its own)
+        if (NB == 256) regs_down<56>();
         const int t = tid - 128;
-        const bool wide = (reinterpret_cast<size_t>(a.x) & 15) == 0 && (a.ldx * (a.in == W4_X_16 ? 2 : 4)) % 16 == 0;
-        constexpr int kLag = kStagesB - 1;  // copies in flight behind the newest
-        auto release = [&](int st) {
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.full_b[st]);
-        };
-        // 16-bit rows: this thread's 16-byte column c of rows r0 + 12 i; 12 rows
-        // on, the swizzle of a column differs in its third bit
-        const int c = t & 7, r0 = t >> 3;
-        const uint32_t to0 = (uint32_t)r0 * 128 + ((c ^ (r0 & 7)) << 4);
-        const uint16_t* x16 = static_cast<const uint16_t*>(a.x) + (size_t)m0 * a.ldx + c * 8;
+        if (a.tma) {
+            if (warp == 4) {
+                int st = 0, ph = 1;
+                for (int sp = s0; sp < s1; ++sp) {
+                    if (sp - s0 >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], ph, &bars)) break;
+                    if (lane == 0) {
+                        const uint32_t dst = smem_u32(smem) + SM::kB + st * (2 * SM::kHalfB);
+                        mbar_arrive_expect_tx(&bars.full_b[st], 2 * SM::kHalfB);
+                        tma_rows(dst, &xmap, sp * 128, m0, &bars.full_b[st]);
+                        tma_rows(dst + SM::kHalfB, &xmap, sp * 128 + 64, m0, &bars.full_b[st]);
+                    }
+                    __syncwarp();
+                    if (++st == kStagesB<NB>) st = 0, ph ^= 1;
+                }
+            }
+        } else {
+        // (columns without a row keep what is there: a column's sums are its own)
+        const bool wide = (reinterpret_cast<size_t>(a.x) & 15) == 0 && (a.ldx * 4) % 16 == 0;  // fp32 rows
         int it = 0;
         for (int sp = s0; sp < s1; ++sp, ++it) {
-            const int st = it % kStagesB;
-            if (it >= kStagesB && !wait_warp(&bars.empty_b[st], (it / kStagesB - 1) & 1, &bars)) break;
+            const int st = it % kStagesB<NB>;
+            if (it >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], (it / kStagesB<NB> - 1) & 1, &bars)) break;
             uint8_t* dst = smem + SM::kB + st * (2 * SM::kHalfB);
             const int k0 = sp * 128;
+            const int units = mrows * 16;  // eight inputs at a time
             if (a.in == W4_X_16) {
-                if (wide && k0 + 128 <= a.K) {
-                    const uint32_t to = smem_u32(dst) + to0;
-#pragma unroll
-                    for (int i = 0; i < (NB + kBWarps * 4 - 1) / (kBWarps * 4); ++i) {
-                        const int r = r0 + i * kBWarps * 4;
-                        if (r < mrows) {
-                            const uint16_t* row = x16 + (size_t)r * a.ldx + k0;
-                            const uint32_t at = (to ^ ((uint32_t)(i & 1) << 6)) + i * (kBWarps * 4 * 128);
-                            cp16(at, row);
-                            cp16(at + SM::kHalfB, row + 64);
-                        }
-                    }
-                } else {
-                    for (int r = r0; r < mrows; r += kBWarps * 4) {
-                        const uint16_t* row = x16 + (size_t)r * a.ldx + k0;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int k = k0 + h * 64 + c * 8;
-                            uint32_t e[8];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) e[j] = k + j < a.K ? (uint32_t)__ldg(row + h * 64 + j) : 0u;
-                            *reinterpret_cast<uint4*>(dst + h * SM::kHalfB + swz(r, c)) =
-                                make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-                        }
-                    }
-                }
-                cp_commit();
-                if (it >= kLag) {
-                    cp_wait<kLag>();
-                    release((it - kLag) % kStagesB);
-                }
-                continue;
-            }
-            // fp32 rows: eight inputs at a time
-            const int units = mrows * 16;
 #pragma unroll 2
-            for (int u = t; u < units; u += kBWarps * 32) {
+                for (int u = t; u < units; u += kBWarps * 32) {
+                    const int r = u >> 4, c = u & 15, k = k0 + c * 8;
+                    const uint16_t* row = static_cast<const uint16_t*>(a.x) + (size_t)(m0 + r) * a.ldx + k;
+                    uint32_t e[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) e[j] = k + j < a.K ? (uint32_t)__ldg(row + j) : 0u;
+                    *reinterpret_cast<uint4*>(dst + (c >> 3) * SM::kHalfB + swz(r, c & 7)) =
+                        make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+                }
+            }
+#pragma unroll 2
+            for (int u = a.in == W4_X_16 ? units : t; u < units; u += kBWarps * 32) {
                 const int m = u >> 4, c = u & 15, k = c * 8;
                 const float* row = static_cast<const float*>(a.x) + (size_t)(m0 + m) * a.ldx + k0 + k;
                 float v[8];
@@ -306,14 +312,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
                 }
             }
-            release(st);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.full_b[st]);
         }
-        if (a.in == W4_X_16) {
-            cp_wait<0>();
-            for (int i = max(it - kLag, 0); i < it; ++i) release(i % kStagesB);
         }
     } else if (warp == kMmaWarp) {
         // ----------------------------------------------------------- MMA issue
+        if (NB == 256) regs_down<56>();
         constexpr uint32_t idesc = idesc_f16(BF, 128, NB, 0);
         const uint32_t leader = lane == 0;
         const uint32_t base = smem_u32(smem);
@@ -346,11 +352,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             commit(&bars.empty_a[sta], leader);
             commit(&bars.empty_b[stb], leader);
             if (++sta == kStagesA) sta = 0, pha ^= 1;
-            if (++stb == kStagesB) stb = 0, phb ^= 1;
+            if (++stb == kStagesB<NB>) stb = 0, phb ^= 1;
         }
         __syncwarp();
     } else {
         // -------------------------------------------------- scale and accumulate
+        if (NB == 256) regs_up<176>();
         const int quarter = warp & 3, half = (warp - 8) >> 2;
         const int r = quarter * 32 + lane;  // weight row of the CTA
         const __half* sc = a.scales[mat_of(r >> 4)] + (size_t)tile_of(r >> 4) * a.Q * 16 + (r & 7) * 2 + ((r >> 3) & 1);
@@ -392,6 +399,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (NB == 256) {  // every warp goes on with the registers of the launch
+        if (warp >= 8) regs_down<128>();
+        else regs_up<128>();
+    }
     const bool failed = *reinterpret_cast<volatile int*>(&bars.failed) != 0;
     if (warp == kMmaWarp) {
         if (failed && lane == 0) {  // MMAs in flight end before their memory goes
@@ -445,12 +456,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (cs > 1) cluster_sync();  // nobody leaves while its sums are read
 }
 
+// x as TMA sees it: [M][K] 16-bit values in boxes of nb rows x 64 inputs, 128-byte swizzle.
+cudaError_t x_map(const W4Args& a, bool bf, int nb, CUtensorMap* map) {
+    static void* const encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return fn;
+    }();
+    if (!encode) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.K, (cuuint64_t)a.M}, strides[1] = {(cuuint64_t)a.ldx * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)nb}, step[2] = {1, 1};
+    const CUresult r = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(encode)(
+        map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(a.x), dims, strides,
+        box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 template <int BF, int GP, int NB, bool GATED>
-cudaError_t launch_inst(const W4Args& a, int gx, int gy, cudaStream_t st) {
+cudaError_t launch_inst(W4Args a, int gx, int gy, cudaStream_t st) {
     auto fn = w4_tc_kernel<BF, GP, NB, GATED>;
     static SmemGrant grant;
     cudaError_t e = grant.raise(reinterpret_cast<const void*>(fn), Smem<NB>::kBytes);
     if (e != cudaSuccess) return e;
+    CUtensorMap map = {};
+    // TMA reads 16-byte aligned rows a multiple of 16 bytes apart
+    a.tma = a.in == W4_X_16 && reinterpret_cast<size_t>(a.x) % 16 == 0 && a.ldx % 8 == 0;
+    if (a.tma && (e = x_map(a, BF != 0, NB, &map)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(gx * a.cs), (unsigned)gy);
     cfg.blockDim = dim3(kThreads);
@@ -465,7 +500,7 @@ cudaError_t launch_inst(const W4Args& a, int gx, int gy, cudaStream_t st) {
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = a.cs > 1 ? 2 : 1;
-    return counted(cudaLaunchKernelEx(&cfg, fn, a));
+    return counted(cudaLaunchKernelEx(&cfg, fn, a, map));
 }
 
 template <int BF, int GP, int NB>
@@ -475,7 +510,9 @@ cudaError_t launch_gated(const W4Args& a, bool gated, int gx, int gy, cudaStream
 
 template <int BF, int GP>
 cudaError_t launch_nb(const W4Args& a, int nb, bool gated, int gx, int gy, cudaStream_t st) {
-    return nb == 64 ? launch_gated<BF, GP, 64>(a, gated, gx, gy, st) : launch_gated<BF, GP, 128>(a, gated, gx, gy, st);
+    return nb == 64    ? launch_gated<BF, GP, 64>(a, gated, gx, gy, st)
+           : nb == 128 ? launch_gated<BF, GP, 128>(a, gated, gx, gy, st)
+                       : launch_gated<BF, GP, 256>(a, gated, gx, gy, st);
 }
 
 template <int BF>
