@@ -46,7 +46,8 @@ namespace {
 constexpr int kStagesA = 2;   // written from registers, so little waits in them
 template <int NB>
 constexpr int kStagesB = NB == 256 ? 2 : 4;  // copies in flight
-constexpr int kAhead = 3;     // spans of codes in registers
+constexpr int kAhead = 3;     // spans of codes in shared memory, per unpacking warp
+constexpr int kCodes = 2 * 1024 + 128;  // a span of a warp's two tiles, and their zero points
 constexpr int kThreads = 16 * 32;
 constexpr int kBWarps = 3, kMmaWarp = 7;
 constexpr int kHalfA = 128 * 128;  // 64 inputs of 128 rows
@@ -57,8 +58,9 @@ struct Smem {
     static constexpr int kHalfB = NB * 128;
     static constexpr int kB = kStagesA * 2 * kHalfA;  // where the B stages start
     static constexpr int kRed = NB * 128 * 4;         // [column][row] sums, over the stages
-    static constexpr int kAll = kB + kStagesB<NB> * 2 * kHalfB;
-    static constexpr int kBytes = 1024 + (kAll > kRed ? kAll : kRed);
+    static constexpr int kRing = kB + kStagesB<NB> * 2 * kHalfB;  // the codes
+    static_assert(kRed <= kRing, "");
+    static constexpr int kBytes = 1024 + kRing + 4 * kAhead * kCodes;
 };
 
 struct Bars {
@@ -170,77 +172,82 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---------------------------------------------------- A: unpack codes
         // 512 threads of 128 registers: warpgroups of 104 + 56 + 2 x 176
         if (NB == 256) regs_down<104>();
+        // A short loop on purpose: sixteen warps of four roles share the
+        // instruction caches, and unrolling this role starved the others.
         const int g = lane >> 2, c = lane & 3, odd = g & 1;
         const uint8_t* src[2];
-        const uint8_t* zp[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int t = warp * 2 + i, q = mat_of(t);
-            src[i] = reinterpret_cast<const uint8_t*>(a.codes[q]) + ((size_t)tile_of(t) * a.S + s0) * 1024 + lane * 16;
-            zp[i] = a.zeros[q] ? a.zeros[q] + (size_t)tile_of(t) * a.Q * 16 + g * 2 : nullptr;
+            const int t = warp * 2 + i;
+            src[i] = reinterpret_cast<const uint8_t*>(a.codes[mat_of(t)]) + ((size_t)tile_of(t) * a.S + s0) * 1024 + lane * 16;
         }
+        // zero points: lane l brings four bytes of group l / 4 % GP of tile l / (4 GP)
+        const int zt = warp * 2 + (lane / (4 * GP) & 1), zg = lane / 4 % GP;
+        const bool zeros = a.zeros[0] != nullptr;
+        const uint8_t* zsrc = zeros && lane < 8 * GP ? a.zeros[mat_of(zt)] + ((size_t)tile_of(zt) * a.Q + (size_t)s0 * GP + zg) * 16 + (lane & 3) * 4
+                                                     : nullptr;
+        uint8_t* const ring = smem + SM::kRing + warp * (kAhead * kCodes);
+        const uint32_t ring_s = smem_u32(ring);
+        int fslot = 0, fsp = s0;
+        auto fetch = [&]() {
+            if (fsp < s1) {
+                const uint32_t to = ring_s + fslot * kCodes + lane * 16;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    cp16(to + i * 1024, src[i]);
+                    cp16(to + i * 1024 + 512, src[i] + 512);
+                    src[i] += 1024;
+                }
+                if (zsrc) {
+                    if (fsp * GP + zg < a.Q) cp4(ring_s + fslot * kCodes + 2048 + lane * 4, zsrc);
+                    zsrc += GP * 16;
+                }
+                ++fsp;
+            }
+            cp_commit();
+            fslot = fslot + 1 == kAhead ? 0 : fslot + 1;
+        };
+#pragma unroll
+        for (int d = 0; d < kAhead - 1; ++d) fetch();
         // odd rows take the words of a pair in the other order, so that eight
         // lanes' stores fall into eight different 16-byte columns
         const uint32_t row0 = (uint32_t)(warp * 32 + g) * 128;
-        const uint32_t chunk[2] = {(uint32_t)((odd * 4 + c) ^ g) << 4, (uint32_t)(((odd ^ 1) * 4 + c) ^ g) << 4};
-        uint4 ring[kAhead][2][2];  // [span][tile][rows g, g + 8]
-        auto fetch = [&](uint4 (&to)[2][2]) {
+        const uint32_t chunk0 = (uint32_t)((odd * 4 + c) ^ g) << 4;
+        uint2 z = zero_consts<BF>(8u);
+        int st = 0, ph = 1, slot = 0;
+        for (int sp = s0; sp < s1; ++sp) {
+            cp_wait<kAhead - 2>();
+            __syncwarp();  // zero points came by other lanes; the slot refilled next was read by all of them
+            fetch();
+            if (sp - s0 >= kStagesA && !wait_warp(&bars.empty_a[st], ph, &bars)) break;
+            const uint8_t* from = ring + slot * kCodes;
+            uint8_t* to = smem + st * (2 * kHalfA) + row0 + chunk0;
+#pragma unroll 1
+            for (int th = 0; th < 4; ++th) {  // tile, rows g or g + 8
+                const uint4 w = *reinterpret_cast<const uint4*>(from + th * 512 + lane * 16);
+                const uint32_t v[4] = {odd ? w.y : w.x, odd ? w.x : w.y, odd ? w.w : w.z, odd ? w.z : w.w};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) to[i][h] = __ldg(reinterpret_cast<const uint4*>(src[i] + h * 512));
-                src[i] += 1024;
-            }
-        };
-#pragma unroll
-        for (int d = 0; d < kAhead; ++d)
-            if (s0 + d < s1) fetch(ring[d]);
-        uint2 z[2] = {zero_consts<BF>(8u), zero_consts<BF>(8u)};
-        bool alive = true;
-        for (int sp0 = s0; alive && sp0 < s1; sp0 += kAhead) {
-#pragma unroll
-          for (int d = 0; d < kAhead; ++d) {
-            const int sp = sp0 + d;
-            if (sp >= s1) break;
-            const int it = sp - s0, st = it % kStagesA;
-            uint4 w[2][2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) w[i][h] = ring[d][i][h];
-            if (sp + kAhead < s1) fetch(ring[d]);
-            if (it >= kStagesA && !wait_warp(&bars.empty_a[st], (it / kStagesA - 1) & 1, &bars)) {
-                alive = false;
-                break;
-            }
-            uint8_t* dst = smem + st * (2 * kHalfA) + row0;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t zz[GP];
-#pragma unroll
-                for (int q = 0; q < GP; ++q)
-                    zz[q] = zp[i] && sp * GP + q < a.Q ? *reinterpret_cast<const uint16_t*>(zp[i] + (size_t)(sp * GP + q) * 16) : 0x0808u;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t v[4] = {odd ? w[i][h].y : w[i][h].x, odd ? w[i][h].x : w[i][h].y,
-                                           odd ? w[i][h].w : w[i][h].z, odd ? w[i][h].z : w[i][h].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        // word j of the lane is inputs 32 (j ^ odd) ..
-                        const int qa = j / (4 / GP), qb = (j ^ 1) / (4 / GP);
-                        if (j == 0 || GP == 4 || (GP == 2 && j == 2)) z[0] = zero_consts<BF>(((qa == qb || !odd ? zz[qa] : zz[qb]) >> (8 * h)) & 15u);
-                        uint32_t p[4];
-                        unpack<BF>(v[j], z[0], p);
-                        *reinterpret_cast<uint4*>(dst + (j >> 1) * kHalfA + (i * 16 + h * 8) * 128 + chunk[j & 1]) =
-                            make_uint4(p[0], p[1], p[2], p[3]);
+                for (int j = 0; j < 4; ++j) {
+                    // word j here is inputs 32 (j ^ odd) ..
+                    if (zeros && j % (4 / GP) == 0) {
+                        const int q = GP == 4 ? j ^ odd : j / (4 / GP);
+                        z = zero_consts<BF>(from[2048 + ((th >> 1) * GP + q) * 16 + g * 2 + (th & 1)] & 15u);
                     }
+                    uint32_t p[4];
+                    unpack<BF>(v[j], z, p);
+                    // the pair's second word is four 16-byte columns on (or back): bit 6 of the address
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(reinterpret_cast<size_t>(to) ^ ((j & 1) << 6)) + (j >> 1) * kHalfA) =
+                        make_uint4(p[0], p[1], p[2], p[3]);
                 }
+                to += 8 * 128;
             }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.full_a[st]);
-          }
+            if (++st == kStagesA) st = 0, ph ^= 1;
+            slot = slot + 1 == kAhead ? 0 : slot + 1;
         }
+        cp_wait<0>();
     } else if (warp < 4 + kBWarps) {
         // --------------------------------------------------------- B: rows of x
         if (NB == 256) regs_down<56>();
