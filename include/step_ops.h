@@ -10,9 +10,9 @@
  * (qw2_quantize_weights, qw2_set_controls).
  *
  * Conventions are those of kvattn.h: int status, kv_last_error(), device
- * pointers, `stream` a cudaStream_t as void*.  The calls allocate nothing,
- * keep nothing between calls and use no workspace, so they may be captured
- * into a CUDA graph and may run on several streams at once.  `device` says
+ * pointers, `stream` a cudaStream_t as void*.  The calls allocate nothing and
+ * keep nothing between calls, so they may be captured into a CUDA graph and may
+ * run on several streams at once (with scratch of their own, where they take it).  `device` says
  * where the pointers live; the calling thread's current device is kept.
  */
 #ifndef STEP_OPS_H
@@ -80,15 +80,21 @@ int w4_dequantize(const w4_matrix* m, float* out, long long ldo, void* stream);
  * itself.  Sums are fp32; an fp32 x keeps all its bits (three bf16 parts);
  * the result is rounded once.  A group's sum of (code - zero) * x is formed
  * before its scale, so that sum has to stay within fp32 (|x| below 1e35 does).
- * out must not overlap x. */
+ * out must not overlap x.
+ * work: w4_work_bytes() of scratch, 16-byte aligned, overlapping nothing else,
+ * or NULL: many rows of an fp32 x go through it, and take longer without it. */
 int w4_linear(const w4_matrix* w, const void* x, int x_dtype, int m, long long ldx, const float* bias,
-              const void* residual, long long ldr, void* out, int out_dtype, long long ldo, void* stream);
+              const void* residual, long long ldr, void* out, int out_dtype, long long ldo, void* work, void* stream);
 
 /* out = silu(x Wg^T) * (x Wu^T), silu(a) = a / (1 + exp(-a)): the first half
  * of a gated feed-forward block.  gate and up have the same n, k, group and
  * device, and both or neither have zero points. */
 int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dtype, int m, long long ldx, void* out,
-             int out_dtype, long long ldo, void* stream);
+             int out_dtype, long long ldo, void* work, void* stream);
+
+/* Scratch of w4_linear (gated 0) or w4_gated (gated 1) for m rows of x: 0
+ * where none helps. */
+int w4_work_bytes(int n, int k, int x_dtype, int m, int gated, size_t* bytes);
 
 /* The waits inside the kernels for many rows are bounded (about a second):
  * *status is KV_OK, or KV_ERR_TIMEOUT if one has run out on `device` since the

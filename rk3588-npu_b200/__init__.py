@@ -114,8 +114,9 @@ _SIGS.update({
     "w4_sizes": [C.c_int, C.c_int, C.c_int] + [C.POINTER(C.c_size_t)] * 3,
     "w4_quantize": [_w4p, _vp, C.c_int, C.c_longlong, _vp],
     "w4_dequantize": [_w4p, _vp, C.c_longlong, _vp],
-    "w4_linear": [_w4p, _vp, C.c_int, C.c_int, C.c_longlong, _vp, _vp, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp],
-    "w4_gated": [_w4p, _w4p, _vp, C.c_int, C.c_int, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp],
+    "w4_linear": [_vp, _vp, C.c_int, C.c_int, C.c_longlong, _vp, _vp, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp, _vp],
+    "w4_gated": [_vp, _vp, _vp, C.c_int, C.c_int, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp, _vp],
+    "w4_work_bytes": [C.c_int] * 5 + [C.POINTER(C.c_size_t)],
     "logits_adjust": [C.POINTER(_LogitsCall), _vp],
     "step_ops_status": [C.c_int, _ip],
 })
@@ -442,11 +443,14 @@ def _step_dtype(t, what: str) -> int:
 
 def _rows(t, device: int, what: str, rows=None, cols=None) -> int:
     """A 2-D device tensor with contiguous rows: the elements from row to row."""
-    if t.dim() != 2 or t.get_device() != device:
+    shape = t.shape
+    if len(shape) != 2 or t.get_device() != device:
         raise ValueError(f"{what}: a 2-D tensor on cuda:{device} is expected")
-    m, n = t.shape
+    m, n = shape
     if (rows is not None and m != rows) or (cols is not None and n != cols):
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected ({rows}, {cols})")
+        raise ValueError(f"{what}: shape {tuple(shape)}, expected ({rows}, {cols})")
+    if t.is_contiguous():
+        return n
     ld, inner = t.stride()
     if inner != 1 and n > 1:
         raise ValueError(f"{what}: the elements of a row must be adjacent")
@@ -469,6 +473,19 @@ def _stream_on(stream, device: int):
         import torch
         return torch.cuda.current_stream(device).cuda_stream
     return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _scratch(w, x, m: int, gated: int, stream):
+    """Scratch for many rows of an fp32 x, held by the caching allocator for `stream`."""
+    import torch
+    n = C.c_size_t()
+    call("w4_work_bytes", w.n, w.k, STEP_F32, m, gated, C.byref(n))
+    if not n.value:
+        return None
+    t = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+    if stream is not None:
+        t.record_stream(torch.cuda.ExternalStream(stream, device=x.device) if isinstance(stream, int) else stream)
+    return t
 
 
 class W4:
@@ -495,6 +512,7 @@ class W4:
         self.n, self.k, self.group, self.device = n, k, group, dev
         self._c = _W4Matrix(dev, n, k, group, codes.data_ptr(), scales.data_ptr(),
                             zeros.data_ptr() if zeros is not None else None)
+        self._at = C.addressof(self._c)
 
     def dequantize(self, out=None, stream=None):
         """The matrix's values, fp32 [n, k]."""
@@ -527,11 +545,12 @@ def w4_linear(w: W4, x, out, bias=None, residual=None, stream=None) -> None:
     """out [m, n] = x [m, k] W^T (+ bias [n] fp32) (+ residual [m, n], of out's
     type; may be out).  x and out fp16, bf16 or fp32, rows any distance apart."""
     dev = w.device
-    m = x.shape[0]
     ldx = _rows(x, dev, "x", None, w.k)
+    m = x.shape[0]
     ldo = _rows(out, dev, "out", m, w.n)
-    b = r = None
+    b = r = work = None
     ldr = 0
+    xd = _step_dtype(x, "x")
     if bias is not None:
         import torch
         b = _words(bias, dev, "bias", torch.float32, w.n)
@@ -540,8 +559,10 @@ def w4_linear(w: W4, x, out, bias=None, residual=None, stream=None) -> None:
         if residual.dtype != out.dtype:
             raise ValueError("residual: out's element type is expected")
         r = residual.data_ptr()
-    rc = _lib.w4_linear(w._c, x.data_ptr(), _step_dtype(x, "x"), m, ldx, b, r, ldr, out.data_ptr(),
-                        _step_dtype(out, "out"), ldo, _stream_on(stream, dev))
+    if xd == STEP_F32 and m > 4:  # fewer rows need none
+        work = _scratch(w, x, m, 0, stream)
+    rc = _lib.w4_linear(w._at, x.data_ptr(), xd, m, ldx, b, r, ldr, out.data_ptr(), _step_dtype(out, "out"), ldo,
+                        work.data_ptr() if work is not None else None, _stream_on(stream, dev))
     if rc:
         _check(rc, "w4_linear")
 
@@ -549,11 +570,13 @@ def w4_linear(w: W4, x, out, bias=None, residual=None, stream=None) -> None:
 def w4_gated(gate: W4, up: W4, x, out, stream=None) -> None:
     """out [m, n] = silu(x Wg^T) * (x Wu^T), types as w4_linear."""
     dev = gate.device
-    m = x.shape[0]
     ldx = _rows(x, dev, "x", None, gate.k)
+    m = x.shape[0]
     ldo = _rows(out, dev, "out", m, gate.n)
-    rc = _lib.w4_gated(gate._c, up._c, x.data_ptr(), _step_dtype(x, "x"), m, ldx, out.data_ptr(),
-                       _step_dtype(out, "out"), ldo, _stream_on(stream, dev))
+    xd = _step_dtype(x, "x")
+    work = _scratch(gate, x, m, 1, stream) if xd == STEP_F32 and m > 4 else None
+    rc = _lib.w4_gated(gate._at, up._at, x.data_ptr(), xd, m, ldx, out.data_ptr(), _step_dtype(out, "out"), ldo,
+                       work.data_ptr() if work is not None else None, _stream_on(stream, dev))
     if rc:
         _check(rc, "w4_gated")
 

@@ -176,6 +176,7 @@ struct qw2_model {
     bool have_embed = false, have_norm = false;
     int w4_group = 0;           // > 0: the projections are in 4 bits
     w4_matrix qhead{};          // lm_head in 4 bits (the lookup keeps the fp16 embedding)
+    uint16_t* x16 = nullptr;    // [R][H] rounded inputs of a projection of many rows
 
     // activations, up to max_position rows
     float* hidden = nullptr;  // [R][H]
@@ -604,6 +605,14 @@ cudaError_t project(const qw2_model* m, int mode, int in, const GemvArgs& a, con
     w.x = a.x;
     w.ldx = a.K;
     w.in = in == 0 ? W4_X_16 : in == 1 ? W4_X_ROUND : W4_X_NORM;
+    if (w.in != W4_X_16 && w4_use_tc(w.M, w.T, 1, q2 ? 2 : 1)) {
+        // many rows: the norm and the rounding once, not in every tile
+        const cudaError_t e = w.in == W4_X_NORM ? launch_rmsnorm_f16(static_cast<const float*>(a.x), a.norm_w, m->x16, a.M, a.K, a.eps, st)
+                                                : launch_to_f16_exact(static_cast<const float*>(a.x), (long)a.M * a.K, m->x16, st);
+        if (e != cudaSuccess) return e;
+        w.x = m->x16;
+        w.in = W4_X_16;
+    }
     w.mode = mode;  // the launch_gemv modes
     w.g = a;
     w.early = true;
@@ -1622,8 +1631,9 @@ int qw2_quantize_weights(qw2_model* m, int group, int zero_points) {
     items.push_back({&m->qhead, &m->embed, V, H});
     // all of the 4-bit matrices first: without room for them nothing changes
     const size_t before = m->allocs.size();
-    int rc = KV_OK;
+    int rc = m->alloc_n(&m->x16, (size_t)m->rows_cap * H);
     for (Item& it : items) {
+        if (rc != KV_OK) break;
         w4_matrix q{m->device, it.n, it.k, group, nullptr, nullptr, nullptr};
         w4_sizes(it.n, it.k, group, &bytes[0], &bytes[1], &bytes[2]);
         rc = m->alloc(&q.codes, bytes[0]);
@@ -1644,6 +1654,7 @@ int qw2_quantize_weights(qw2_model* m, int group, int zero_points) {
             m->allocs.pop_back();
         }
         for (Item& it : items) *it.q = w4_matrix{};
+        m->x16 = nullptr;
         return rc;
     }
     m->w4_group = group;

@@ -89,6 +89,20 @@ void set_x(W4Args& a, const void* x, int x_dtype, int m, long long ldx) {
     a.pieces = x_dtype == STEP_F32 ? 3 : 1;
 }
 
+size_t work_bytes(int n, int k, int x_dtype, int m, int gated) {
+    return x_dtype == STEP_F32 && w4_use_tc(m, (n + 15) / 16, 3, gated ? 2 : 1) ? w4_split_bytes(m, k) : 0;
+}
+
+int check_work(const w4_matrix& w, const void* x, int x_dtype, int m, long long ldx, const void* out, int out_dtype,
+               long long ldo, int gated, const void* work) {
+    if (!work || m == 0) return KV_OK;
+    if (!aligned(work, 16)) return sfail(KV_ERR_INVAL, "scratch needs 16-byte alignment");
+    const Range r(work, 1, (long long)work_bytes(w.n, w.k, x_dtype, m, gated), 0, 1);
+    if (r.meets(Range(x, m, w.k, ldx, esize(x_dtype))) || r.meets(Range(out, m, w.n, ldo, esize(out_dtype))))
+        return sfail(KV_ERR_INVAL, "scratch overlaps x or out");
+    return KV_OK;
+}
+
 int launched(cudaError_t e, const char* what) {
     if (e == cudaSuccess) return KV_OK;
     return sfail(KV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
@@ -128,9 +142,10 @@ int w4_dequantize(const w4_matrix* m, float* out, long long ldo, void* stream) {
 }
 
 int w4_linear(const w4_matrix* w, const void* x, int x_dtype, int m, long long ldx, const float* bias,
-              const void* residual, long long ldr, void* out, int out_dtype, long long ldo, void* stream) {
+              const void* residual, long long ldr, void* out, int out_dtype, long long ldo, void* work, void* stream) {
     ST_OK(check_matrix(w, "matrix"));
     ST_OK(check_rows(*w, x, x_dtype, m, ldx, out, out_dtype, ldo));
+    ST_OK(check_work(*w, x, x_dtype, m, ldx, out, out_dtype, ldo, 0, work));
     if (!aligned(bias, 4)) return sfail(KV_ERR_INVAL, "bias is not aligned to its element");
     if (residual) {
         if (ldr < w->n || ldr > (1ll << 40)) return sfail(KV_ERR_INVAL, "residual rows %lld apart for %d outputs", ldr, w->n);
@@ -145,6 +160,7 @@ int w4_linear(const w4_matrix* w, const void* x, int x_dtype, int m, long long l
     W4Args a;
     a.set_matrix(0, *w);
     set_x(a, x, x_dtype, m, ldx);
+    a.work = work;
     a.mode = W4_LINEAR;
     a.bias = bias;
     a.residual = residual;
@@ -156,13 +172,14 @@ int w4_linear(const w4_matrix* w, const void* x, int x_dtype, int m, long long l
 }
 
 int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dtype, int m, long long ldx, void* out,
-             int out_dtype, long long ldo, void* stream) {
+             int out_dtype, long long ldo, void* work, void* stream) {
     ST_OK(check_matrix(gate, "gate matrix"));
     ST_OK(check_matrix(up, "up matrix"));
     if (gate->n != up->n || gate->k != up->k || gate->group != up->group || gate->device != up->device ||
         !gate->zeros != !up->zeros)
         return sfail(KV_ERR_INVAL, "gate and up differ in shape, group, device or zero points");
     ST_OK(check_rows(*gate, x, x_dtype, m, ldx, out, out_dtype, ldo));
+    ST_OK(check_work(*gate, x, x_dtype, m, ldx, out, out_dtype, ldo, 1, work));
     if (m == 0) return KV_OK;
     DeviceGuard g(gate->device);
     if (!g.ok) return sfail(KV_ERR_INVAL, "no CUDA device %d", gate->device);
@@ -170,11 +187,20 @@ int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dt
     a.set_matrix(0, *gate);
     a.set_matrix(1, *up);
     set_x(a, x, x_dtype, m, ldx);
+    a.work = work;
     a.mode = W4_GATED;
     a.out = out;
     a.out_dtype = out_dtype;
     a.ldo = ldo;
     return launched(launch_w4(a, gate->group, x_dtype != STEP_F16, 2, static_cast<cudaStream_t>(stream)), "w4_gated");
+}
+
+int w4_work_bytes(int n, int k, int x_dtype, int m, int gated, size_t* bytes) {
+    ST_OK(check_shape(n, k, 32));
+    ST_OK(check_dtype(x_dtype, "x"));
+    if (m < 0 || m > 1 << 20 || !bytes) return sfail(KV_ERR_INVAL, "%d rows, or NULL bytes", m);
+    *bytes = work_bytes(n, k, x_dtype, m, gated);
+    return KV_OK;
 }
 
 int step_ops_status(int device, int* status) {

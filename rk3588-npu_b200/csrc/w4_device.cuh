@@ -86,15 +86,32 @@ __device__ __forceinline__ void split3(float x, uint16_t& a, uint16_t& b, uint16
 }
 
 // ------------------------------------------------------------------ epilogue
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// f(a value of the element type).
+template <class F>
+__device__ __forceinline__ void with_type(int dtype, F f) {
+    if (dtype == STEP_F32) f(0.f);
+    else if (dtype == STEP_F16) f(__half());
+    else f(__nv_bfloat16());
+}
+
 __device__ __forceinline__ float load_as(const void* p, size_t i, int dtype) {
-    if (dtype == STEP_F32) return static_cast<const float*>(p)[i];
-    if (dtype == STEP_F16) return __half2float(static_cast<const __half*>(p)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+    float v = 0.f;
+    with_type(dtype, [&](auto one) { v = to_float(static_cast<const decltype(one)*>(p)[i]); });
+    return v;
 }
 __device__ __forceinline__ void store_as(void* p, size_t i, int dtype, float v) {
-    if (dtype == STEP_F32) static_cast<float*>(p)[i] = v;
-    else if (dtype == STEP_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    with_type(dtype, [&](auto one) { static_cast<decltype(one)*>(p)[i] = from_float<decltype(one)>(v); });
 }
 
 // silu(g) u

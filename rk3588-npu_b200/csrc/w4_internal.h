@@ -30,6 +30,7 @@ struct W4Args {
     long long ldx = 0;
     int in = W4_X_16, mode = W4_LINEAR;
     int pieces = 1;           // operand rows per x row (3 for W4_X_F32)
+    void* work = nullptr;     // room for w4_split_bytes, or NULL
     int out_dtype = STEP_F32;
     const float* bias = nullptr;
     const void* residual = nullptr;
@@ -57,7 +58,6 @@ struct W4Args {
     }
 };
 
-constexpr int kW4TcRows = 64;
 constexpr int kSms = 148;
 constexpr int kW4MaxSmem = 227 * 1024;
 // Spans that a warp copies at a time (two such batches in shared memory).
@@ -105,9 +105,8 @@ struct W4TcPlan {
 
 inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw) {
     W4TcPlan p{};
-    auto rows_of = [&](int nb) { return pieces == 3 ? nb / 2 / 3 * 2 : nb; };
-    p.nb = M <= rows_of(64) ? 64 : M <= rows_of(128) ? 128 : 256;
-    p.rows = rows_of(p.nb);
+    p.nb = M * pieces <= 64 ? 64 : M * pieces <= 128 ? 128 : 256;
+    p.rows = p.nb / pieces;
     p.gy = (M + p.rows - 1) / p.rows;
     const int per = nw == 2 ? 4 : 8;
     p.gx = (T + per - 1) / per;
@@ -120,10 +119,20 @@ inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw) {
     return p;
 }
 
-// Rows from which the tcgen05 form is the faster one.
-inline bool w4_use_tc(int M, int pieces) { return M * pieces > kW4TcRows; }
+// Rows from which the tcgen05 form is the faster one: its tiles cost the same
+// for one row as for 64, so it depends on how many of them there are.  Measured, us
+// (w4_kernels.cu / tcgen05): 1536 x 8960, 16 rows 18 / 12, 12 rows 12.3 / 12.3;
+// 8960 x 1536 gated, 24 rows 15.9 / 14, 16 rows 11.4 / 14; 151936 x 1536, 48 rows
+// 158 / 138, 32 rows 103 / 137.
+inline bool w4_use_tc(int M, int T, int pieces, int nw) {
+    const int tiles = (T + 7) / 8 * nw, rows = M * pieces;
+    return rows > (tiles <= kSms / 2 ? 14 : tiles <= kSms ? 20 : 40);
+}
 
 cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st);
+// The three bf16 parts of fp32 rows, for the tcgen05 form: [3 M][K rounded up to 8].
+inline size_t w4_split_bytes(int M, int K) { return (size_t)3 * M * ((K + 7) / 8 * 8) * 2; }
+cudaError_t launch_split_rows(const float* x, long long ldx, int M, int K, void* parts, cudaStream_t st);
 cudaError_t launch_w4_tc(W4Args a, int group, bool bf, int nw, cudaStream_t st);
 // The status of the waits in launch_w4_tc's kernels on the current device
 // (0, or KV_ERR_TIMEOUT), cleared by reading it.

@@ -631,7 +631,17 @@ cudaError_t launch_nt(const W4Args& a, int nt, int nw, int group, int gx, int pa
 }  // namespace
 
 cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st) {
-    if (a.in != W4_X_NORM && w4_use_tc(a.M, a.pieces)) return launch_w4_tc(a, group, bf, nw, st);
+    if (w4_use_tc(a.M, a.T, a.pieces, nw)) {
+        if (a.in == W4_X_16) return launch_w4_tc(a, group, bf, nw, st);
+        if (a.in == W4_X_F32 && a.work) {
+            const cudaError_t e = launch_split_rows(static_cast<const float*>(a.x), a.ldx, a.M, a.K, a.work, st);
+            if (e != cudaSuccess) return e;
+            a.x = a.work;
+            a.ldx = (a.K + 7) / 8 * 8;
+            a.in = W4_X_16;
+            return launch_w4_tc(a, group, bf, nw, st);
+        }
+    }
     const W4Plan p = w4_plan(a.M, a.T, a.S, a.pieces, nw, kSms);
     a.rows = p.rows;
     a.ks = p.ks;

@@ -1,15 +1,14 @@
 // w4_tc_kernel.cu -- the 4-bit projections for many rows of x, on tcgen05.
 //
+// x is 16-bit here: an fp32 x comes as its three bf16 parts (w4_split_rows).
 // The same sums as w4_kernels.cu (integers q - z exact in the operand type,
 // a group's products summed in fp32, the scale applied to the sum), with the
 // roles of a tile spread over the warps of one CTA:
 //   warps 0-3   unpack codes into the A operand: 128 weight rows x 128 inputs
 //               in shared memory, 128-byte-swizzled K-major;
 //   warps 4-6   bring the B operand: NB rows of x x 128 inputs, the same
-//               layout (16-bit rows by TMA, which fills what lies outside x
-//               with zeros; rows that TMA cannot address element by element,
-//               fp32 rows rounded, or split into their three bf16 parts, on
-//               the way);
+//               layout (by TMA, which fills what lies outside x with zeros;
+//               rows that TMA cannot address, element by element);
 //   warp 7      issues the MMAs: each group of inputs into a fresh sum in
 //               tensor memory, two of them in turn;
 //   warps 8-15  read a finished group (lane = weight row) and add it, times
@@ -84,23 +83,19 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Bars* 
     return __all_sync(0xffffffffu, ok);
 }
 
-// D (+)= A B by the warp's leader.  The whole warp runs the loop around it, so
-// that the operands are uniform: issued from a branch of one lane, each MMA
-// waited for its operands' way to uniform registers (134 clocks a piece,
-// whatever its size).
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
+// D (+)= A B.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 e, %5, 0;\n"
-        " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader)
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void commit(uint64_t* bar, uint32_t leader) {
-    asm volatile(
-        "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n"
-        " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)),
-        "r"(leader)
-        : "memory");
+// One lane of the (whole) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one = 0;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n @p mov.u32 %0, 1;\n}" : "+r"(one));
+    return one != 0;
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -132,10 +127,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tile0 = (int)blockIdx.x / cs * (GATED ? 4 : 8);  // first 16-row tile
     const int m0 = blockIdx.y * a.rows, mrows = min(a.rows, a.M - m0);
     const int s0 = (int)((long long)a.S * rank / cs), s1 = (int)((long long)a.S * (rank + 1) / cs);
-    // column of part p of row m: the three parts of an fp32 row stay in one half of the columns
-    const int per_half = a.pieces == 3 ? NB / 2 / 3 : NB / 2;  // rows per half
-    auto column = [&](int m, int p) { return m / per_half * (NB / 2) + m % per_half * a.pieces + p; };
-
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
         for (int i = 0; i < kStagesA; ++i) {
@@ -260,8 +251,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) {
                         const uint32_t dst = smem_u32(smem) + SM::kB + st * (2 * SM::kHalfB);
                         mbar_arrive_expect_tx(&bars.full_b[st], 2 * SM::kHalfB);
-                        tma_rows(dst, &xmap, sp * 128, m0, &bars.full_b[st]);
-                        tma_rows(dst + SM::kHalfB, &xmap, sp * 128 + 64, m0, &bars.full_b[st]);
+                        tma_rows(dst, &xmap, sp * 128, m0 * a.pieces, &bars.full_b[st]);
+                        tma_rows(dst + SM::kHalfB, &xmap, sp * 128 + 64, m0 * a.pieces, &bars.full_b[st]);
                     }
                     __syncwarp();
                     if (++st == kStagesB<NB>) st = 0, ph ^= 1;
@@ -269,55 +260,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         } else {
         // (columns without a row keep what is there: a column's sums are its own)
-        const bool wide = (reinterpret_cast<size_t>(a.x) & 15) == 0 && (a.ldx * 4) % 16 == 0;  // fp32 rows
         int it = 0;
         for (int sp = s0; sp < s1; ++sp, ++it) {
             const int st = it % kStagesB<NB>;
             if (it >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], (it / kStagesB<NB> - 1) & 1, &bars)) break;
             uint8_t* dst = smem + SM::kB + st * (2 * SM::kHalfB);
-            const int k0 = sp * 128;
-            const int units = mrows * 16;  // eight inputs at a time
-            if (a.in == W4_X_16) {
 #pragma unroll 2
-                for (int u = t; u < units; u += kBWarps * 32) {
-                    const int r = u >> 4, c = u & 15, k = k0 + c * 8;
-                    const uint16_t* row = static_cast<const uint16_t*>(a.x) + (size_t)(m0 + r) * a.ldx + k;
-                    uint32_t e[8];
+            for (int u = t; u < mrows * 16; u += kBWarps * 32) {  // eight inputs at a time
+                const int r = u >> 4, c = u & 15, k = sp * 128 + c * 8;
+                const uint16_t* row = static_cast<const uint16_t*>(a.x) + (size_t)(m0 + r) * a.ldx + k;
+                uint32_t e[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) e[j] = k + j < a.K ? (uint32_t)__ldg(row + j) : 0u;
-                    *reinterpret_cast<uint4*>(dst + (c >> 3) * SM::kHalfB + swz(r, c & 7)) =
-                        make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-                }
-            }
-#pragma unroll 2
-            for (int u = a.in == W4_X_16 ? units : t; u < units; u += kBWarps * 32) {
-                const int m = u >> 4, c = u & 15, k = c * 8;
-                const float* row = static_cast<const float*>(a.x) + (size_t)(m0 + m) * a.ldx + k0 + k;
-                float v[8];
-                if (wide && k0 + k + 8 <= a.K) {
-                    const float4 f = __ldg(reinterpret_cast<const float4*>(row)), e = __ldg(reinterpret_cast<const float4*>(row) + 1);
-                    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = e.x, v[5] = e.y, v[6] = e.z, v[7] = e.w;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = k0 + k + j < a.K ? __ldg(row + j) : 0.f;
-                }
-                uint8_t* half = dst + (c >> 3) * SM::kHalfB;
-                if (a.pieces == 3) {
-                    uint16_t p[3][8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) split3(v[j], p[0][j], p[1][j], p[2][j]);
-#pragma unroll
-                    for (int q = 0; q < 3; ++q)
-                        *reinterpret_cast<uint4*>(half + swz(column(m, q), c & 7)) =
-                            make_uint4(p[q][0] | (uint32_t)p[q][1] << 16, p[q][2] | (uint32_t)p[q][3] << 16,
-                                       p[q][4] | (uint32_t)p[q][5] << 16, p[q][6] | (uint32_t)p[q][7] << 16);
-                } else {
-                    uint32_t e[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) e[j] = enc_f16_trunc(v[j]);
-                    *reinterpret_cast<uint4*>(half + swz(m, c & 7)) =
-                        make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-                }
+                for (int j = 0; j < 8; ++j) e[j] = k + j < a.K ? (uint32_t)__ldg(row + j) : 0u;
+                *reinterpret_cast<uint4*>(dst + (c >> 3) * SM::kHalfB + swz(r, c & 7)) =
+                    make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
             }
             fence_async_smem();
             __syncwarp();
@@ -327,37 +283,45 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kMmaWarp) {
         // ----------------------------------------------------------- MMA issue
         if (NB == 256) regs_down<56>();
+        // The whole warp runs the loop and one lane issues: the operands of an
+        // MMA live in uniform registers, which only uniform control flow fills
+        // directly.
         constexpr uint32_t idesc = idesc_f16(BF, 128, NB, 0);
-        const uint32_t leader = lane == 0;
-        const uint32_t base = smem_u32(smem);
+        const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0), d0 = __shfl_sync(0xffffffffu, tmem, 0);
         int f = 0, sta = 0, stb = 0, pha = 0, phb = 0;  // groups so far; stages and their phases
         bool ok = true;
         for (int sp = s0; ok && sp < s1; ++sp) {
             ok = wait_warp(&bars.full_b[stb], phb, &bars) && wait_warp(&bars.full_a[sta], pha, &bars);
             if (!ok) break;
             tc_fence_after();
-            const uint64_t da = sdesc(base + sta * (2 * kHalfA), 16, 1024), db = sdesc(base + SM::kB + stb * (2 * SM::kHalfB), 16, 1024);
+            const int ua = __shfl_sync(0xffffffffu, sta, 0), ub = __shfl_sync(0xffffffffu, stb, 0);
+            const uint64_t da = sdesc(base + ua * (2 * kHalfA), 16, 1024), db = sdesc(base + SM::kB + ub * (2 * SM::kHalfB), 16, 1024);
             const int nf = flushes(sp);
 #pragma unroll
             for (int q = 0; q < GP; ++q) {
                 if (q >= nf) break;
-                const int buf = f & 1;
+                const int buf = __shfl_sync(0xffffffffu, f & 1, 0);
                 if (f >= 2) {
                     ok = wait_warp(&bars.sum_empty[buf], (f / 2 - 1) & 1, &bars);
                     if (!ok) break;
                     tc_fence_after();
                 }
+                if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < 8 / GP; ++i) {
-                    const int kk = q * (8 / GP) + i;  // 16 inputs: 32 bytes on (the descriptors count 16)
-                    mma_ss(tmem + buf * NB, da + ((kk >> 2) * kHalfA + (kk & 3) * 32) / 16,
-                           db + ((kk >> 2) * SM::kHalfB + (kk & 3) * 32) / 16, idesc, i != 0, leader);
+                    for (int i = 0; i < 8 / GP; ++i) {
+                        const int kk = q * (8 / GP) + i;  // 16 inputs: 32 bytes on (the descriptors count 16)
+                        mma_ss(d0 + buf * NB, da + ((kk >> 2) * kHalfA + (kk & 3) * 32) / 16,
+                               db + ((kk >> 2) * SM::kHalfB + (kk & 3) * 32) / 16, idesc, i != 0);
+                    }
+                    tc_commit(&bars.sum_full[buf]);
+                    if (q == nf - 1) {
+                        tc_commit(&bars.empty_a[ua]);
+                        tc_commit(&bars.empty_b[ub]);
+                    }
                 }
-                commit(&bars.sum_full[buf], leader);
+                __syncwarp();
                 ++f;
             }
-            commit(&bars.empty_a[sta], leader);
-            commit(&bars.empty_b[stb], leader);
             if (++sta == kStagesA) sta = 0, pha ^= 1;
             if (++stb == kStagesB<NB>) stb = 0, phb ^= 1;
         }
@@ -412,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const bool failed = *reinterpret_cast<volatile int*>(&bars.failed) != 0;
     if (warp == kMmaWarp) {
-        if (failed && lane == 0) {  // MMAs in flight end before their memory goes
+        if (failed && elect_one()) {  // MMAs in flight end before their memory goes
             mbar_init(&bars.full_a[0], 1);
             fence_mbar_init();
             tc_commit(&bars.full_a[0]);
@@ -426,8 +390,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kN = GATED ? 64 : 128, kStep = kThreads / kN;
     const int i = tid % kN, n = tile0 * 16 + i;
     if (!failed && n < a.N) {
-        const float* red = reinterpret_cast<const float*>(smem) + i;
-        // the finished sum of row m: its parts', the smallest first, over the cluster in rank order
+        const int first = tid / kN + rank * kStep, step = cs * kStep;
+        const float* red = reinterpret_cast<const float*>(smem) + first * a.pieces * 128 + i;
+        // the finished sum at `at`: over the cluster, in rank order
         auto sum_at = [&](const float* at) {
             if (cs == 1) return *at;
             float v[8], y = 0.f;
@@ -437,27 +402,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < 8; ++k) y += v[k];
             return y;
         };
-        auto sum = [&](int m, int q) {
-            if (a.pieces == 1) return sum_at(red + m * 128 + q * 64);
-            const float* at = red + column(m, 0) * 128 + q * 64;
-            return sum_at(at + 256) + sum_at(at + 128) + sum_at(at);
+        auto sum = [&](const float* at) {  // over the parts of a row, the smallest first
+            return a.pieces == 1 ? sum_at(at) : sum_at(at + 256) + sum_at(at + 128) + sum_at(at);
         };
-        const int step = cs * kStep;
-        if (a.mode == W4_LINEAR) {
-            const float bias = a.bias ? __ldg(a.bias + n) : 0.f;
+        if (a.mode == W4_LINEAR || a.mode == W4_GATED) {
+            with_type(a.out_dtype, [&](auto one) {
+                using T = decltype(one);
+                T* out = static_cast<T*>(a.out) + (size_t)(m0 + first) * a.ldo + n;
+                const T* res = static_cast<const T*>(a.residual);
+                if (res) res += (size_t)(m0 + first) * a.ldr + n;
+                const float bias = !GATED && a.bias ? __ldg(a.bias + n) : 0.f;
 #pragma unroll 4
-            for (int m = tid / kN + rank * kStep; m < mrows; m += step) {
-                float y = sum(m, 0) + bias;
-                if (a.residual) y += load_as(a.residual, (size_t)(m0 + m) * a.ldr + n, a.out_dtype);
-                store_as(a.out, (size_t)(m0 + m) * a.ldo + n, a.out_dtype, y);
-            }
-        } else if (a.mode == W4_GATED) {
-#pragma unroll 2
-            for (int m = tid / kN + rank * kStep; m < mrows; m += step)
-                store_as(a.out, (size_t)(m0 + m) * a.ldo + n, a.out_dtype, gated(sum(m, 0), sum(m, GATED ? 1 : 0)));
+                for (int m = first; m < mrows; m += step) {
+                    float y = sum(red);
+                    if (GATED) {
+                        y = gated(y, sum(red + 64));
+                    } else {
+                        if (a.bias) y += bias;
+                        if (res) y += to_float(*res), res += (size_t)step * a.ldr;
+                    }
+                    *out = from_float<T>(y);
+                    out += (size_t)step * a.ldo;
+                    red += step * a.pieces * 128;
+                }
+            });
         } else {
-            for (int m = tid / kN + rank * kStep; m < mrows; m += step)
-                w4_epilogue(a, m0 + m, n, sum(m, 0), sum(m, GATED ? 1 : 0));
+            for (int m = first; m < mrows; m += step, red += step * 128)
+                w4_epilogue(a, m0 + m, n, sum(red), sum(red + (GATED ? 64 : 0)));
         }
     }
     if (cs > 1) cluster_sync();  // nobody leaves while its sums are read
@@ -474,7 +445,7 @@ cudaError_t x_map(const W4Args& a, bool bf, int nb, CUtensorMap* map) {
         return fn;
     }();
     if (!encode) return cudaErrorNotSupported;
-    const cuuint64_t dims[2] = {(cuuint64_t)a.K, (cuuint64_t)a.M}, strides[1] = {(cuuint64_t)a.ldx * 2};
+    const cuuint64_t dims[2] = {(cuuint64_t)a.K, (cuuint64_t)a.M * a.pieces}, strides[1] = {(cuuint64_t)a.ldx * 2};
     const cuuint32_t box[2] = {64, (cuuint32_t)nb}, step[2] = {1, 1};
     const CUresult r = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(encode)(
         map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(a.x), dims, strides,
@@ -491,7 +462,7 @@ cudaError_t launch_inst(W4Args a, int gx, int gy, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     CUtensorMap map = {};
     // TMA reads 16-byte aligned rows a multiple of 16 bytes apart
-    a.tma = a.in == W4_X_16 && reinterpret_cast<size_t>(a.x) % 16 == 0 && a.ldx % 8 == 0;
+    a.tma = reinterpret_cast<size_t>(a.x) % 16 == 0 && a.ldx % 8 == 0;
     if (a.tma && (e = x_map(a, BF != 0, NB, &map)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(gx * a.cs), (unsigned)gy);
@@ -538,6 +509,51 @@ cudaError_t launch_w4_tc(W4Args a, int group, bool bf, int nw, cudaStream_t st) 
     a.last_groups = a.Q - (a.S - 1) * (128 / group);
     return bf ? launch_group<1>(a, group, p.nb, nw == 2, p.gx, p.gy, st)
               : launch_group<0>(a, group, p.nb, nw == 2, p.gx, p.gy, st);
+}
+
+// Row m of x as rows 3 m .. 3 m + 2 of parts, ldp elements apart.
+__global__ void __launch_bounds__(256)
+    split_rows_kernel(const float* __restrict__ x, long long ldx, int M, int K, uint16_t* __restrict__ parts, int ldp) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int per = ldp / 8;  // eight elements at a time, zeros from K on
+    const bool wide = (reinterpret_cast<size_t>(x) & 15) == 0 && ldx % 4 == 0;
+    for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < (long long)M * per; u += (long long)gridDim.x * 256) {
+        const long long m = u / per;
+        const int k = (int)(u % per) * 8;
+        const float* row = x + m * ldx + k;
+        float v[8];
+        if (wide && k + 8 <= K) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(row)), e = __ldg(reinterpret_cast<const float4*>(row) + 1);
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = e.x, v[5] = e.y, v[6] = e.z, v[7] = e.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = k + j < K ? __ldg(row + j) : 0.f;
+        }
+        uint16_t p[3][8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) split3(v[j], p[0][j], p[1][j], p[2][j]);
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+            *reinterpret_cast<uint4*>(parts + (m * 3 + q) * ldp + k) =
+                make_uint4(p[q][0] | (uint32_t)p[q][1] << 16, p[q][2] | (uint32_t)p[q][3] << 16,
+                           p[q][4] | (uint32_t)p[q][5] << 16, p[q][6] | (uint32_t)p[q][7] << 16);
+    }
+}
+
+cudaError_t launch_split_rows(const float* x, long long ldx, int M, int K, void* parts, cudaStream_t st) {
+    const int ldp = (K + 7) / 8 * 8;
+    const long long units = (long long)M * (ldp / 8), blocks = (units + 255) / 256;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min(blocks, 8ll * kSms));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return counted(cudaLaunchKernelEx(&cfg, split_rows_kernel, x, ldx, M, K, static_cast<uint16_t*>(parts), ldp));
 }
 
 cudaError_t step_status(int* status) {

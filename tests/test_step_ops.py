@@ -493,8 +493,12 @@ def test_step_of_operators(kv):
 
 
 # ------------------------------------------------------------------- refusals
+_matrices = []
+
+
 def matrix(kv, n=32, k=64, group=32, device=0, codes=0x1000, scales=0x1000, zeros=None):
-    return C.byref(kv._W4Matrix(device, n, k, group, codes, scales, zeros))
+    _matrices.append(kv._W4Matrix(device, n, k, group, codes, scales, zeros))
+    return C.addressof(_matrices[-1])
 
 
 def refused(kv, fn, *args):
@@ -506,7 +510,7 @@ def refused(kv, fn, *args):
 
 def test_linear_refusals(kv):
     A, B = 0x100000, 0x900000
-    ok = dict(w=matrix(kv), x=A, xd=0, m=4, ldx=64, bias=None, res=None, ldr=0, out=B, od=2, ldo=32)
+    ok = dict(w=matrix(kv), x=A, xd=0, m=4, ldx=64, bias=None, res=None, ldr=0, out=B, od=2, ldo=32, work=None)
 
     def go(**kw):
         return refused(kv, "w4_linear", *{**ok, **kw}.values(), None)
@@ -535,20 +539,34 @@ def test_linear_refusals(kv):
     go(res=A, ldr=31)
     assert "without being out" in go(res=B + 4, ldr=32)
     assert "without being out" in go(res=B, ldr=33)
-    g = dict(gate=matrix(kv), up=matrix(kv), x=A, xd=0, m=4, ldx=64, out=B, od=2, ldo=32)
+    go(work=A + 8)
+    assert "scratch overlaps" in go(xd=2, m=100, work=A + 16)
+    assert "scratch overlaps" in go(xd=2, m=100, work=B - 16)
+    g = dict(gate=matrix(kv), up=matrix(kv), x=A, xd=0, m=4, ldx=64, out=B, od=2, ldo=32, work=None)
     for up in (None, matrix(kv, n=33), matrix(kv, k=65), matrix(kv, group=64), matrix(kv, device=1), matrix(kv, zeros=0x1000)):
         refused(kv, "w4_gated", *{**g, "up": up}.values(), None)
-    refused(kv, "w4_quantize", matrix(kv), A, 2, 64, None)
-    refused(kv, "w4_quantize", matrix(kv), A, 0, 63, None)
-    refused(kv, "w4_quantize", matrix(kv), A + 1, 0, 64, None)
-    refused(kv, "w4_dequantize", matrix(kv), None, 64, None)
-    refused(kv, "w4_dequantize", matrix(kv), A, 63, None)
+    m = C.byref(_matrices[0])
+    refused(kv, "w4_quantize", m, A, 2, 64, None)
+    refused(kv, "w4_quantize", m, A, 0, 63, None)
+    refused(kv, "w4_quantize", m, A + 1, 0, 64, None)
+    refused(kv, "w4_dequantize", m, None, 64, None)
+    refused(kv, "w4_dequantize", m, A, 63, None)
 
 
 def test_no_rows_need_no_device(kv):
-    kv.call("w4_linear", matrix(kv), None, 0, 0, 64, None, None, 0, None, 2, 32, None)
-    kv.call("w4_gated", matrix(kv), matrix(kv), None, 0, 0, 64, None, 2, 32, None)
+    kv.call("w4_linear", matrix(kv), None, 0, 0, 64, None, None, 0, None, 2, 32, None, None)
+    kv.call("w4_gated", matrix(kv), matrix(kv), None, 0, 0, 64, None, 2, 32, None, None)
     kv.call("logits_adjust", C.byref(kv._LogitsCall(device=0, rows=0, vocab=5, dtype=2)), None)
+
+
+def test_work_bytes(kv):
+    n = C.c_size_t()
+    for m, k, dtype, some in ((1, 100, 2, False), (300, 100, 2, True), (300, 100, 0, False), (300, 101, 1, False)):
+        kv.call("w4_work_bytes", 64, k, dtype, m, 0, C.byref(n))
+        assert n.value == (3 * m * -(-k // 8) * 16 if some else 0)
+    refused(kv, "w4_work_bytes", 64, 64, 5, 1, 0, C.byref(n))
+    refused(kv, "w4_work_bytes", 64, 64, 2, -1, 0, C.byref(n))
+    refused(kv, "w4_work_bytes", 64, 64, 2, 1, 0, None)
 
 
 def test_w4_sizes(kv):
