@@ -82,7 +82,8 @@ int w4_dequantize(const w4_matrix* m, float* out, long long ldo, void* stream);
  * before its scale, so that sum has to stay within fp32 (|x| below 1e35 does).
  * out must not overlap x.
  * work: w4_work_bytes() of scratch, 16-byte aligned, overlapping nothing else,
- * or NULL: many rows of an fp32 x go through it, and take longer without it. */
+ * or NULL: many rows of an x that is fp32, or not in 16-byte aligned rows, go
+ * through it, and take longer without it. */
 int w4_linear(const w4_matrix* w, const void* x, int x_dtype, int m, long long ldx, const float* bias,
               const void* residual, long long ldr, void* out, int out_dtype, long long ldo, void* work, void* stream);
 
@@ -94,7 +95,7 @@ int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dt
 
 /* Scratch of w4_linear (gated 0) or w4_gated (gated 1) for m rows of x: 0
  * where none helps. */
-int w4_work_bytes(int n, int k, int x_dtype, int m, int gated, size_t* bytes);
+int w4_work_bytes(int n, int k, int group, int x_dtype, int m, int gated, size_t* bytes);
 
 /* The waits inside the kernels for many rows are bounded (about a second):
  * *status is KV_OK, or KV_ERR_TIMEOUT if one has run out on `device` since the

@@ -116,7 +116,7 @@ _SIGS.update({
     "w4_dequantize": [_w4p, _vp, C.c_longlong, _vp],
     "w4_linear": [_vp, _vp, C.c_int, C.c_int, C.c_longlong, _vp, _vp, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp, _vp],
     "w4_gated": [_vp, _vp, _vp, C.c_int, C.c_int, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp, _vp],
-    "w4_work_bytes": [C.c_int] * 5 + [C.POINTER(C.c_size_t)],
+    "w4_work_bytes": [C.c_int] * 6 + [C.POINTER(C.c_size_t)],
     "logits_adjust": [C.POINTER(_LogitsCall), _vp],
     "step_ops_status": [C.c_int, _ip],
 })
@@ -475,13 +475,16 @@ def _stream_on(stream, device: int):
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _scratch(w, x, m: int, gated: int, stream):
-    """Scratch for many rows of an fp32 x, held by the caching allocator for `stream`."""
-    import torch
+def _scratch(w, x, dtype: int, m: int, ldx: int, gated: int, stream):
+    """Scratch for many rows of an x that is fp32 or not in 16-byte aligned
+    rows, held by the caching allocator for `stream`; None where none helps."""
+    if m < 5 or (dtype != STEP_F32 and ldx % 8 == 0 and x.data_ptr() % 16 == 0):
+        return None
     n = C.c_size_t()
-    call("w4_work_bytes", w.n, w.k, STEP_F32, m, gated, C.byref(n))
+    call("w4_work_bytes", w.n, w.k, w.group, dtype, m, gated, C.byref(n))
     if not n.value:
         return None
+    import torch
     t = torch.empty(n.value, dtype=torch.uint8, device=x.device)
     if stream is not None:
         t.record_stream(torch.cuda.ExternalStream(stream, device=x.device) if isinstance(stream, int) else stream)
@@ -548,7 +551,7 @@ def w4_linear(w: W4, x, out, bias=None, residual=None, stream=None) -> None:
     ldx = _rows(x, dev, "x", None, w.k)
     m = x.shape[0]
     ldo = _rows(out, dev, "out", m, w.n)
-    b = r = work = None
+    b = r = None
     ldr = 0
     xd = _step_dtype(x, "x")
     if bias is not None:
@@ -559,8 +562,7 @@ def w4_linear(w: W4, x, out, bias=None, residual=None, stream=None) -> None:
         if residual.dtype != out.dtype:
             raise ValueError("residual: out's element type is expected")
         r = residual.data_ptr()
-    if xd == STEP_F32 and m > 4:  # fewer rows need none
-        work = _scratch(w, x, m, 0, stream)
+    work = _scratch(w, x, xd, m, ldx, 0, stream)
     rc = _lib.w4_linear(w._at, x.data_ptr(), xd, m, ldx, b, r, ldr, out.data_ptr(), _step_dtype(out, "out"), ldo,
                         work.data_ptr() if work is not None else None, _stream_on(stream, dev))
     if rc:
@@ -574,7 +576,7 @@ def w4_gated(gate: W4, up: W4, x, out, stream=None) -> None:
     m = x.shape[0]
     ldo = _rows(out, dev, "out", m, gate.n)
     xd = _step_dtype(x, "x")
-    work = _scratch(gate, x, m, 1, stream) if xd == STEP_F32 and m > 4 else None
+    work = _scratch(gate, x, xd, m, ldx, 1, stream)
     rc = _lib.w4_gated(gate._at, up._at, x.data_ptr(), xd, m, ldx, out.data_ptr(), _step_dtype(out, "out"), ldo,
                        work.data_ptr() if work is not None else None, _stream_on(stream, dev))
     if rc:

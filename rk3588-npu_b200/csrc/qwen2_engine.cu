@@ -605,7 +605,7 @@ cudaError_t project(const qw2_model* m, int mode, int in, const GemvArgs& a, con
     w.x = a.x;
     w.ldx = a.K;
     w.in = in == 0 ? W4_X_16 : in == 1 ? W4_X_ROUND : W4_X_NORM;
-    if (w.in != W4_X_16 && w4_use_tc(w.M, w.T, 1, q2 ? 2 : 1)) {
+    if (w.in != W4_X_16 && w4_use_tc(w.M, w.T, w.S, 1, q2 ? 2 : 1, q.group)) {
         // many rows: the norm and the rounding once, not in every tile
         const cudaError_t e = w.in == W4_X_NORM ? launch_rmsnorm_f16(static_cast<const float*>(a.x), a.norm_w, m->x16, a.M, a.K, a.eps, st)
                                                 : launch_to_f16_exact(static_cast<const float*>(a.x), (long)a.M * a.K, m->x16, st);

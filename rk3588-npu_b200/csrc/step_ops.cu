@@ -89,15 +89,16 @@ void set_x(W4Args& a, const void* x, int x_dtype, int m, long long ldx) {
     a.pieces = x_dtype == STEP_F32 ? 3 : 1;
 }
 
-size_t work_bytes(int n, int k, int x_dtype, int m, int gated) {
-    return x_dtype == STEP_F32 && w4_use_tc(m, (n + 15) / 16, 3, gated ? 2 : 1) ? w4_split_bytes(m, k) : 0;
+size_t work_bytes(int n, int k, int group, int x_dtype, int m, int gated) {
+    const int pieces = x_dtype == STEP_F32 ? 3 : 1;
+    return w4_use_tc(m, (n + 15) / 16, (k + 127) / 128, pieces, gated ? 2 : 1, group) ? w4_rows_bytes(m, k, pieces) : 0;
 }
 
 int check_work(const w4_matrix& w, const void* x, int x_dtype, int m, long long ldx, const void* out, int out_dtype,
                long long ldo, int gated, const void* work) {
     if (!work || m == 0) return KV_OK;
     if (!aligned(work, 16)) return sfail(KV_ERR_INVAL, "scratch needs 16-byte alignment");
-    const Range r(work, 1, (long long)work_bytes(w.n, w.k, x_dtype, m, gated), 0, 1);
+    const Range r(work, 1, (long long)work_bytes(w.n, w.k, w.group, x_dtype, m, gated), 0, 1);
     if (r.meets(Range(x, m, w.k, ldx, esize(x_dtype))) || r.meets(Range(out, m, w.n, ldo, esize(out_dtype))))
         return sfail(KV_ERR_INVAL, "scratch overlaps x or out");
     return KV_OK;
@@ -195,11 +196,11 @@ int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dt
     return launched(launch_w4(a, gate->group, x_dtype != STEP_F16, 2, static_cast<cudaStream_t>(stream)), "w4_gated");
 }
 
-int w4_work_bytes(int n, int k, int x_dtype, int m, int gated, size_t* bytes) {
-    ST_OK(check_shape(n, k, 32));
+int w4_work_bytes(int n, int k, int group, int x_dtype, int m, int gated, size_t* bytes) {
+    ST_OK(check_shape(n, k, group));
     ST_OK(check_dtype(x_dtype, "x"));
     if (m < 0 || m > 1 << 20 || !bytes) return sfail(KV_ERR_INVAL, "%d rows, or NULL bytes", m);
-    *bytes = work_bytes(n, k, x_dtype, m, gated);
+    *bytes = work_bytes(n, k, group, x_dtype, m, gated);
     return KV_OK;
 }
 

@@ -30,7 +30,7 @@ struct W4Args {
     long long ldx = 0;
     int in = W4_X_16, mode = W4_LINEAR;
     int pieces = 1;           // operand rows per x row (3 for W4_X_F32)
-    void* work = nullptr;     // room for w4_split_bytes, or NULL
+    void* work = nullptr;     // room for w4_rows_bytes, or NULL
     int out_dtype = STEP_F32;
     const float* bias = nullptr;
     const void* residual = nullptr;
@@ -42,8 +42,8 @@ struct W4Args {
     int rows = 0;             // x rows per pass
     int ks = 1, cs = 1;       // a tile's spans over ks warps and cs CTAs
     int chunk = 0;            // spans of x staged at a time
+    int batches = 2;          // of codes per warp in shared memory
     int last_groups = 0;      // groups of a row's last span
-    bool tma = false;         // (tcgen05 form) x comes by TMA
     bool early = false;       // the weights may be read before the previous kernel of the stream ends
 
     void set_matrix(int i, const w4_matrix& w) {
@@ -61,40 +61,57 @@ struct W4Args {
 constexpr int kSms = 148;
 constexpr int kW4MaxSmem = 227 * 1024;
 // Spans that a warp copies at a time (two such batches in shared memory).
-constexpr int w4_batch(int nw, int nt) { return nw == 2 || nt >= 4 ? 2 : 4; }
+constexpr int w4_batch(int nw) { return nw == 2 ? 2 : 4; }
 // Floats of a warp's partial tile: 20 per column (16 rows, padded against bank
 // conflicts), 4 more so that the warps' tiles start in different banks.
 constexpr int w4_red_floats(int nw, int nt) { return nw * nt * 8 * 20 + 4; }
 
 struct W4Plan {
-    int nt, rows, passes, ks, cs, chunk, gx, smem;
+    int nt, rows, passes, ks, cs, chunk, batches, gx, smem;
 };
 
+// How a product is laid out: x rows per pass; the warps that share a tile's
+// spans (ks), by the least
+//   tiles in turn * (a warp's spans + 2 for joining the parts),
+// where a last turn that fills part of the SMs counts half of itself at least; and
+// the CTAs that share them (cs) where tiles are few, as long as all run at once.
+// Measured, us at ks = 1 / 2 / 4 / 8: 2048 x 1536, one row 5.9 / 4.7 / 3.9 / 3.6; gated 8960 x
+// 1536, one row 9.7 / 8.9 / 6.5 / 8.1, 16 rows 13.7 / 10.8 / 11.6 / 12.9; 20000 x 4096, one row
+// 18.1 / 15.3 / 14.5 / 16.3; 151936 x 1536, one row 29.5 / 36 / 44 / 67.  Clusters in several
+// waves lost: 1536 x 8960, one row 6.1 us without, 9.0 in threes, 21 in sixes.
 inline W4Plan w4_plan(int M, int T, int S, int pieces, int nw, int sms) {
-    W4Plan p{};
-    const int nt_max = nw == 2 ? 4 : 8;
-    const int most = nt_max * 8 / pieces;
-    p.passes = (M + most - 1) / most;
-    p.rows = (M + p.passes - 1) / p.passes;
-    const int vr = p.rows * pieces;
-    p.nt = vr <= 8 ? 1 : vr <= 16 ? 2 : vr <= 32 ? 4 : 8;
-    // warps that share a tile's spans: as many as keep every warp of two
-    // CTAs per SM busy, no more than there are spans
-    const int share = std::max(1, std::min(S, sms * 16 / std::max(1, T * p.passes)));
-    p.ks = share >= 8 ? 8 : share >= 4 ? 4 : share >= 2 ? 2 : 1;
-    p.cs = share >= 64 ? 8 : share >= 32 ? 4 : share >= 16 ? 2 : 1;
-    const int fixed = 8 * (2 * w4_batch(nw, p.nt) * nw * 1216 + w4_red_floats(nw, p.nt) * 4);
-    const int spans = (S + p.cs - 1) / p.cs;
-    // staged spans: all of the CTA's, or as many batches of its warps as fit
-    const int fit = ((kW4MaxSmem - fixed) / (vr * 2) - 32) / 128;
-    const int unit = w4_batch(nw, p.nt);
-    while (p.ks > 1 && p.ks * unit > fit) p.ks /= 2;
-    p.chunk = spans <= fit ? spans : fit / (p.ks * unit) * (p.ks * unit);
-    p.smem = fixed + vr * (p.chunk * 128 + 32) * 2;
-    const int groups = (T + 8 / p.ks - 1) / (8 / p.ks);
-    const int per_sm = p.smem <= 113 * 1024 && p.nt * nw <= 2 ? 2 : 1;
-    p.gx = std::min(groups, std::max(1, sms * per_sm / (p.passes * p.cs)));
-    return p;
+    W4Plan best{};
+    const int most = 32 / pieces;
+    const int passes = (M + most - 1) / most, rows = (M + passes - 1) / passes, vr = rows * pieces;
+    const int nt = vr <= 8 ? 1 : vr <= 16 ? 2 : 4;
+    const int unit = w4_batch(nw), batch = unit * nw * 1216, red = 8 * w4_red_floats(nw, nt) * 4;
+    const int fit = ((kW4MaxSmem - red - 8 * 2 * batch) / (vr * 2) - 32) / 128;  // spans of x that fit at once
+    double least = 0;
+    for (int ks = 1; ks <= 8 && ks <= S; ks *= 2) {
+        W4Plan p{nt, rows, passes, ks, 1};
+        const int groups = (T + 8 / ks - 1) / (8 / ks);
+        if (ks == 8)
+            while (p.cs < 8 && groups * passes * p.cs * 2 <= sms && S >= 8 * p.cs * 2 * 2) p.cs *= 2;
+        const int spans = (S + p.cs - 1) / p.cs, per_warp = (spans + ks - 1) / ks;
+        if (fit < ks * unit && fit < spans) continue;
+        // all of the CTA's spans, or as many batches of its warps as fit
+        p.chunk = spans <= fit ? spans : fit / (ks * unit) * (ks * unit);
+        const int fixed = red + vr * (p.chunk * 128 + 32) * 2;
+        double turns = 0;
+        for (p.batches = 1; p.batches <= 2; ++p.batches) {  // one batch of codes is enough for one tile of so many spans
+            p.smem = fixed + 8 * p.batches * batch;
+            const int per_sm = p.smem <= 113 * 1024 && nt * nw <= 2 ? 2 : 1;
+            const int slots = std::max(1, sms * per_sm / (passes * p.cs));
+            p.gx = std::min(groups, slots);
+            turns = (double)groups / slots;
+            if (turns <= 1 && per_warp <= unit) break;
+        }
+        p.batches = std::min(p.batches, 2);
+        const double whole = (double)(long long)turns, part = turns - whole;
+        const double cost = std::max(1.0, whole + (part > 0 ? 0.5 + 0.5 * part : 0)) * (per_warp + 2);
+        if (least == 0 || cost < least) least = cost, best = p;
+    }
+    return best;
 }
 
 // The tcgen05 form's plan: tiles of 128 weight rows (64 of each matrix of a
@@ -120,19 +137,25 @@ inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw) {
 }
 
 // Rows from which the tcgen05 form is the faster one: its tiles cost the same
-// for one row as for 64, so it depends on how many of them there are.  Measured, us
-// (w4_kernels.cu / tcgen05): 1536 x 8960, 16 rows 18 / 12, 12 rows 12.3 / 12.3;
-// 8960 x 1536 gated, 24 rows 15.9 / 14, 16 rows 11.4 / 14; 151936 x 1536, 48 rows
-// 158 / 138, 32 rows 103 / 137.
-inline bool w4_use_tc(int M, int T, int pieces, int nw) {
+// for one row as for 64, more with small groups (each is read and scaled by
+// itself), and the other form suffers from long rows, of which it keeps every
+// staged x.  Measured, us (w4_kernels.cu / tcgen05): 1536 x 8960, 16 rows 18 / 12,
+// 12 rows 12.2 / 12.3; 2048 x 1536, 48 rows 11.1 / 10.5, 32 rows 6.3 / 9.9; 8960 x 1536
+// gated, 24 rows 15.9 / 13.7, 16 rows 11.4 / 14; the same in groups of 32, 48 rows
+// 30.5 / 24, 32 rows 20.7 / 23.5; 151936 x 1536, 48 rows 158 / 129, 32 rows 103 / 137.
+inline bool w4_use_tc(int M, int T, int S, int pieces, int nw, int group) {
     const int tiles = (T + 7) / 8 * nw, rows = M * pieces;
-    return rows > (tiles <= kSms / 2 ? 14 : tiles <= kSms ? 20 : 40);
+    if (tiles <= kSms && S >= 32) return rows > (group == 32 ? 24 : 8);
+    return rows > (nw == 2 && tiles <= kSms && group > 32 ? 20 : 40);
 }
+// Rows of 16-bit values that a tensor map can describe.
+inline bool w4_tma_rows(const void* x, long long ldx) { return reinterpret_cast<size_t>(x) % 16 == 0 && ldx % 8 == 0; }
 
 cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st);
-// The three bf16 parts of fp32 rows, for the tcgen05 form: [3 M][K rounded up to 8].
-inline size_t w4_split_bytes(int M, int K) { return (size_t)3 * M * ((K + 7) / 8 * 8) * 2; }
-cudaError_t launch_split_rows(const float* x, long long ldx, int M, int K, void* parts, cudaStream_t st);
+// Rows of x made for the tcgen05 form: an fp32 row's three bf16 parts, or a 16-bit row
+// as it is, K rounded up to 8 elements each.
+inline size_t w4_rows_bytes(int M, int K, int pieces) { return (size_t)pieces * M * ((K + 7) / 8 * 8) * 2; }
+cudaError_t launch_rows(bool f32, const void* x, long long ldx, int M, int K, void* to, cudaStream_t st);
 cudaError_t launch_w4_tc(W4Args a, int group, bool bf, int nw, cudaStream_t st);
 // The status of the waits in launch_w4_tc's kernels on the current device
 // (0, or KV_ERR_TIMEOUT), cleared by reading it.

@@ -3,7 +3,7 @@
 // that bring a matrix to 4 bits and back.
 //
 // Product: y^T = W x^T as mma.sync m16n8k16 tiles, W the A operand (16 weight
-// rows x 16 inputs), up to 64 rows of x the B operand.  With
+// rows x 16 inputs), up to 32 rows of x the B operand.  With
 //   y[m][n] = sum_g s[n][g] * (sum_{k in g} (q[n][k] - z[n][g]) x[m][k])
 // the integers q - z are exact in fp16 and in bf16, so the tensor core sums
 // exact products in fp32 within a group, and the group's scale multiplies
@@ -170,8 +170,8 @@ __device__ __forceinline__ void stage_rows(const W4Args& a, int m0, int mrows, i
 template <int BF, int NT, int NW, int GP>
 __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     w4_kernel(const __grid_constant__ W4Args a) {
-    constexpr int kU = w4_batch(NW, NT);        // spans per batch
-    constexpr int kBatch = kU * NW * kSlot;     // bytes; two batches per warp: one in flight, one in use
+    constexpr int kU = w4_batch(NW);        // spans per batch
+    constexpr int kBatch = kU * NW * kSlot;     // bytes; two batches per warp, one in flight, one in use (or one is all)
     constexpr int kCols = NT * 8;
     constexpr int kRedWarp = w4_red_floats(NW, NT);
     extern __shared__ __align__(16) uint8_t smem[];
@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     const int m0 = blockIdx.y * a.rows, mrows = min(a.rows, a.M - m0), vr = mrows * a.pieces;
     const int ldx = a.chunk * 128 + 32;  // halves per staged row: an odd number of 64-byte units
     uint16_t* xs = reinterpret_cast<uint16_t*>(smem);
-    uint8_t* ring = smem + (size_t)a.rows * a.pieces * ldx * 2 + (size_t)warp * (2 * kBatch);
-    float* red = reinterpret_cast<float*>(smem + (size_t)a.rows * a.pieces * ldx * 2 + kWarps * 2 * kBatch);
+    uint8_t* ring = smem + (size_t)a.rows * a.pieces * ldx * 2 + (size_t)warp * (a.batches * kBatch);
+    float* red = reinterpret_cast<float*>(smem + (size_t)a.rows * a.pieces * ldx * 2 + (size_t)kWarps * a.batches * kBatch);
 
     const int s0 = (int)((long long)a.S * rank / cs), s1 = (int)((long long)a.S * (rank + 1) / cs);
     const int rounds = (a.T + tpc * gx - 1) / (tpc * gx);
@@ -624,17 +624,16 @@ cudaError_t launch_nt(const W4Args& a, int nt, int nw, int group, int gx, int pa
     }
     if (nt == 1) return launch_gp<BF, 1, 1>(a, group, gx, passes, smem, st);
     if (nt == 2) return launch_gp<BF, 2, 1>(a, group, gx, passes, smem, st);
-    if (nt == 4) return launch_gp<BF, 4, 1>(a, group, gx, passes, smem, st);
-    return launch_gp<BF, 8, 1>(a, group, gx, passes, smem, st);
+    return launch_gp<BF, 4, 1>(a, group, gx, passes, smem, st);
 }
 
 }  // namespace
 
 cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st) {
-    if (w4_use_tc(a.M, a.T, a.pieces, nw)) {
-        if (a.in == W4_X_16) return launch_w4_tc(a, group, bf, nw, st);
-        if (a.in == W4_X_F32 && a.work) {
-            const cudaError_t e = launch_split_rows(static_cast<const float*>(a.x), a.ldx, a.M, a.K, a.work, st);
+    if (w4_use_tc(a.M, a.T, a.S, a.pieces, nw, group)) {
+        if (a.in == W4_X_16 && w4_tma_rows(a.x, a.ldx)) return launch_w4_tc(a, group, bf, nw, st);
+        if ((a.in == W4_X_16 || a.in == W4_X_F32) && a.work) {
+            const cudaError_t e = launch_rows(a.in == W4_X_F32, a.x, a.ldx, a.M, a.K, a.work, st);
             if (e != cudaSuccess) return e;
             a.x = a.work;
             a.ldx = (a.K + 7) / 8 * 8;
@@ -643,6 +642,7 @@ cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st) {
         }
     }
     const W4Plan p = w4_plan(a.M, a.T, a.S, a.pieces, nw, kSms);
+    a.batches = p.batches;
     a.rows = p.rows;
     a.ks = p.ks;
     a.cs = p.cs;

@@ -1,14 +1,14 @@
 // w4_tc_kernel.cu -- the 4-bit projections for many rows of x, on tcgen05.
 //
-// x is 16-bit here: an fp32 x comes as its three bf16 parts (w4_split_rows).
+// x is 16-bit here, in rows that TMA can address: an fp32 x comes as its three
+// bf16 parts, unaligned rows as copies (launch_rows).
 // The same sums as w4_kernels.cu (integers q - z exact in the operand type,
 // a group's products summed in fp32, the scale applied to the sum), with the
 // roles of a tile spread over the warps of one CTA:
 //   warps 0-3   unpack codes into the A operand: 128 weight rows x 128 inputs
 //               in shared memory, 128-byte-swizzled K-major;
-//   warps 4-6   bring the B operand: NB rows of x x 128 inputs, the same
-//               layout (by TMA, which fills what lies outside x with zeros;
-//               rows that TMA cannot address, element by element);
+//   warp 4      brings the B operand: NB rows of x x 128 inputs, the same
+//               layout, by TMA, which fills what lies outside x with zeros;
 //   warp 7      issues the MMAs: each group of inputs into a fresh sum in
 //               tensor memory, two of them in turn;
 //   warps 8-15  read a finished group (lane = weight row) and add it, times
@@ -48,7 +48,7 @@ constexpr int kStagesB = NB == 256 ? 2 : 4;  // copies in flight
 constexpr int kAhead = 3;     // spans of codes in shared memory, per unpacking warp
 constexpr int kCodes = 2 * 1024 + 128;  // a span of a warp's two tiles, and their zero points
 constexpr int kThreads = 16 * 32;
-constexpr int kBWarps = 3, kMmaWarp = 7;
+constexpr int kMmaWarp = 7;
 constexpr int kHalfA = 128 * 128;  // 64 inputs of 128 rows
 constexpr long long kWaitLimit = 2000000000LL;  // SM clocks: about a second
 
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bars.empty_a[i], 1);
         }
         for (int i = 0; i < kStagesB<NB>; ++i) {
-            mbar_init(&bars.full_b[i], a.tma ? 1 : kBWarps);
+            mbar_init(&bars.full_b[i], 1);
             mbar_init(&bars.empty_b[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -239,46 +239,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             slot = slot + 1 == kAhead ? 0 : slot + 1;
         }
         cp_wait<0>();
-    } else if (warp < 4 + kBWarps) {
-        // --------------------------------------------------------- B: rows of x
+    } else if (warp < kMmaWarp) {
+        // ------------------------------------------- B: rows of x (warp 4; 5 and 6 idle)
         if (NB == 256) regs_down<56>();
-        const int t = tid - 128;
-        if (a.tma) {
-            if (warp == 4) {
-                int st = 0, ph = 1;
-                for (int sp = s0; sp < s1; ++sp) {
-                    if (sp - s0 >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], ph, &bars)) break;
-                    if (lane == 0) {
-                        const uint32_t dst = smem_u32(smem) + SM::kB + st * (2 * SM::kHalfB);
-                        mbar_arrive_expect_tx(&bars.full_b[st], 2 * SM::kHalfB);
-                        tma_rows(dst, &xmap, sp * 128, m0 * a.pieces, &bars.full_b[st]);
-                        tma_rows(dst + SM::kHalfB, &xmap, sp * 128 + 64, m0 * a.pieces, &bars.full_b[st]);
-                    }
-                    __syncwarp();
-                    if (++st == kStagesB<NB>) st = 0, ph ^= 1;
+        if (warp == 4) {
+            int st = 0, ph = 1;
+            for (int sp = s0; sp < s1; ++sp) {
+                if (sp - s0 >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], ph, &bars)) break;
+                if (lane == 0) {
+                    const uint32_t dst = smem_u32(smem) + SM::kB + st * (2 * SM::kHalfB);
+                    mbar_arrive_expect_tx(&bars.full_b[st], 2 * SM::kHalfB);
+                    tma_rows(dst, &xmap, sp * 128, m0 * a.pieces, &bars.full_b[st]);
+                    tma_rows(dst + SM::kHalfB, &xmap, sp * 128 + 64, m0 * a.pieces, &bars.full_b[st]);
                 }
+                __syncwarp();
+                if (++st == kStagesB<NB>) st = 0, ph ^= 1;
             }
-        } else {
-        // (columns without a row keep what is there: a column's sums are its own)
-        int it = 0;
-        for (int sp = s0; sp < s1; ++sp, ++it) {
-            const int st = it % kStagesB<NB>;
-            if (it >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], (it / kStagesB<NB> - 1) & 1, &bars)) break;
-            uint8_t* dst = smem + SM::kB + st * (2 * SM::kHalfB);
-#pragma unroll 2
-            for (int u = t; u < mrows * 16; u += kBWarps * 32) {  // eight inputs at a time
-                const int r = u >> 4, c = u & 15, k = sp * 128 + c * 8;
-                const uint16_t* row = static_cast<const uint16_t*>(a.x) + (size_t)(m0 + r) * a.ldx + k;
-                uint32_t e[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = k + j < a.K ? (uint32_t)__ldg(row + j) : 0u;
-                *reinterpret_cast<uint4*>(dst + (c >> 3) * SM::kHalfB + swz(r, c & 7)) =
-                    make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.full_b[st]);
-        }
         }
     } else if (warp == kMmaWarp) {
         // ----------------------------------------------------------- MMA issue
@@ -335,30 +311,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         float acc[NB / 2];
 #pragma unroll
         for (int i = 0; i < NB / 2; ++i) acc[i] = 0.f;
-        const int g0 = s0 * GP, g1 = min(s1 * GP, a.Q);
-        float s = __half2float(sc[(size_t)g0 * 16]);
+        float next[GP];  // the scales of a span, loaded a span ahead
+        auto load_scales = [&](int sp) {
+#pragma unroll
+            for (int q = 0; q < GP; ++q) next[q] = sp < s1 && sp * GP + q < a.Q ? __half2float(sc[(size_t)(sp * GP + q) * 16]) : 0.f;
+        };
+        load_scales(s0);
         bool ok = true;
-        for (int gi = g0; ok && gi < g1; ++gi) {
-            const int f = gi - g0, buf = f & 1;
-            const float s_next = gi + 1 < g1 ? __half2float(sc[(size_t)(gi + 1) * 16]) : 0.f;
-            ok = wait_warp(&bars.sum_full[buf], (f / 2) & 1, &bars);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * NB + half * (NB / 2));
+        int f = 0;
+        for (int sp = s0; ok && sp < s1; ++sp) {
+            float now[GP];
 #pragma unroll
-            for (int b = 0; b < NB / 64; ++b) {
-                float d[32];
-                tmem_ld32(at + b * 32, d);
-                tc_wait_ld();
-                if (b == NB / 64 - 1) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars.sum_empty[buf]);
+            for (int q = 0; q < GP; ++q) now[q] = next[q];
+            load_scales(sp + 1);
+            const int nf = flushes(sp);
+#pragma unroll
+            for (int q = 0; q < GP; ++q) {
+                if (q >= nf) break;
+                const int buf = f & 1;
+                ok = wait_warp(&bars.sum_full[buf], (f / 2) & 1, &bars);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * NB + half * (NB / 2));
+#pragma unroll
+                for (int b = 0; b < NB / 64; ++b) {
+                    float d[32];
+                    tmem_ld32(at + b * 32, d);
+                    tc_wait_ld();
+                    if (b == NB / 64 - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bars.sum_empty[buf]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[b * 32 + i] = fmaf(now[q], d[i], acc[b * 32 + i]);
                 }
-#pragma unroll
-                for (int i = 0; i < 32; ++i) acc[b * 32 + i] = fmaf(s, d[i], acc[b * 32 + i]);
+                ++f;
             }
-            s = s_next;
         }
         // every MMA has read its operands: the stages become the sums
         float* red = reinterpret_cast<float*>(smem) + (size_t)half * (NB / 2) * 128 + r;
@@ -455,15 +444,13 @@ cudaError_t x_map(const W4Args& a, bool bf, int nb, CUtensorMap* map) {
 }
 
 template <int BF, int GP, int NB, bool GATED>
-cudaError_t launch_inst(W4Args a, int gx, int gy, cudaStream_t st) {
+cudaError_t launch_inst(const W4Args& a, int gx, int gy, cudaStream_t st) {
     auto fn = w4_tc_kernel<BF, GP, NB, GATED>;
     static SmemGrant grant;
     cudaError_t e = grant.raise(reinterpret_cast<const void*>(fn), Smem<NB>::kBytes);
     if (e != cudaSuccess) return e;
     CUtensorMap map = {};
-    // TMA reads 16-byte aligned rows a multiple of 16 bytes apart
-    a.tma = reinterpret_cast<size_t>(a.x) % 16 == 0 && a.ldx % 8 == 0;
-    if (a.tma && (e = x_map(a, BF != 0, NB, &map)) != cudaSuccess) return e;
+    if ((e = x_map(a, BF != 0, NB, &map)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(gx * a.cs), (unsigned)gy);
     cfg.blockDim = dim3(kThreads);
@@ -511,39 +498,46 @@ cudaError_t launch_w4_tc(W4Args a, int group, bool bf, int nw, cudaStream_t st) 
               : launch_group<0>(a, group, p.nb, nw == 2, p.gx, p.gy, st);
 }
 
-// Row m of x as rows 3 m .. 3 m + 2 of parts, ldp elements apart.
+// Rows of x as TMA can address them, ldp elements apart, zeros from K on:
+// row m as rows 3 m .. 3 m + 2 of its parts (T float), or as it is.
+template <class T>
 __global__ void __launch_bounds__(256)
-    split_rows_kernel(const float* __restrict__ x, long long ldx, int M, int K, uint16_t* __restrict__ parts, int ldp) {
+    rows_kernel(const T* __restrict__ x, long long ldx, int M, int K, uint16_t* __restrict__ to, int ldp) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int per = ldp / 8;  // eight elements at a time, zeros from K on
-    const bool wide = (reinterpret_cast<size_t>(x) & 15) == 0 && ldx % 4 == 0;
+    const int per = ldp / 8;  // eight elements at a time
+    const bool wide = (reinterpret_cast<size_t>(x) & 15) == 0 && ldx * sizeof(T) % 16 == 0;
     for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < (long long)M * per; u += (long long)gridDim.x * 256) {
         const long long m = u / per;
         const int k = (int)(u % per) * 8;
-        const float* row = x + m * ldx + k;
-        float v[8];
+        const T* row = x + m * ldx + k;
+        T v[8];
         if (wide && k + 8 <= K) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(row)), e = __ldg(reinterpret_cast<const float4*>(row) + 1);
-            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = e.x, v[5] = e.y, v[6] = e.z, v[7] = e.w;
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(v)[j] = __ldg(reinterpret_cast<const uint4*>(row) + j);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = k + j < K ? __ldg(row + j) : 0.f;
+            for (int j = 0; j < 8; ++j) v[j] = k + j < K ? __ldg(row + j) : T(0);
         }
-        uint16_t p[3][8];
+        constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+        uint16_t p[kParts][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) split3(v[j], p[0][j], p[1][j], p[2][j]);
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (kParts == 3) split3(v[j], p[0][j], p[1][j], p[2][j]);
+            else p[0][j] = v[j];
+        }
 #pragma unroll
-        for (int q = 0; q < 3; ++q)
-            *reinterpret_cast<uint4*>(parts + (m * 3 + q) * ldp + k) =
+        for (int q = 0; q < kParts; ++q)
+            *reinterpret_cast<uint4*>(to + (m * kParts + q) * ldp + k) =
                 make_uint4(p[q][0] | (uint32_t)p[q][1] << 16, p[q][2] | (uint32_t)p[q][3] << 16,
                            p[q][4] | (uint32_t)p[q][5] << 16, p[q][6] | (uint32_t)p[q][7] << 16);
     }
 }
 
-cudaError_t launch_split_rows(const float* x, long long ldx, int M, int K, void* parts, cudaStream_t st) {
+template <class T>
+cudaError_t launch_rows_t(const void* x, long long ldx, int M, int K, void* to, cudaStream_t st) {
     const int ldp = (K + 7) / 8 * 8;
-    const long long units = (long long)M * (ldp / 8), blocks = (units + 255) / 256;
+    const long long blocks = ((long long)M * (ldp / 8) + 255) / 256;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)std::min(blocks, 8ll * kSms));
     cfg.blockDim = dim3(256);
@@ -553,7 +547,11 @@ cudaError_t launch_split_rows(const float* x, long long ldx, int M, int K, void*
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return counted(cudaLaunchKernelEx(&cfg, split_rows_kernel, x, ldx, M, K, static_cast<uint16_t*>(parts), ldp));
+    return counted(cudaLaunchKernelEx(&cfg, rows_kernel<T>, static_cast<const T*>(x), ldx, M, K, static_cast<uint16_t*>(to), ldp));
+}
+
+cudaError_t launch_rows(bool f32, const void* x, long long ldx, int M, int K, void* to, cudaStream_t st) {
+    return f32 ? launch_rows_t<float>(x, ldx, M, K, to, st) : launch_rows_t<uint16_t>(x, ldx, M, K, to, st);
 }
 
 cudaError_t step_status(int* status) {

@@ -561,12 +561,13 @@ def test_no_rows_need_no_device(kv):
 
 def test_work_bytes(kv):
     n = C.c_size_t()
-    for m, k, dtype, some in ((1, 100, 2, False), (300, 100, 2, True), (300, 100, 0, False), (300, 101, 1, False)):
-        kv.call("w4_work_bytes", 64, k, dtype, m, 0, C.byref(n))
-        assert n.value == (3 * m * -(-k // 8) * 16 if some else 0)
-    refused(kv, "w4_work_bytes", 64, 64, 5, 1, 0, C.byref(n))
-    refused(kv, "w4_work_bytes", 64, 64, 2, -1, 0, C.byref(n))
-    refused(kv, "w4_work_bytes", 64, 64, 2, 1, 0, None)
+    for m, k, dtype, some in ((1, 100, 2, False), (300, 100, 2, True), (300, 100, 0, True), (300, 101, 1, True), (1, 9000, 1, False)):
+        kv.call("w4_work_bytes", 64, k, 64, dtype, m, 0, C.byref(n))
+        assert n.value == ((3 if dtype == 2 else 1) * m * -(-k // 8) * 16 if some else 0)
+    refused(kv, "w4_work_bytes", 64, 64, 64, 5, 1, 0, C.byref(n))
+    refused(kv, "w4_work_bytes", 64, 64, 65, 2, 1, 0, C.byref(n))
+    refused(kv, "w4_work_bytes", 64, 64, 64, 2, -1, 0, C.byref(n))
+    refused(kv, "w4_work_bytes", 64, 64, 64, 2, 1, 0, None)
 
 
 def test_w4_sizes(kv):
