@@ -109,11 +109,10 @@ class _LogitsCall(C.Structure):
                 ("bias_n", C.c_longlong), ("mask", _vp), ("ld_mask", C.c_longlong)]
 
 
-_w4p = C.POINTER(_W4Matrix)
 _SIGS.update({
     "w4_sizes": [C.c_int, C.c_int, C.c_int] + [C.POINTER(C.c_size_t)] * 3,
-    "w4_quantize": [_w4p, _vp, C.c_int, C.c_longlong, _vp],
-    "w4_dequantize": [_w4p, _vp, C.c_longlong, _vp],
+    "w4_quantize": [_vp, _vp, C.c_int, C.c_longlong, _vp],
+    "w4_dequantize": [_vp, _vp, C.c_longlong, _vp],
     "w4_linear": [_vp, _vp, C.c_int, C.c_int, C.c_longlong, _vp, _vp, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp, _vp],
     "w4_gated": [_vp, _vp, _vp, C.c_int, C.c_int, C.c_longlong, _vp, C.c_int, C.c_longlong, _vp, _vp],
     "w4_work_bytes": [C.c_int] * 6 + [C.POINTER(C.c_size_t)],
@@ -461,18 +460,32 @@ def _words(t, device: int, what: str, dtype, n=None):
     """The address of a contiguous 1-D device tensor of 4-byte values (None: NULL)."""
     if t is None:
         return None
-    if t.dtype != dtype or t.get_device() != device or t.dim() != 1 or not t.is_contiguous():
+    shape = t.shape
+    if t.dtype is not dtype or t.get_device() != device or len(shape) != 1 or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous 1-D {dtype} tensor on cuda:{device} is expected")
-    if n is not None and t.shape[0] != n:
-        raise ValueError(f"{what}: {t.shape[0]} values, expected {n}")
+    if n is not None and shape[0] != n:
+        raise ValueError(f"{what}: {shape[0]} values, expected {n}")
     return t.data_ptr()
 
 
+_raw_stream = None  # device index -> address of torch's current stream
+
+
 def _stream_on(stream, device: int):
+    global _raw_stream
     if stream is None:
-        import torch
-        return torch.cuda.current_stream(device).cuda_stream
+        if _raw_stream is None:
+            import torch
+            # the plain address where torch has it, without a Stream object around it
+            _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+                (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        return _raw_stream(device)
     return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _stream_object(stream, device):
+    import torch
+    return torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
 
 
 def _scratch(w, x, dtype: int, m: int, ldx: int, gated: int, stream):
@@ -487,7 +500,7 @@ def _scratch(w, x, dtype: int, m: int, ldx: int, gated: int, stream):
     import torch
     t = torch.empty(n.value, dtype=torch.uint8, device=x.device)
     if stream is not None:
-        t.record_stream(torch.cuda.ExternalStream(stream, device=x.device) if isinstance(stream, int) else stream)
+        t.record_stream(_stream_object(stream, x.device))
     return t
 
 
@@ -511,6 +524,9 @@ class W4:
                 continue
             if t.dtype != dtype or t.get_device() != dev or not t.is_contiguous() or t.nbytes != size.value:
                 raise ValueError(f"{what}: {size.value} contiguous bytes of {dtype} on cuda:{dev} are expected")
+        self._hold(codes, scales, zeros, n, k, group, dev)
+
+    def _hold(self, codes, scales, zeros, n, k, group, dev) -> None:
         self.codes, self.scales, self.zeros = codes, scales, zeros
         self.n, self.k, self.group, self.device = n, k, group, dev
         self._c = _W4Matrix(dev, n, k, group, codes.data_ptr(), scales.data_ptr(),
@@ -522,10 +538,12 @@ class W4:
         import torch
         if out is None:
             out = torch.empty(self.n, self.k, dtype=torch.float32, device=self.codes.device)
+            if stream is not None:
+                out.record_stream(_stream_object(stream, out.device))
         elif out.dtype != torch.float32:
             raise ValueError("out: fp32 is expected")
         ld = _rows(out, self.device, "out", self.n, self.k)
-        call("w4_dequantize", C.byref(self._c), out.data_ptr(), ld, _stream_on(stream, self.device))
+        call("w4_dequantize", self._at, out.data_ptr(), ld, _stream_on(stream, self.device))
         return out
 
 
@@ -536,11 +554,20 @@ def w4_quantize(w, group: int = 128, zero_points: bool = False, stream=None) -> 
     if not (n > 0 and k > 0 and group in (32, 64, 128)):
         raise ValueError(f"a 4-bit matrix of {n} x {k} in groups of {group}: groups of 32, 64 or 128 are supported")
     T, S, Q = (n + 15) // 16, (k + 127) // 128, (k + group - 1) // group
-    m = W4(torch.empty((T, S, 2, 32, 4), dtype=torch.int32, device=w.device),
-           torch.empty((T, Q, 8, 2), dtype=torch.float16, device=w.device),
-           torch.empty((T, Q, 8, 2), dtype=torch.uint8, device=w.device) if zero_points else None, n, k, group)
+    dev, dtype = w.device, _step_dtype(w, "w")
+    if dev.type != "cuda":
+        raise ValueError("w: a device tensor is expected")
+    load()
+    m = W4.__new__(W4)
+    m._hold(torch.empty((T, S, 2, 32, 4), dtype=torch.int32, device=dev),
+            torch.empty((T, Q, 8, 2), dtype=torch.float16, device=dev),
+            torch.empty((T, Q, 8, 2), dtype=torch.uint8, device=dev) if zero_points else None, n, k, group, dev.index)
     ld = _rows(w, m.device, "w")
-    call("w4_quantize", C.byref(m._c), w.data_ptr(), _step_dtype(w, "w"), ld, _stream_on(stream, m.device))
+    call("w4_quantize", m._at, w.data_ptr(), dtype, ld, _stream_on(stream, m.device))
+    if stream is not None:  # the arrays were allocated for the current stream
+        for t in (m.codes, m.scales, m.zeros):
+            if t is not None:
+                t.record_stream(_stream_object(stream, dev))
     return m
 
 

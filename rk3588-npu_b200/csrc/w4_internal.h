@@ -20,6 +20,12 @@ enum { W4_X_16 = 0, W4_X_F32 = 1, W4_X_ROUND = 2, W4_X_NORM = 3 };
 // Epilogues: the model's call sites (GemvArgs) and the public operators.
 enum { W4_QKV = 0, W4_RESID = 1, W4_GATE_UP = 2, W4_LOGITS = 3, W4_LINEAR = 4, W4_GATED = 5 };
 
+// Spans that a warp copies at a time, and how many such batches it has
+// room for.  Measured, us with 4 x 2 / 2 x 4: 151936 x 1536, one row 29.5 / 33.2 (fewer, larger
+// batches pay for less pointer arithmetic); two matrices with 2 x 2 / 1 x 4: 8960 x 1536 in
+// groups of 32, 8 rows 9.9 / 8.9.
+constexpr int w4_batch(int nw) { return nw == 2 ? 1 : 4; }
+constexpr int w4_ring(int nw) { return nw == 2 ? 4 : 2; }
 struct W4Args {
     const uint32_t* codes[2] = {};
     const __half* scales[2] = {};
@@ -42,7 +48,7 @@ struct W4Args {
     int rows = 0;             // x rows per pass
     int ks = 1, cs = 1;       // a tile's spans over ks warps and cs CTAs
     int chunk = 0;            // spans of x staged at a time
-    int batches = 2;          // of codes per warp in shared memory
+    int batches = 2;    // of codes per warp in shared memory
     int last_groups = 0;      // groups of a row's last span
     bool early = false;       // the weights may be read before the previous kernel of the stream ends
 
@@ -60,8 +66,6 @@ struct W4Args {
 
 constexpr int kSms = 148;
 constexpr int kW4MaxSmem = 227 * 1024;
-// Spans that a warp copies at a time (two such batches in shared memory).
-constexpr int w4_batch(int nw) { return nw == 2 ? 2 : 4; }
 // Floats of a warp's partial tile: 20 per column (16 rows, padded against bank
 // conflicts), 4 more so that the warps' tiles start in different banks.
 constexpr int w4_red_floats(int nw, int nt) { return nw * nt * 8 * 20 + 4; }
@@ -85,7 +89,7 @@ inline W4Plan w4_plan(int M, int T, int S, int pieces, int nw, int sms) {
     const int passes = (M + most - 1) / most, rows = (M + passes - 1) / passes, vr = rows * pieces;
     const int nt = vr <= 8 ? 1 : vr <= 16 ? 2 : 4;
     const int unit = w4_batch(nw), batch = unit * nw * 1216, red = 8 * w4_red_floats(nw, nt) * 4;
-    const int fit = ((kW4MaxSmem - red - 8 * 2 * batch) / (vr * 2) - 32) / 128;  // spans of x that fit at once
+    const int fit = ((kW4MaxSmem - red - 8 * w4_ring(nw) * batch) / (vr * 2) - 32) / 128;  // spans of x that fit at once
     double least = 0;
     for (int ks = 1; ks <= 8 && ks <= S; ks *= 2) {
         W4Plan p{nt, rows, passes, ks, 1};
@@ -97,16 +101,16 @@ inline W4Plan w4_plan(int M, int T, int S, int pieces, int nw, int sms) {
         // all of the CTA's spans, or as many batches of its warps as fit
         p.chunk = spans <= fit ? spans : fit / (ks * unit) * (ks * unit);
         const int fixed = red + vr * (p.chunk * 128 + 32) * 2;
+        const int own = (per_warp + unit - 1) / unit;  // a tile's batches: no more room than that where there is one tile
         double turns = 0;
-        for (p.batches = 1; p.batches <= 2; ++p.batches) {  // one batch of codes is enough for one tile of so many spans
+        for (p.batches = std::min(own, w4_ring(nw));; p.batches = w4_ring(nw)) {
             p.smem = fixed + 8 * p.batches * batch;
             const int per_sm = p.smem <= 113 * 1024 && nt * nw <= 2 ? 2 : 1;
             const int slots = std::max(1, sms * per_sm / (passes * p.cs));
             p.gx = std::min(groups, slots);
             turns = (double)groups / slots;
-            if (turns <= 1 && per_warp <= unit) break;
+            if (turns <= 1 || p.batches == w4_ring(nw)) break;
         }
-        p.batches = std::min(p.batches, 2);
         const double whole = (double)(long long)turns, part = turns - whole;
         const double cost = std::max(1.0, whole + (part > 0 ? 0.5 + 0.5 * part : 0)) * (per_warp + 2);
         if (least == 0 || cost < least) least = cost, best = p;

@@ -20,7 +20,7 @@
 //
 // Bound: the codes' bytes for few rows.  Each lane copies the 32 bytes of
 // codes that it will unpack itself to its own slots of a ring in shared memory
-// (cp.async, a batch of spans ahead, across tiles), so loads never wait for the
+// (cp.async, batches of spans ahead, across tiles), so loads never wait for the
 // math and need no barrier; a warp's 16 rows x 128 inputs are one contiguous
 // KiB in memory.
 #include <cuda_bf16.h>
@@ -170,8 +170,9 @@ __device__ __forceinline__ void stage_rows(const W4Args& a, int m0, int mrows, i
 template <int BF, int NT, int NW, int GP>
 __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     w4_kernel(const __grid_constant__ W4Args a) {
-    constexpr int kU = w4_batch(NW);        // spans per batch
-    constexpr int kBatch = kU * NW * kSlot;     // bytes; two batches per warp, one in flight, one in use (or one is all)
+    constexpr int kRing = w4_ring(NW);
+    constexpr int kU = w4_batch(NW);         // spans per batch
+    constexpr int kBatch = kU * NW * kSlot;  // bytes; kRing batches per warp, one in use, the others in flight
     constexpr int kCols = NT * 8;
     constexpr int kRedWarp = w4_red_floats(NW, NT);
     extern __shared__ __align__(16) uint8_t smem[];
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
     const int nmine = s0 + part < s1 ? (s1 - s0 - part + ks - 1) / ks : 0;  // this warp's
     const int tile0 = sub * gx + bx, tstep = tpc * gx;
 
-    // The warp's (tile, span) sequence, a batch ahead of the math: pointers that
+    // The warp's (tile, span) sequence, kRing - 1 batches ahead of the math: pointers that
     // advance by constants; a batch ends with its tile.
     int ptiles = nmine > 0 && tile0 < a.T ? (a.T - tile0 + tstep - 1) / tstep : 0, pleft = nmine;
     int pgroup = (s0 + part) * GP;  // the next span's first group
@@ -240,14 +241,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
             }
         }
         cp_commit();
-        poff ^= kBatch;
+        poff = poff == (kRing - 1) * kBatch ? 0 : poff + kBatch;
     };
 
     // In the model's chain (a.early) the weights, which no kernel of the chain
     // writes, are fetched before the wait for the previous kernel.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (!a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
-    issue();
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) issue();
     if (a.early) asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const bool wide = (reinterpret_cast<size_t>(a.x) & 15) == 0 && (a.ldx * (a.in == W4_X_16 ? 2 : 4)) % 16 == 0;
@@ -291,7 +293,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
                 xp = xs + part * 128 + 8 * c;
             }
             if (it >= nmine || !live) continue;
-            cp_wait<0>();
+            cp_wait<kRing - 2>();
             __syncwarp();  // scales came by other lanes; the batch refilled next was read by all of them
             issue();
 #pragma unroll
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
             xp += ks * 128;
             left -= ks;
             }
-            slot ^= kBatch;
+            slot = slot == (kRing - 1) * kBatch ? 0 : slot + kBatch;
         }
         // partial tiles of this warp: [matrix][column][row]
         if (live) {

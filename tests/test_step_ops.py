@@ -545,7 +545,7 @@ def test_linear_refusals(kv):
     g = dict(gate=matrix(kv), up=matrix(kv), x=A, xd=0, m=4, ldx=64, out=B, od=2, ldo=32, work=None)
     for up in (None, matrix(kv, n=33), matrix(kv, k=65), matrix(kv, group=64), matrix(kv, device=1), matrix(kv, zeros=0x1000)):
         refused(kv, "w4_gated", *{**g, "up": up}.values(), None)
-    m = C.byref(_matrices[0])
+    m = C.addressof(_matrices[0])
     refused(kv, "w4_quantize", m, A, 2, 64, None)
     refused(kv, "w4_quantize", m, A, 0, 63, None)
     refused(kv, "w4_quantize", m, A + 1, 0, 64, None)
