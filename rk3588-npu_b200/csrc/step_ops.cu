@@ -27,7 +27,8 @@ int sfail(int status, const char* fmt, ...) {
         if (s_ != KV_OK) return s_; \
     } while (0)
 
-constexpr int kMaxDim = 1 << 30;  // rows, inputs, tokens of one call
+constexpr int kMaxDim = 1 << 30;   // outputs, inputs, tokens of one call
+constexpr int kMaxRows = 1 << 19;  // rows of x of one call: 65535 passes of 10 hold them
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<size_t>(p) & (n - 1)) == 0; }
 size_t esize(int dtype) { return dtype == STEP_F32 ? 4 : 2; }
@@ -75,7 +76,7 @@ int check_rows(const w4_matrix& w, const void* x, int x_dtype, int m, long long 
     if (!x || !out) return sfail(KV_ERR_INVAL, "NULL x or out");
     if (!aligned(x, esize(x_dtype)) || !aligned(out, esize(out_dtype)))
         return sfail(KV_ERR_INVAL, "x or out is not aligned to its element");
-    if (m > 1 << 20) return sfail(KV_ERR_RANGE, "%d rows in one call (at most %d)", m, 1 << 20);
+    if (m > kMaxRows) return sfail(KV_ERR_RANGE, "%d rows in one call (at most %d)", m, kMaxRows);
     if (Range(x, m, w.k, ldx, esize(x_dtype)).meets(Range(out, m, w.n, ldo, esize(out_dtype))))
         return sfail(KV_ERR_INVAL, "out overlaps x");
     return KV_OK;
@@ -199,7 +200,7 @@ int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dt
 int w4_work_bytes(int n, int k, int group, int x_dtype, int m, int gated, size_t* bytes) {
     ST_OK(check_shape(n, k, group));
     ST_OK(check_dtype(x_dtype, "x"));
-    if (m < 0 || m > 1 << 20 || !bytes) return sfail(KV_ERR_INVAL, "%d rows, or NULL bytes", m);
+    if (m < 0 || m > kMaxRows || !bytes) return sfail(KV_ERR_INVAL, "%d rows, or NULL bytes", m);
     *bytes = work_bytes(n, k, group, x_dtype, m, gated);
     return KV_OK;
 }

@@ -153,7 +153,9 @@ inline bool w4_use_tc(int M, int T, int S, int pieces, int nw, int group) {
     return rows > (nw == 2 && tiles <= kSms && group > 32 ? 20 : 40);
 }
 // Rows of 16-bit values that a tensor map can describe.
-inline bool w4_tma_rows(const void* x, long long ldx) { return reinterpret_cast<size_t>(x) % 16 == 0 && ldx % 8 == 0; }
+inline bool w4_tma_rows(const void* x, long long ldx) {
+    return reinterpret_cast<size_t>(x) % 16 == 0 && ldx % 8 == 0 && ldx < 1ll << 38;
+}
 
 cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st);
 // Rows of x made for the tcgen05 form: an fp32 row's three bf16 parts, or a 16-bit row

@@ -102,6 +102,15 @@ LINEAR = [
     (1, 20000, 640, 128, True, "f16", "f32"),
     (4, 64, 40000, 128, False, "f32", "f32"),
     (60, 32, 30000, 64, True, "bf16", "f32"),
+    # many rows: short and unaligned ones, columns that fill a tile and one more, several tiles, fp32 in parts
+    (100, 20, 1, 32, True, "f16", "f32"),
+    (200, 64, 8, 128, False, "bf16", "f16"),
+    (90, 33, 40, 32, True, "f32", "f32"),
+    (128, 1153, 264, 64, False, "f16", "f32"),
+    (129, 129, 4100, 128, True, "bf16", "bf16"),
+    (256, 16, 127, 32, False, "f16", "f16"),
+    (600, 272, 1537, 64, True, "f32", "bf16"),
+    (41, 20000, 200, 128, False, "f16", "f16"),
 ]
 
 
@@ -138,6 +147,9 @@ GATED = [
     (33, 48, 300, 128, False, "bf16", "f32"),
     (100, 130, 640, 64, False, "f16", "f16"),
     (300, 96, 520, 128, True, "bf16", "bf16"),
+    (70, 65, 2000, 32, True, "f32", "f32"),
+    (257, 700, 129, 64, False, "f16", "f32"),
+    (86, 1, 300, 128, True, "f32", "f16"),
 ]
 
 
@@ -192,6 +204,23 @@ def test_linear_strided_rows(kv, xd, yd, offset):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("xd", ["f16", "f32"])
+def test_linear_many_rows_without_scratch(kv, xd):
+    """A C caller without scratch: rows that would go through it take the other form."""
+    need_gpu()
+    rng = np.random.default_rng(77)
+    m, n, k = 100, 60, 333
+    w, ref = random_matrix(kv, rng, n, k, 64, True)
+    x = fill(rng, (m, k), xd)
+    out = torch.empty(m, n, device="cuda")
+    kv.call("w4_linear", w._at, x.data_ptr(), kv.STEP_F32 if xd == "f32" else kv.STEP_F16, m, k, None, None, 0, out.data_ptr(),
+            kv.STEP_F32, n, None, torch.cuda.current_stream().cuda_stream)
+    want = dbl(x) @ ref.T
+    tol = sum_tol(dbl(x), ref, 64) + 2.0**-23 * np.abs(want)
+    assert np.all(np.abs(dbl(out) - want) <= tol)
+
+
+@pytest.mark.gpu
 def test_linear_no_rows_and_non_finite(kv):
     need_gpu()
     rng = np.random.default_rng(8)
@@ -228,14 +257,26 @@ def test_linear_repeats_on_streams_and_in_graphs(kv):
     kv.w4_linear(w, x, b, stream=s)
     torch.cuda.synchronize()
     assert torch.equal(a, b)
+    # many fp32 rows, through scratch, on both streams at once
+    y = fill(rng, (64, 8960), "f32")
+    one, two = torch.empty(64, 1536, device="cuda"), torch.empty(64, 1536, device="cuda")
+    s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        kv.w4_linear(w, y, one)
+        kv.w4_linear(w, y, two, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(one, two)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         kv.w4_linear(w, x, c)
         kv.w4_gated(w, w, x, b)
+        kv.w4_linear(w, y, two)
+        kv.logits_adjust(two, two, frequency=torch.ones(64, device="cuda"))
     x.mul_(2)
+    y.mul_(2)
     graph.replay()
     torch.cuda.synchronize()
-    assert torch.equal(c, 2 * a)  # every step scales exactly by 2
+    assert torch.equal(c, 2 * a) and torch.equal(two, 2 * one)  # every step scales exactly by 2
 
 
 # ------------------------------------------------------------------- quantise
@@ -320,6 +361,9 @@ LOGITS = [
     (1, 128257, "bf16", 20000, 300, True),
     (3, 200001, "f16", 10, 0, False),
     (70, 257, "f32", 33, 5, True),
+    (18, 160001, "bf16", 50, 3, True),   # more tokens than a CTA notes at a time
+    (1, 320000, "f32", 2000, 10, True),
+    (2, 300, "f32", 7, 40000, False),    # more bias entries than 16 bits number
 ]
 
 
