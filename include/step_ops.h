@@ -47,8 +47,7 @@ enum { STEP_F16 = 0, STEP_BF16 = 1, STEP_F32 = 2 };
  *   scales  fp16 [T][Q][8][2]: element [t][q][g][h] is row 16 t + 8 h + g;
  *   zeros   uint8, the same shape, or NULL.
  * Codes and scales of the last tile's and span's padding have to be there
- * (they are read) and may hold anything.  codes are 16-byte aligned, scales
- * and zeros 4-byte aligned. */
+ * (they are read) and may hold anything.  All three are 16-byte aligned. */
 typedef struct w4_matrix {
     int device;
     int n, k, group;

@@ -45,8 +45,8 @@ int check_matrix(const w4_matrix* m, const char* what) {
     ST_OK(check_shape(m->n, m->k, m->group));
     if (m->device < 0) return sfail(KV_ERR_INVAL, "%s: no device", what);
     if (!m->codes || !m->scales) return sfail(KV_ERR_INVAL, "%s: NULL codes or scales", what);
-    if (!aligned(m->codes, 16) || !aligned(m->scales, 4) || !aligned(m->zeros, 4))
-        return sfail(KV_ERR_INVAL, "%s: codes need 16-byte, scales and zero points 4-byte alignment", what);
+    if (!aligned(m->codes, 16) || !aligned(m->scales, 16) || !aligned(m->zeros, 16))
+        return sfail(KV_ERR_INVAL, "%s: codes, scales and zero points need 16-byte alignment", what);
     return KV_OK;
 }
 

@@ -488,48 +488,77 @@ __global__ void __launch_bounds__(256)
         }
     }
     const int gi = s * (32 / GL) + lane / GL;
+    // The 16 rows' extremes over the GL lanes of a group together: at each step a
+    // lane hands half of its rows to its partner and takes the partner's other
+    // half, so each lane ends with kRows rows' (16 / GL, or one) and makes their
+    // scales, which come back by shuffles: no lane repeats another's division.
+    constexpr int kRows = GL >= 16 ? 1 : 16 / GL;
+    const int li = lane % GL;
+    auto reduce = [&](float (&x)[16]) {
+#pragma unroll
+        for (int o = 1, n = 8; o < GL; o <<= 1, n >>= 1) {
+            if (n >= 1) {
+                const bool up = li & o;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < n) {
+                        const float mine = up ? x[r + n] : x[r], other = up ? x[r] : x[r + n];
+                        x[r] = fmaxf(mine, __shfl_xor_sync(0xffffffffu, other, o));
+                    }
+            } else {
+                x[0] = fmaxf(x[0], __shfl_xor_sync(0xffffffffu, x[0], o));
+            }
+        }
+    };
+    float top[16], neg[16];  // max w (max |w| without zero points), max -w
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const float f0 = to_f(v[r].e[0]), f1 = to_f(v[r].e[1]), f2 = to_f(v[r].e[2]), f3 = to_f(v[r].e[3]);
+        if (ZP) {
+            top[r] = fmaxf(fmaxf(fmaxf(f0, f1), fmaxf(f2, f3)), 0.f);
+            neg[r] = fmaxf(-fminf(fminf(f0, f1), fminf(f2, f3)), 0.f);
+        } else {
+            top[r] = fmaxf(fmaxf(fabsf(f0), fabsf(f1)), fmaxf(fabsf(f2), fabsf(f3)));
+        }
+    }
+    reduce(top);
+    if (ZP) reduce(neg);
+    // this lane's rows: bit i of li decided bit 3 - i of the row
+    const int row0 = (li & 1) << 3 | (li & 2) << 1 | (GL > 4 ? (li & 4) >> 1 : 0) | (GL > 8 ? (li & 8) >> 3 : 0);
+    float sc[kRows], inv[kRows];
+    int zi[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        const __half sh = __float2half_rn(ZP ? __fdiv_rn(__fadd_rn(top[r], neg[r]), 15.0f) : __fdiv_rn(top[r], 7.0f));
+        sc[r] = __half2float(sh);
+        zi[r] = ZP && sc[r] > 0.f ? (int)fminf(fmaxf(rintf(__fdiv_rn(neg[r], sc[r])), 0.f), 15.f) : 8;
+        inv[r] = sc[r] > 0.f ? __frcp_rn(sc[r]) : 0.f;  // no scale: every code is the zero point
+        const int row = row0 + r, h = row >> 3, g = row & 7;
+        if (gi < Q && li < 16) {
+            const size_t at = ((size_t)t * Q + gi) * 16 + g * 2 + h;
+            scales[at] = sh;
+            if (ZP) zeros[at] = (uint8_t)zi[r];
+        }
+    }
     uint32_t* word = codes + ((size_t)t * S + s) * 256 + ((lane >> 1) & 3) * 4 + (lane >> 3);  // + [h][4 g][.]
-    const size_t note = ((size_t)t * Q + gi) * 16;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         const int h = r >> 3, g = r & 7;
-        float f[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = to_f(v[r].e[i]);
-        float sc, z = 8.f;
-        __half sh;
-        if (ZP) {
-            float lo = fminf(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), 0.f);
-            float hi = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), 0.f);
-#pragma unroll
-            for (int o = 1; o < GL; o <<= 1) {
-                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            }
-            sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
-            sc = __half2float(sh);
-            if (sc > 0.f) z = fminf(fmaxf(rintf(__fdiv_rn(-lo, sc)), 0.f), 15.f);
-        } else {
-            float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
-#pragma unroll
-            for (int o = 1; o < GL; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            sh = __float2half_rn(__fdiv_rn(top, 7.0f));
-            sc = __half2float(sh);
-        }
-        const float inv = sc > 0.f ? __frcp_rn(sc) : 0.f;  // no scale: every code is the zero point
-        const int zi = (int)z;
+        // the lane of the group that has row r
+        const int from = lane - li + ((r >> 3 & 1) | (r >> 2 & 1) << 1 | (GL > 4 ? (r >> 1 & 1) << 2 : 0) | (GL > 8 ? (r & 1) << 3 : 0));
+        const float s_r = __shfl_sync(0xffffffffu, sc[r % kRows], from), i_r = __shfl_sync(0xffffffffu, inv[r % kRows], from);
+        const int z_r = ZP ? __shfl_sync(0xffffffffu, zi[r % kRows], from) : 8;
         uint32_t q[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = (uint32_t)min(max(round_quotient(sc > 0.f ? f[i] : 0.f, sc, inv) + zi, 0), 15);
+        for (int i = 0; i < 4; ++i) {
+            const float f = i_r > 0.f ? to_f(v[r].e[i]) : 0.f;
+            q[i] = (uint32_t)min(max(round_quotient(f, s_r, i_r) + z_r, 0), 15);
+        }
         // inputs 0..3 of a word stand at 0, 4, 1, 5 (times four bits), 4..7 at 2, 6, 3, 7
         uint32_t part = q[0] | q[1] << 16 | q[2] << 4 | q[3] << 20;
         part = (lane & 1) ? part << 8 : part;
         part |= __shfl_xor_sync(0xffffffffu, part, 1);
         if (!(lane & 1)) word[h * 128 + g * 16] = part;
-        if (lane % GL == 0 && gi < Q) {
-            scales[note + g * 2 + h] = sh;
-            if (ZP) zeros[note + g * 2 + h] = (uint8_t)zi;
-        }
     }
 }
 
@@ -546,37 +575,50 @@ __global__ void __launch_bounds__(256)
     if (s >= S) return;
     const uint32_t* span = codes + ((size_t)t * S + s) * 256;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll 4
-        for (int g = 0; g < 8; ++g) {
-            const int n = t * 16 + h * 8 + g;
-            if (n >= N) break;
+    for (int b = 0; b < kB; ++b) {
+        const int kk = b * 32 * kE + lane * kE, k = s * 128 + kk;  // inside the span, inside the row
+        if (k >= K) continue;
+        // the group's scales and zero points of all 16 rows
+        const size_t at = ((size_t)t * Q + (k >> lg)) * 16;
+        union {
+            uint4 u[2];
+            __half h[16];
+        } sc;
+        sc.u[0] = __ldg(reinterpret_cast<const uint4*>(scales + at));
+        sc.u[1] = __ldg(reinterpret_cast<const uint4*>(scales + at) + 1);
+        union {
+            uint4 u;
+            uint8_t b[16];
+        } z;
+        z.u = make_uint4(0x08080808u, 0x08080808u, 0x08080808u, 0x08080808u);
+        if (zeros) z.u = __ldg(reinterpret_cast<const uint4*>(zeros + at));
+        const uint32_t* word = span + ((kk >> 3) & 3) * 4 + (kk >> 5);
+        float* to = out + (size_t)t * 16 * ldo + k;
 #pragma unroll
-            for (int b = 0; b < kB; ++b) {
-                const int kk = b * 32 * kE + lane * kE, k = s * 128 + kk;  // inside the span, inside the row
-                if (k >= K) continue;
-                const uint32_t w = __ldg(span + h * 128 + (g * 4 + ((kk >> 3) & 3)) * 4 + (kk >> 5));
-                const size_t at = ((size_t)t * Q + (k >> lg)) * 16 + g * 2 + h;
-                const float sc = __half2float(scales[at]), z = zeros ? (float)(zeros[at] & 15) : 8.f;
-                union {
-                    U u;
-                    float f[kE];
-                } v;
+        for (int r = 0; r < 16; ++r) {
+            if (t * 16 + r >= N) break;
+            const int h = r >> 3, g = r & 7;
+            const uint32_t w = __ldg(word + h * 128 + g * 16);
+            const float s_r = __half2float(sc.h[g * 2 + h]), z_r = 8388608.f + (float)(z.b[g * 2 + h] & 15);
+            union {
+                U u;
+                float f[kE];
+            } v;
 #pragma unroll
-                for (int i = 0; i < kE; ++i) {
-                    const int ii = (kk & 7) + i;
-                    v.f[i] = ((float)((w >> (4 * ((ii >> 1) + 4 * (ii & 1)))) & 15u) - z) * sc;
-                }
-                float* to = out + (size_t)n * ldo + k;
-                if (k + kE <= K) {
-                    *reinterpret_cast<U*>(to) = v.u;
-                } else {
+            for (int i = 0; i < kE; ++i) {
+                const int ii = (kk & 7) + i;
+                // 2^23 + code, exactly, then the code less its zero point
+                v.f[i] = (__uint_as_float((w >> (4 * ((ii >> 1) + 4 * (ii & 1)))) & 15u | 0x4B000000u) - z_r) * s_r;
+            }
+            if (k + kE <= K) {
+                *reinterpret_cast<U*>(to + (size_t)r * ldo) = v.u;
+            } else {
 #pragma unroll
-                    for (int i = 0; i < kE; ++i)
-                        if (k + i < K) to[i] = v.f[i];
-                }
+                for (int i = 0; i < kE; ++i)
+                    if (k + i < K) to[(size_t)r * ldo + i] = v.f[i];
             }
         }
+    }
 }
 
 // ------------------------------------------------------------------ launching
