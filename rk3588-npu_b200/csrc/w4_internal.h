@@ -141,16 +141,17 @@ inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw) {
 }
 
 // Rows from which the tcgen05 form is the faster one: its tiles cost the same
-// for one row as for 64, more with small groups (each is read and scaled by
+// for one row as for 64, somewhat more with small groups (each is scaled by
 // itself), and the other form suffers from long rows, of which it keeps every
 // staged x.  Measured, us (w4_kernels.cu / tcgen05): 1536 x 8960, 16 rows 18 / 12,
-// 12 rows 12.2 / 12.3; 2048 x 1536, 48 rows 11.1 / 10.5, 32 rows 6.3 / 9.9; 8960 x 1536
-// gated, 24 rows 15.9 / 13.7, 16 rows 11.4 / 14; the same in groups of 32, 48 rows
-// 30.5 / 24, 32 rows 20.7 / 23.5; 151936 x 1536, 48 rows 158 / 129, 32 rows 103 / 137.
+// 8 rows 7.8 / 12; 2048 x 1536, 48 rows 11.1 / 10.5, 32 rows 6.3 / 9.7; 8960 x 1536
+// gated, 24 rows 15.9 / 13.4, 16 rows 10.6 / 13.3; the same in groups of 32, 48 rows
+// 30.5 / 19.5, 32 rows 18.9 / 19.3; 151936 x 1536, 48 rows 158 / 127, 32 rows 96 / 125.
 inline bool w4_use_tc(int M, int T, int S, int pieces, int nw, int group) {
     const int tiles = (T + 7) / 8 * nw, rows = M * pieces;
-    if (tiles <= kSms && S >= 32) return rows > (group == 32 ? 24 : 8);
-    return rows > (nw == 2 && tiles <= kSms && group > 32 ? 20 : 40);
+    if (tiles <= kSms && S >= 32) return rows > (group == 32 ? 10 : 8);
+    if (tiles <= kSms && nw == 2) return rows > (group == 32 ? 32 : 20);
+    return rows > 40;
 }
 // Rows of 16-bit values that a tensor map can describe.
 inline bool w4_tma_rows(const void* x, long long ldx) {

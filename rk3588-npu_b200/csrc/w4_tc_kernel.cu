@@ -10,7 +10,7 @@
 //   warp 4      brings the B operand: NB rows of x x 128 inputs, the same
 //               layout, by TMA, which fills what lies outside x with zeros;
 //   warp 7      issues the MMAs: each group of inputs into a fresh sum in
-//               tensor memory, two of them in turn;
+//               tensor memory, two or four of them in turn;
 //   warps 8-15  read a finished group (lane = weight row) and add it, times
 //               the row's scale, to fp32 sums in registers, while the next
 //               group is multiplied.
@@ -45,6 +45,12 @@ namespace {
 constexpr int kStagesA = 2;   // written from registers, so little waits in them
 template <int NB>
 constexpr int kStagesB = NB == 256 ? 2 : 4;  // copies in flight
+// Sums in tensor memory: groups that are committed and read together (a unit: the
+// round trip between the MMAs and the reading is paid once for it), and units.
+template <int NB, int GP>
+constexpr int kUnit = GP < 256 / NB ? GP : 256 / NB;
+template <int NB, int GP>
+constexpr int kUnits = 512 / (kUnit<NB, GP> * NB) < 4 ? 512 / (kUnit<NB, GP> * NB) : 4;
 constexpr int kAhead = 3;     // spans of codes in shared memory, per unpacking warp
 constexpr int kCodes = 2 * 1024 + 128;  // a span of a warp's two tiles, and their zero points
 constexpr int kThreads = 16 * 32;
@@ -63,7 +69,7 @@ struct Smem {
 };
 
 struct Bars {
-    uint64_t full_a[kStagesA], empty_a[kStagesA], full_b[4], empty_b[4], sum_full[2], sum_empty[2];
+    uint64_t full_a[kStagesA], empty_a[kStagesA], full_b[4], empty_b[4], sum_full[4], sum_empty[4];
     uint32_t tmem;
     int failed;
 };
@@ -137,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bars.full_b[i], 1);
             mbar_init(&bars.empty_b[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kUnits<NB, GP>; ++i) {
             mbar_init(&bars.sum_full[i], 1);
             mbar_init(&bars.sum_empty[i], 8);
         }
@@ -145,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fence_mbar_init();
     if (warp == kMmaWarp) {
-        tmem_alloc(&bars.tmem, 2 * NB);
+        tmem_alloc(&bars.tmem, kUnits<NB, GP> * kUnit<NB, GP> * NB);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -264,7 +270,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // directly.
         constexpr uint32_t idesc = idesc_f16(BF, 128, NB, 0);
         const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0), d0 = __shfl_sync(0xffffffffu, tmem, 0);
-        int f = 0, sta = 0, stb = 0, pha = 0, phb = 0;  // groups so far; stages and their phases
+        constexpr int kG = kUnit<NB, GP>, kN = kUnits<NB, GP>;
+        int f = 0, sta = 0, stb = 0, pha = 0, phb = 0;  // units so far; stages and their phases
         bool ok = true;
         for (int sp = s0; ok && sp < s1; ++sp) {
             ok = wait_warp(&bars.full_b[stb], phb, &bars) && wait_warp(&bars.full_a[sta], pha, &bars);
@@ -274,23 +281,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t da = sdesc(base + ua * (2 * kHalfA), 16, 1024), db = sdesc(base + SM::kB + ub * (2 * SM::kHalfB), 16, 1024);
             const int nf = flushes(sp);
 #pragma unroll
-            for (int q = 0; q < GP; ++q) {
-                if (q >= nf) break;
-                const int buf = __shfl_sync(0xffffffffu, f & 1, 0);
-                if (f >= 2) {
-                    ok = wait_warp(&bars.sum_empty[buf], (f / 2 - 1) & 1, &bars);
+            for (int q0 = 0; q0 < GP; q0 += kG) {
+                if (q0 >= nf) break;
+                const int unit = __shfl_sync(0xffffffffu, f % kN, 0);
+                if (f >= kN) {
+                    ok = wait_warp(&bars.sum_empty[unit], (f / kN - 1) & 1, &bars);
                     if (!ok) break;
                     tc_fence_after();
                 }
                 if (elect_one()) {
 #pragma unroll
-                    for (int i = 0; i < 8 / GP; ++i) {
-                        const int kk = q * (8 / GP) + i;  // 16 inputs: 32 bytes on (the descriptors count 16)
-                        mma_ss(d0 + buf * NB, da + ((kk >> 2) * kHalfA + (kk & 3) * 32) / 16,
-                               db + ((kk >> 2) * SM::kHalfB + (kk & 3) * 32) / 16, idesc, i != 0);
+                    for (int q = q0; q < q0 + kG; ++q) {
+                        if (q >= nf) break;
+#pragma unroll
+                        for (int i = 0; i < 8 / GP; ++i) {
+                            const int kk = q * (8 / GP) + i;  // 16 inputs: 32 bytes on (the descriptors count 16)
+                            mma_ss(d0 + (unit * kG + q - q0) * NB, da + ((kk >> 2) * kHalfA + (kk & 3) * 32) / 16,
+                                   db + ((kk >> 2) * SM::kHalfB + (kk & 3) * 32) / 16, idesc, i != 0);
+                        }
                     }
-                    tc_commit(&bars.sum_full[buf]);
-                    if (q == nf - 1) {
+                    tc_commit(&bars.sum_full[unit]);
+                    if (q0 + kG >= nf) {
                         tc_commit(&bars.empty_a[ua]);
                         tc_commit(&bars.empty_b[ub]);
                     }
@@ -325,26 +336,34 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int q = 0; q < GP; ++q) now[q] = next[q];
             load_scales(sp + 1);
             const int nf = flushes(sp);
+            constexpr int kG = kUnit<NB, GP>, kN = kUnits<NB, GP>;
+            constexpr int kD = NB == 64 ? 2 : 1;  // 32 columns read while 32 are added, where registers allow
 #pragma unroll
-            for (int q = 0; q < GP; ++q) {
-                if (q >= nf) break;
-                const int buf = f & 1;
-                ok = wait_warp(&bars.sum_full[buf], (f / 2) & 1, &bars);
+            for (int q0 = 0; q0 < GP; q0 += kG) {
+                if (q0 >= nf) break;
+                const int unit = f % kN;
+                ok = wait_warp(&bars.sum_full[unit], (f / kN) & 1, &bars);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * NB + half * (NB / 2));
+                const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(unit * kG * NB + half * (NB / 2));
+                constexpr int kReads = kG * (NB / 64);  // of 32 columns
+                const int reads = min(kG, nf - q0) * (NB / 64);
+                float d[kD][32];
+                if (kD == 2) tmem_ld32(at, d[0]);
 #pragma unroll
-                for (int b = 0; b < NB / 64; ++b) {
-                    float d[32];
-                    tmem_ld32(at + b * 32, d);
+                for (int i = 0; i < kReads; ++i) {
+                    if (i >= reads) break;
+                    const int q = q0 + i / (NB / 64), b = i % (NB / 64);
+                    if (kD == 1) tmem_ld32(at + (i / (NB / 64)) * NB + b * 32, d[0]);
                     tc_wait_ld();
-                    if (b == NB / 64 - 1) {
+                    if (kD == 2 && i + 1 < reads) tmem_ld32(at + ((i + 1) / (NB / 64)) * NB + (i + 1) % (NB / 64) * 32, d[(i + 1) % kD]);
+                    if (i == reads - 1) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&bars.sum_empty[buf]);
+                        if (lane == 0) mbar_arrive(&bars.sum_empty[unit]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) acc[b * 32 + i] = fmaf(now[q], d[i], acc[b * 32 + i]);
+                    for (int c = 0; c < 32; ++c) acc[b * 32 + c] = fmaf(now[q], d[i % kD][c], acc[b * 32 + c]);
                 }
                 ++f;
             }
@@ -372,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_wait_bounded(&bars.full_a[0], 0, kWaitLimit);
         }
         __syncwarp();
-        tmem_dealloc(tmem, 2 * NB);
+        tmem_dealloc(tmem, kUnits<NB, GP> * kUnit<NB, GP> * NB);
     }
     if (cs > 1) cluster_sync();
     // finished outputs: a thread keeps its output n and walks the rows of x
