@@ -69,7 +69,7 @@ __device__ __forceinline__ void stage_rows(const W4Args& a, int m0, int mrows, i
                                            bool wide) {
     constexpr int kU = 4;  // 16-byte loads in flight per lane
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = a.K;
-    const int wpr = mrows >= 8 ? 1 : mrows > 4 ? 1 : mrows > 2 ? 2 : mrows > 1 ? 4 : 8;
+    const int wpr = mrows > 4 ? 1 : mrows > 2 ? 2 : mrows > 1 ? 4 : 8;
     const int first = (warp % wpr) * 32 + lane, step = wpr * 32;
     for (int m = warp / wpr; m < mrows; m += kWarps / wpr) {
         if (a.in == W4_X_16) {
@@ -298,61 +298,61 @@ __global__ void __launch_bounds__(kWarps * 32, NT * NW <= 2 ? 2 : 1)
             issue();
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
-            if (it + u >= nmine) break;
-            const uint8_t* const sl0 = ring + slot + u * NW * kSlot;
-            uint32_t lo[NW][4], hi[NW][4];  // codes of rows g and g + 8, 8 inputs a word
-#pragma unroll
-            for (int q = 0; q < NW; ++q) {
-                const uint8_t* sl = sl0 + q * kSlot + lane * 16;
-                const uint4 a4 = *reinterpret_cast<const uint4*>(sl), b4 = *reinterpret_cast<const uint4*>(sl + 512);
-                lo[q][0] = a4.x, lo[q][1] = a4.y, lo[q][2] = a4.z, lo[q][3] = a4.w;
-                hi[q][0] = b4.x, hi[q][1] = b4.y, hi[q][2] = b4.z, hi[q][3] = b4.w;
-            }
-            float d[NW][NT][4];  // this group's sums
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t p[NW][4], r[NW][4];
+                if (it + u >= nmine) break;
+                const uint8_t* const sl0 = ring + slot + u * NW * kSlot;
+                uint32_t lo[NW][4], hi[NW][4];  // codes of rows g and g + 8, 8 inputs a word
 #pragma unroll
                 for (int q = 0; q < NW; ++q) {
-                    if (j % (4 / GP) == 0 && a.zeros[q]) {
-                        const uint32_t z = *reinterpret_cast<const uint16_t*>(sl0 + q * kSlot + 1152 + j / (4 / GP) * 16 + g * 2);
-                        zl[q] = zero_consts<BF>(z & 15u);
-                        zh[q] = zero_consts<BF>((z >> 8) & 15u);
-                    }
-                    unpack<BF>(lo[q][j], zl[q], p[q]);
-                    unpack<BF>(hi[q][j], zh[q], r[q]);
+                    const uint8_t* sl = sl0 + q * kSlot + lane * 16;
+                    const uint4 a4 = *reinterpret_cast<const uint4*>(sl), b4 = *reinterpret_cast<const uint4*>(sl + 512);
+                    lo[q][0] = a4.x, lo[q][1] = a4.y, lo[q][2] = a4.z, lo[q][3] = a4.w;
+                    hi[q][0] = b4.x, hi[q][1] = b4.y, hi[q][2] = b4.z, hi[q][3] = b4.w;
                 }
+                float d[NW][NT][4];  // this group's sums
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    // columns from vr on hold some row's values and are not read
-                    const uint4 b = *reinterpret_cast<const uint4*>(xp + xrow[t] + 32 * j);
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t p[NW][4], r[NW][4];
 #pragma unroll
                     for (int q = 0; q < NW; ++q) {
-                        if (j % (4 / GP) == 0) mma16816_first<BF>(d[q][t], p[q][0], r[q][0], p[q][1], r[q][1], b.x, b.y);
-                        else mma16816<BF>(d[q][t], p[q][0], r[q][0], p[q][1], r[q][1], b.x, b.y);
-                        mma16816<BF>(d[q][t], p[q][2], r[q][2], p[q][3], r[q][3], b.z, b.w);
+                        if (j % (4 / GP) == 0 && a.zeros[q]) {
+                            const uint32_t z = *reinterpret_cast<const uint16_t*>(sl0 + q * kSlot + 1152 + j / (4 / GP) * 16 + g * 2);
+                            zl[q] = zero_consts<BF>(z & 15u);
+                            zh[q] = zero_consts<BF>((z >> 8) & 15u);
+                        }
+                        unpack<BF>(lo[q][j], zl[q], p[q]);
+                        unpack<BF>(hi[q][j], zh[q], r[q]);
                     }
-                }
-                if ((j + 1) % (4 / GP) == 0) {
-                    const int gq = j / (4 / GP);
-                    // a group that the row does not have: its x is zero, its slot's old bytes may be anything
-                    const bool none = GP > 1 && gq > 0 && left == 1 && s1 == a.S && gq >= a.last_groups;
 #pragma unroll
-                    for (int q = 0; q < NW; ++q) {
-                        float2 sc = __half22float2(*reinterpret_cast<const __half2*>(sl0 + q * kSlot + 1024 + gq * 32 + g * 4));
-                        if (none) sc = make_float2(0.f, 0.f);
+                    for (int t = 0; t < NT; ++t) {
+                        // columns from vr on hold some row's values and are not read
+                        const uint4 b = *reinterpret_cast<const uint4*>(xp + xrow[t] + 32 * j);
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            acc[q][t][0] = fmaf(sc.x, d[q][t][0], acc[q][t][0]);
-                            acc[q][t][1] = fmaf(sc.x, d[q][t][1], acc[q][t][1]);
-                            acc[q][t][2] = fmaf(sc.y, d[q][t][2], acc[q][t][2]);
-                            acc[q][t][3] = fmaf(sc.y, d[q][t][3], acc[q][t][3]);
+                        for (int q = 0; q < NW; ++q) {
+                            if (j % (4 / GP) == 0) mma16816_first<BF>(d[q][t], p[q][0], r[q][0], p[q][1], r[q][1], b.x, b.y);
+                            else mma16816<BF>(d[q][t], p[q][0], r[q][0], p[q][1], r[q][1], b.x, b.y);
+                            mma16816<BF>(d[q][t], p[q][2], r[q][2], p[q][3], r[q][3], b.z, b.w);
+                        }
+                    }
+                    if ((j + 1) % (4 / GP) == 0) {
+                        const int gq = j / (4 / GP);
+                        // a group that the row does not have: its x is zero, its slot's old bytes may be anything
+                        const bool none = GP > 1 && gq > 0 && left == 1 && s1 == a.S && gq >= a.last_groups;
+#pragma unroll
+                        for (int q = 0; q < NW; ++q) {
+                            float2 sc = __half22float2(*reinterpret_cast<const __half2*>(sl0 + q * kSlot + 1024 + gq * 32 + g * 4));
+                            if (none) sc = make_float2(0.f, 0.f);
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                acc[q][t][0] = fmaf(sc.x, d[q][t][0], acc[q][t][0]);
+                                acc[q][t][1] = fmaf(sc.x, d[q][t][1], acc[q][t][1]);
+                                acc[q][t][2] = fmaf(sc.y, d[q][t][2], acc[q][t][2]);
+                                acc[q][t][3] = fmaf(sc.y, d[q][t][3], acc[q][t][3]);
+                            }
                         }
                     }
                 }
-            }
-            xp += ks * 128;
-            left -= ks;
+                xp += ks * 128;
+                left -= ks;
             }
             slot = slot == (kRing - 1) * kBatch ? 0 : slot + kBatch;
         }

@@ -106,8 +106,6 @@ __device__ __forceinline__ bool elect_one() {
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// BF: bf16 operands (else fp16).  GP: groups per span.  NB: columns (operand
-// rows of x) of a tile.  GATED: two matrices.
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -121,6 +119,8 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// BF: bf16 operands (else fp16).  GP: groups per span.  NB: columns (operand
+// rows of x) of a tile.  GATED: two matrices.
 template <int BF, int GP, int NB, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
     w4_tc_kernel(const __grid_constant__ W4Args a, const __grid_constant__ CUtensorMap xmap) {
@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ------------------------------------------- B: rows of x (warp 4; 5 and 6 idle)
         if (NB == 256) regs_down<56>();
         if (warp == 4) {
-            int st = 0, ph = 1;
-            for (int sp = s0; sp < s1; ++sp) {
+            int st = 0, ph = 1, sp = s0;
+            for (; sp < s1; ++sp) {
                 if (sp - s0 >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], ph, &bars)) break;
                 if (lane == 0) {
                     const uint32_t dst = smem_u32(smem) + SM::kB + st * (2 * SM::kHalfB);
@@ -261,6 +261,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (++st == kStagesB<NB>) st = 0, ph ^= 1;
             }
+            // no copy outlives the CTA, wherever another warp gave up
+            for (int i = max(sp - s0 - kStagesB<NB>, 0); i < sp - s0; ++i)
+                mbar_wait_bounded(&bars.full_b[i % kStagesB<NB>], (i / kStagesB<NB>) & 1, kWaitLimit);
         }
     } else if (warp == kMmaWarp) {
         // ----------------------------------------------------------- MMA issue
