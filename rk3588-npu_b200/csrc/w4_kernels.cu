@@ -594,11 +594,14 @@ __global__ void __launch_bounds__(256)
         if (zeros) z.u = __ldg(reinterpret_cast<const uint4*>(zeros + at));
         const uint32_t* word = span + ((kk >> 3) & 3) * 4 + (kk >> 5);
         float* to = out + (size_t)t * 16 * ldo + k;
+        uint32_t all[16];  // every row's word before any is used
+#pragma unroll
+        for (int r = 0; r < 16; ++r) all[r] = __ldg(word + (r >> 3) * 128 + (r & 7) * 16);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             if (t * 16 + r >= N) break;
             const int h = r >> 3, g = r & 7;
-            const uint32_t w = __ldg(word + h * 128 + g * 16);
+            const uint32_t w = all[r];
             const float s_r = __half2float(sc.h[g * 2 + h]), z_r = 8388608.f + (float)(z.b[g * 2 + h] & 15);
             union {
                 U u;
