@@ -1448,6 +1448,7 @@ int qw2_session_destroy(qw2_model* m, int session) {
     }
     QW_OK(kvp_seq_free(m->pool, m->session_seq[session]));
     m->session_seq[session] = -1;
+    m->controls[session].reset();
     return KV_OK;
 }
 

@@ -286,6 +286,7 @@ class Model:
 
     def destroy_session(self, session: int) -> None:
         _check(self.L.qw2_session_destroy(self.h, session), "qw2_session_destroy")
+        self._callbacks.pop(session, None)
 
     def session_exists(self, session: int) -> bool:
         e = C.c_int()

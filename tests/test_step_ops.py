@@ -102,6 +102,10 @@ LINEAR = [
     (1, 20000, 640, 128, True, "f16", "f32"),
     (4, 64, 40000, 128, False, "f32", "f32"),
     (60, 32, 30000, 64, True, "bf16", "f32"),
+    # few tiles: their spans over a cluster; long rows: x staged in turns
+    (1, 100, 8200, 64, True, "f16", "f32"),
+    (2, 17, 20000, 32, True, "bf16", "bf16"),
+    (8, 2400, 12000, 64, True, "f16", "f32"),
     # many rows: short and unaligned ones, columns that fill a tile and one more, several tiles, fp32 in parts
     (100, 20, 1, 32, True, "f16", "f32"),
     (200, 64, 8, 128, False, "bf16", "f16"),
@@ -147,6 +151,8 @@ GATED = [
     (33, 48, 300, 128, False, "bf16", "f32"),
     (100, 130, 640, 64, False, "f16", "f16"),
     (300, 96, 520, 128, True, "bf16", "bf16"),
+    (1, 40, 9000, 128, False, "f32", "f32"),
+    (4, 2400, 12500, 128, True, "bf16", "f32"),
     (70, 65, 2000, 32, True, "f32", "f32"),
     (257, 700, 129, 64, False, "f16", "f32"),
     (86, 1, 300, 128, True, "f32", "f16"),
