@@ -181,17 +181,23 @@ __global__ void __launch_bounds__(kThreads, 2)
         p.from = min(p.from, p.to);
         return p;
     };
+    // an access's logits and, where there is a mask, the word with its first bit
     uint4 x[kU];
-    auto load = [&](const T* p, int left) {
+    uint32_t bits[kU];
+    const uint32_t* const mask = q.mask ? q.mask + (size_t)row * q.ld_mask : nullptr;
+    auto load = [&](int t, int left) {
 #pragma unroll
         for (int u = 0; u < kU; ++u)
-            if (u < left) x[u] = ld16_once(p + u * apart);
+            if (u < left) {
+                x[u] = ld16_once(in + t + u * apart);
+                if (mask) bits[u] = __ldg(mask + ((t + u * apart) >> 5));
+            }
     };
     Part part = part_of(0, min(chunk, own));
-    load(in + part.t0 + part.from * apart, part.to - part.from);
+    load(part.t0 + part.from * apart, part.to - part.from);
 
     RowRules rules;
-    rules.mask = q.mask ? q.mask + (size_t)row * q.ld_mask : nullptr;
+    rules.mask = mask;
     rules.rep = q.repetition ? __ldg(q.repetition + row) : 1.f;
     rules.inv = __frcp_rn(rules.rep);
     const uint32_t rb = __float_as_uint(rules.rep);
@@ -271,14 +277,12 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
             }
         };
-        const T* pin = in + part.t0 + part.from * apart;
         T* pout = out + part.t0 + part.from * apart;
         int t = part.t0 + part.from * apart, i = i_first + part.from * kStep;
         const uint32_t sh = t & 31;  // the same for all of a thread's accesses
-        const uint32_t* pm = rules.mask ? rules.mask + (t >> 5) : nullptr;
 #pragma unroll 1
         for (int left = part.to - part.from; left > 0; left -= kU) {
-            if (c0 || left != part.to - part.from) load(pin, left);
+            if (c0 || left != part.to - part.from) load(t, left);
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
                 if (u >= left) break;
@@ -307,12 +311,11 @@ __global__ void __launch_bounds__(kThreads, 2)
                                 if (last[i + k]) l[k] = __fadd_rn(l[k], __ldg(rules.bias + last[i + k] - 1));
                         }
                 }
-                if (pm) {
-                    uint32_t ok = __ldg(pm) >> sh;
-                    if (sh + kVec > 32) ok |= __ldg(pm + 1) << (32 - sh);
+                if (mask) {
+                    uint32_t ok = bits[u] >> sh;
+                    if (sh + kVec > 32) ok |= __ldg(mask + (t >> 5) + 1) << (32 - sh);
 #pragma unroll
                     for (int j = 0; j < kVec; ++j) l[j] = (ok >> j) & 1u ? l[j] : -INFINITY;
-                    pm += apart >> 5;
                 }
                 float most = l[0];
 #pragma unroll
@@ -330,7 +333,6 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) y.el[j] = Elem<T>::put(l[j]);
                 *reinterpret_cast<uint4*>(pout) = y.v;
-                pin += apart;
                 pout += apart;
                 t += apart;
                 i += kStep;
