@@ -488,17 +488,14 @@ def _stream_object(stream, device):
     return torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
 
 
-def _scratch(w, x, dtype: int, m: int, ldx: int, gated: int, stream):
+def _scratch(w, x, dtype: int, m: int, ldx: int, stream):
     """Scratch for many rows of an x that is fp32 or not in 16-byte aligned
-    rows, held by the caching allocator for `stream`; None where none helps."""
+    rows, held by the caching allocator for `stream`.  At least what
+    w4_work_bytes says; fewer than five rows never use any."""
     if m < 5 or (dtype != STEP_F32 and ldx % 8 == 0 and x.data_ptr() % 16 == 0):
         return None
-    n = C.c_size_t()
-    call("w4_work_bytes", w.n, w.k, w.group, dtype, m, gated, C.byref(n))
-    if not n.value:
-        return None
     import torch
-    t = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+    t = torch.empty((3 if dtype == STEP_F32 else 1) * m * ((w.k + 7) // 8), 8, dtype=torch.float16, device=x.device)
     if stream is not None:
         t.record_stream(_stream_object(stream, x.device))
     return t
@@ -589,7 +586,7 @@ def w4_linear(w: W4, x, out, bias=None, residual=None, stream=None) -> None:
         if residual.dtype != out.dtype:
             raise ValueError("residual: out's element type is expected")
         r = residual.data_ptr()
-    work = _scratch(w, x, xd, m, ldx, 0, stream)
+    work = _scratch(w, x, xd, m, ldx, stream)
     rc = _lib.w4_linear(w._at, x.data_ptr(), xd, m, ldx, b, r, ldr, out.data_ptr(), _step_dtype(out, "out"), ldo,
                         work.data_ptr() if work is not None else None, _stream_on(stream, dev))
     if rc:
@@ -603,7 +600,7 @@ def w4_gated(gate: W4, up: W4, x, out, stream=None) -> None:
     m = x.shape[0]
     ldo = _rows(out, dev, "out", m, gate.n)
     xd = _step_dtype(x, "x")
-    work = _scratch(gate, x, xd, m, ldx, 1, stream)
+    work = _scratch(gate, x, xd, m, ldx, stream)
     rc = _lib.w4_gated(gate._at, up._at, x.data_ptr(), xd, m, ldx, out.data_ptr(), _step_dtype(out, "out"), ldo,
                        work.data_ptr() if work is not None else None, _stream_on(stream, dev))
     if rc:
