@@ -378,7 +378,8 @@ class Model:
                 got = mask(s, [tokens[i] for i in range(n)], gen_from)
                 if got is None:
                     return 0
-                C.memmove(out, self._mask_words(got).ctypes.data, n_words * 4)
+                words = self._mask_words(got)  # held by name while its memory is read: the address alone does not
+                C.memmove(out, words.ctypes.data, n_words * 4)
                 return 1
             except Exception:  # no exception may leave a C callback
                 return -1
