@@ -381,7 +381,7 @@ class Model:
                 words = self._mask_words(got)  # held by name while its memory is read: the address alone does not
                 C.memmove(out, words.ctypes.data, n_words * 4)
                 return 1
-            except Exception:  # no exception may leave a C callback
+            except BaseException:  # none may leave a C callback, and none may pass for "no mask"
                 return -1
 
         cb = MASK_CB(call) if mask is not None else MASK_CB()

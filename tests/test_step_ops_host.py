@@ -64,3 +64,23 @@ def test_mask_callback_hands_over_every_word(vocab, form):
             assert np.array_equal(bits[:vocab].astype(bool), want) and not bits[vocab:].any()
         else:
             assert np.array_equal(got, want)
+
+
+@pytest.mark.filterwarnings("error::pytest.PytestUnraisableExceptionWarning")
+@pytest.mark.parametrize("error", [RuntimeError, KeyboardInterrupt, SystemExit, GeneratorExit])
+def test_mask_callback_that_raises_fails_its_request(error):
+    """Whatever it raises: a status of 0 would choose without the mask."""
+    M = _Model(1000)
+
+    def mask(session, ids, gen_from):
+        raise error
+
+    M.set_controls(0, mask=mask)
+    assert mask_of(M, 0, [5], 0, 32)[0] < 0
+
+
+@pytest.mark.parametrize("answer", [np.ones(999, bool), np.ones((1, 1000), bool), np.ones(32, np.int64), np.ones(31, np.uint32)])
+def test_mask_callback_with_an_unfit_answer_fails_its_request(answer):
+    M = _Model(1000)
+    M.set_controls(0, mask=lambda session, ids, gen_from: answer)
+    assert mask_of(M, 0, [5], 0, 32)[0] < 0
