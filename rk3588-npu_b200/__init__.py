@@ -483,22 +483,37 @@ def _stream_on(stream, device: int):
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
-def _stream_object(stream, device):
+def _on_stream(stream, device, make):
+    """make()'s tensors, allocated for the stream that a call runs on: a block of
+    the current stream's may still be in use by that stream's pending work,
+    which `stream` does not wait for."""
+    if stream is None:
+        return make()
     import torch
-    return torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
+    s = torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
+    with torch.cuda.stream(s):
+        return make()
+
+
+def _handed_over(stream, device, *tensors):
+    """Results made for `stream`, which the caller may use on the current stream and free there."""
+    if stream is not None:
+        import torch
+        current = torch.cuda.current_stream(device)
+        for t in tensors:
+            if t is not None:
+                t.record_stream(current)
 
 
 def _scratch(w, x, dtype: int, m: int, ldx: int, stream):
     """Scratch for many rows of an x that is fp32 or not in 16-byte aligned
-    rows, held by the caching allocator for `stream`.  At least what
+    rows, held by the caching allocator for the call's stream.  At least what
     w4_work_bytes says; fewer than five rows never use any."""
     if m < 5 or (dtype != STEP_F32 and ldx % 8 == 0 and x.data_ptr() % 16 == 0):
         return None
     import torch
-    t = torch.empty((3 if dtype == STEP_F32 else 1) * m * ((w.k + 7) // 8), 8, dtype=torch.float16, device=x.device)
-    if stream is not None:
-        t.record_stream(_stream_object(stream, x.device))
-    return t
+    return _on_stream(stream, x.device, lambda: torch.empty((3 if dtype == STEP_F32 else 1) * m * ((w.k + 7) // 8), 8,
+                                                            dtype=torch.float16, device=x.device))
 
 
 class W4:
@@ -534,9 +549,9 @@ class W4:
         """The matrix's values, fp32 [n, k]."""
         import torch
         if out is None:
-            out = torch.empty(self.n, self.k, dtype=torch.float32, device=self.codes.device)
-            if stream is not None:
-                out.record_stream(_stream_object(stream, out.device))
+            dev = self.codes.device
+            out = _on_stream(stream, dev, lambda: torch.empty(self.n, self.k, dtype=torch.float32, device=dev))
+            _handed_over(stream, dev, out)
         elif out.dtype != torch.float32:
             raise ValueError("out: fp32 is expected")
         ld = _rows(out, self.device, "out", self.n, self.k)
@@ -556,15 +571,13 @@ def w4_quantize(w, group: int = 128, zero_points: bool = False, stream=None) -> 
         raise ValueError("w: a device tensor is expected")
     load()
     m = W4.__new__(W4)
-    m._hold(torch.empty((T, S, 2, 32, 4), dtype=torch.int32, device=dev),
-            torch.empty((T, Q, 8, 2), dtype=torch.float16, device=dev),
-            torch.empty((T, Q, 8, 2), dtype=torch.uint8, device=dev) if zero_points else None, n, k, group, dev.index)
+    arrays = _on_stream(stream, dev, lambda: (
+        torch.empty((T, S, 2, 32, 4), dtype=torch.int32, device=dev), torch.empty((T, Q, 8, 2), dtype=torch.float16, device=dev),
+        torch.empty((T, Q, 8, 2), dtype=torch.uint8, device=dev) if zero_points else None))
+    m._hold(*arrays, n, k, group, dev.index)
     ld = _rows(w, m.device, "w")
     call("w4_quantize", m._at, w.data_ptr(), dtype, ld, _stream_on(stream, m.device))
-    if stream is not None:  # the arrays were allocated for the current stream
-        for t in (m.codes, m.scales, m.zeros):
-            if t is not None:
-                t.record_stream(_stream_object(stream, dev))
+    _handed_over(stream, dev, *arrays)
     return m
 
 

@@ -1,0 +1,72 @@
+"""More forms of the step operators on a GPU: calls on several streams, operand
+rows at the borders between the kernels, special values in each of them,
+waits that run out.  Tolerances are those of test_step_ops.py."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from test_step_ops import dbl, fill, half_step, need_gpu, plain_quantize, random_matrix, sum_tol  # noqa: F401
+
+
+# ------------------------------------------------------------------ streams
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["linear", "gated"])
+@pytest.mark.parametrize("xd,offset", [("f32", 0), ("f16", 1)])
+def test_calls_on_two_streams_at_once(kv, op, xd, offset):
+    """Different rows on two streams at once, both through scratch: each result is the one that its rows have alone."""
+    need_gpu()
+    rng = np.random.default_rng(41)
+    m, n, k = 64, 1536, 8960
+    w, _ = random_matrix(kv, rng, n, k, 128, False)
+    xs = [fill(rng, (m, k + 8), xd)[:, offset:offset + k] for _ in range(2)]
+
+    def go(x, out, stream=None):
+        if op == "linear":
+            kv.w4_linear(w, x, out, stream=stream)
+        else:
+            kv.w4_gated(w, w, x, out, stream=stream)
+
+    alone = [torch.empty(m, n, device="cuda") for _ in xs]
+    for x, out in zip(xs, alone):
+        go(x, out)
+        torch.cuda.synchronize()
+    assert not torch.equal(*alone)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    outs = [[torch.empty(m, n, device="cuda") for _ in xs] for _ in range(12)]
+    torch.cuda.synchronize()
+    for a, b in outs:
+        go(xs[0], a)
+        go(xs[1], b, s)
+    for a, b in outs[:2]:  # an address in place of a stream object
+        go(xs[1], b, s.cuda_stream)
+    torch.cuda.synchronize()
+    for a, b in outs:
+        assert torch.equal(a, alone[0]) and torch.equal(b, alone[1])
+
+
+@pytest.mark.gpu
+def test_results_on_another_stream_leave_pending_work_alone(kv):
+    """Quantising and reading back on another stream while the current one still has work on a tensor that was freed."""
+    need_gpu()
+    rng = np.random.default_rng(42)
+    w = fill(rng, (512, 1024), "f16")
+    want = kv.w4_quantize(w, 32, zero_points=True)
+    values = want.dequantize()
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        ones = [torch.ones(size, dtype=torch.uint8, device="cuda")
+                for size in (want.codes.nbytes, want.scales.nbytes, want.zeros.nbytes, values.nbytes)]
+        s.wait_stream(torch.cuda.current_stream())
+        torch.cuda._sleep(20_000_000)  # the sums come ten milliseconds later
+        sums = [t.sum(dtype=torch.int64) for t in ones]
+        sizes = [t.numel() for t in ones]
+        del ones
+        got = kv.w4_quantize(w, 32, zero_points=True, stream=s)
+        read = got.dequantize(stream=s)
+        torch.cuda.synchronize()
+        assert [int(t) for t in sums] == sizes
+        assert torch.equal(got.codes, want.codes) and torch.equal(read, values)

@@ -84,3 +84,98 @@ def test_mask_callback_with_an_unfit_answer_fails_its_request(answer):
     M = _Model(1000)
     M.set_controls(0, mask=lambda session, ids, gen_from: answer)
     assert mask_of(M, 0, [5], 0, 32)[0] < 0
+
+
+# ------------------------------------------------------------- memory of calls on a stream
+class Tensor:
+    """What the wrappers ask of a contiguous 2-D device tensor; `home`: the stream it was allocated for."""
+
+    def __init__(self, shape, dtype, home=None):
+        import torch
+        self.shape, self.dtype, self.home = tuple(shape), dtype, home
+        self.device, self.used = torch.device("cuda", 0), set()
+        self.nbytes = int(np.prod(self.shape)) * dtype.itemsize
+
+    def get_device(self):
+        return 0
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return 0x100000
+
+    def record_stream(self, s):
+        self.used.add(s.cuda_stream)
+
+
+class Stream:
+    def __init__(self, address):
+        self.cuda_stream = address
+
+
+HERE, SIDE = 0xC0, 0x51DE  # the current stream, another one
+
+
+@pytest.fixture
+def streams(kv, monkeypatch):
+    """torch's allocations and the library's calls, recorded: {"made": tensors, "calls": (name, arguments)}."""
+    import torch
+    log, now = dict(made=[], calls=[]), [HERE]
+
+    class On:
+        def __init__(self, s):
+            self.s = s
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.s.cuda_stream
+
+        def __exit__(self, *a):
+            now[0] = self.before
+
+    def empty(*shape, dtype=None, device=None):
+        shape = shape[0] if isinstance(shape[0], tuple) else shape
+        log["made"].append(Tensor(shape, dtype, now[0]))
+        return log["made"][-1]
+
+    class Lib:
+        def __getattr__(self, name):
+            real = getattr(lib, name)
+            if name in ("w4_linear", "w4_gated", "w4_quantize", "w4_dequantize"):
+                return lambda *a: log["calls"].append((name, a)) or 0
+            return real
+
+    lib = kv.load()
+    monkeypatch.setattr(torch, "empty", empty)
+    monkeypatch.setattr(torch.cuda, "stream", On)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: Stream(now[0]))
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda a, device=None: Stream(a))
+    monkeypatch.setattr(kv, "_raw_stream", lambda d: now[0])
+    monkeypatch.setattr(kv, "_lib", Lib())
+    return log
+
+
+def w4_of(kv, n, k, group):
+    import torch
+    m = kv.W4.__new__(kv.W4)
+    m._hold(Tensor((1,), torch.int32), Tensor((1,), torch.float16), None, n, k, group, 0)
+    return m
+
+
+@pytest.mark.parametrize("stream", [None, Stream(SIDE), SIDE], ids=["current", "object", "address"])
+def test_memory_of_a_call_belongs_to_its_stream(kv, streams, stream):
+    """Scratch, quantised arrays and values read back are allocated for the stream that writes them: a block of the
+    current stream's may still be read or written by that stream's pending work, which another stream does not wait for."""
+    import torch
+    w, at = w4_of(kv, 64, 512, 64), HERE if stream is None else SIDE
+    x, out = Tensor((64, 512), torch.float32), Tensor((64, 64), torch.float32)
+    kv.w4_linear(w, x, out, stream=stream)
+    kv.w4_gated(w, w, x, out, stream=stream)
+    assert [t.home for t in streams["made"]] == [at, at]  # scratch of both
+    m = kv.w4_quantize(Tensor((64, 512), torch.float16), 64, zero_points=True, stream=stream)
+    y = w.dequantize(stream=stream)
+    assert all(t.home == at for t in (m.codes, m.scales, m.zeros, y))
+    # what is handed to the caller may be used on the current stream too, and freed there
+    assert all(t.home == HERE or HERE in t.used for t in (m.codes, m.scales, m.zeros, y))
+    assert [name for name, _ in streams["calls"]] == ["w4_linear", "w4_gated", "w4_quantize", "w4_dequantize"]
+    assert all(a[-1] == at for _, a in streams["calls"])
