@@ -282,9 +282,10 @@ class Pool:
         import torch
         n = self.cur_pos(seq)
         dev = torch.device("cuda", self.device)
-        k = torch.empty((n, self.kv_dim), dtype=torch.int16, device=dev)
-        v = torch.empty((n, self.kv_dim), dtype=torch.int16, device=dev)
+        rows = _on_stream(stream, dev, lambda: [torch.empty((n, self.kv_dim), dtype=torch.int16, device=dev) for _ in range(2)])
+        k, v = rows
         call("kvp_gather", self.h, layer, seq, _ptr(k), _ptr(v), _stream(stream))
+        _handed_over(stream, dev, *rows)
         return k, v
 
     def import_i8(self, layer, seq, pos0, k_codes, v_codes, k_scales, v_scales, stream=None) -> None:
@@ -298,11 +299,11 @@ class Pool:
         import torch
         n = self.cur_pos(seq)
         dev = torch.device("cuda", self.device)
-        kc = torch.empty((n, self.kv_dim), dtype=torch.int8, device=dev)
-        vc = torch.empty((n, self.kv_dim), dtype=torch.int8, device=dev)
-        ks = torch.empty((n, self.kv_dim // HEAD_DIM), dtype=torch.float32, device=dev)
-        vs = torch.empty((n, self.kv_dim // HEAD_DIM), dtype=torch.float32, device=dev)
+        rows = _on_stream(stream, dev, lambda: [torch.empty((n, self.kv_dim), dtype=torch.int8, device=dev) for _ in range(2)] + [
+            torch.empty((n, self.kv_dim // HEAD_DIM), dtype=torch.float32, device=dev) for _ in range(2)])
+        kc, vc, ks, vs = rows
         call("kvp_gather_i8", self.h, layer, seq, _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), _stream(stream))
+        _handed_over(stream, dev, *rows)
         return kc, vc, ks, vs
 
     def append_chunk(self, layer, seq, pos0, k, v, stream=None) -> None:

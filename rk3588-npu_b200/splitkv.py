@@ -35,7 +35,7 @@ import torch.distributed as dist
 
 import ctypes as C
 
-from . import Pool, call, _ptr, _stream, _vp, HEAD_DIM, KVX_HANDLE_BYTES, KVN_UNIQUE_ID_BYTES
+from . import Pool, call, _on_stream, _ptr, _stream, _vp, HEAD_DIM, KVX_HANDLE_BYTES, KVN_UNIQUE_ID_BYTES
 
 
 def slice_bounds(length: int, rank: int, world: int) -> tuple[int, int]:
@@ -139,8 +139,8 @@ class SplitKV:
         if self._buf is None and self.pool.device >= 0 and self.transport == "collective":  # host-only pools never run
             dev = torch.device("cuda", self.pool.device)
             n = self.rows * (2 + HEAD_DIM)
-            self._buf = torch.empty(n, device=dev)
-            self._all = torch.empty((self.world, n), device=dev)
+            self._buf, self._all = _on_stream(stream, dev, lambda: (torch.empty(n, device=dev),
+                                                                    torch.empty((self.world, n), device=dev)))
 
     def layer(self, layer: int, q, k_new, v_new, out, stream=None) -> None:
         """One layer of the step.  q [B, q_heads*128], k/v [B, kv_heads*128]

@@ -141,7 +141,7 @@ def streams(kv, monkeypatch):
     class Lib:
         def __getattr__(self, name):
             real = getattr(lib, name)
-            if name in ("w4_linear", "w4_gated", "w4_quantize", "w4_dequantize"):
+            if name in ("w4_linear", "w4_gated", "w4_quantize", "w4_dequantize", "kvp_gather", "kvp_gather_i8"):
                 return lambda *a: log["calls"].append((name, a)) or 0
             return real
 
@@ -179,3 +179,14 @@ def test_memory_of_a_call_belongs_to_its_stream(kv, streams, stream):
     assert all(t.home == HERE or HERE in t.used for t in (m.codes, m.scales, m.zeros, y))
     assert [name for name, _ in streams["calls"]] == ["w4_linear", "w4_gated", "w4_quantize", "w4_dequantize"]
     assert all(a[-1] == at for _, a in streams["calls"])
+
+
+@pytest.mark.parametrize("stream", [None, Stream(SIDE), SIDE], ids=["current", "object", "address"])
+def test_gathered_rows_belong_to_the_calls_stream(kv, streams, stream):
+    at = HERE if stream is None else SIDE
+    P = kv.Pool.__new__(kv.Pool)
+    P.h, P.device, P.kv_dim, P.cur_pos = None, 0, 256, lambda seq: 40
+    rows = [*P.gather(0, 0, stream=stream), *P.gather_i8(0, 0, stream=stream)]
+    P.h = None
+    assert all(t.home == at and (at == HERE or HERE in t.used) for t in rows)
+    assert [(name, a[-1]) for name, a in streams["calls"]] == [("kvp_gather", at), ("kvp_gather_i8", at)]
