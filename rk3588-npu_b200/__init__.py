@@ -506,15 +506,22 @@ def _handed_over(stream, device, *tensors):
                 t.record_stream(current)
 
 
-def _scratch(w, x, dtype: int, m: int, ldx: int, stream):
-    """Scratch for many rows of an x that is fp32 or not in 16-byte aligned
-    rows, held by the caching allocator for the call's stream.  At least what
-    w4_work_bytes says; fewer than five rows never use any."""
-    if m < 5 or (dtype != STEP_F32 and ldx % 8 == 0 and x.data_ptr() % 16 == 0):
+def _scratch(w, x, dtype: int, m: int, ldx: int, gated: int, stream):
+    """Scratch of w4_work_bytes() for an x that is fp32 or not in 16-byte aligned
+    rows, held by the caching allocator for the call's stream; None where no
+    rows go through it."""
+    if dtype != STEP_F32 and ldx % 8 == 0 and x.data_ptr() % 16 == 0:
+        return None
+    key = (m, dtype == STEP_F32, gated)
+    size = w._work.get(key)
+    if size is None:  # the sizes of a matrix do not change
+        n = C.c_size_t()
+        call("w4_work_bytes", w.n, w.k, w.group, dtype, m, gated, C.byref(n))
+        size = w._work[key] = n.value
+    if not size:
         return None
     import torch
-    return _on_stream(stream, x.device, lambda: torch.empty((3 if dtype == STEP_F32 else 1) * m * ((w.k + 7) // 8), 8,
-                                                            dtype=torch.float16, device=x.device))
+    return _on_stream(stream, x.device, lambda: torch.empty(size, dtype=torch.uint8, device=x.device))
 
 
 class W4:
@@ -545,6 +552,7 @@ class W4:
         self._c = _W4Matrix(dev, n, k, group, codes.data_ptr(), scales.data_ptr(),
                             zeros.data_ptr() if zeros is not None else None)
         self._at = C.addressof(self._c)
+        self._work = {}  # (rows, fp32, gated) -> w4_work_bytes
 
     def dequantize(self, out=None, stream=None):
         """The matrix's values, fp32 [n, k]."""
@@ -600,7 +608,7 @@ def w4_linear(w: W4, x, out, bias=None, residual=None, stream=None) -> None:
         if residual.dtype != out.dtype:
             raise ValueError("residual: out's element type is expected")
         r = residual.data_ptr()
-    work = _scratch(w, x, xd, m, ldx, stream)
+    work = _scratch(w, x, xd, m, ldx, 0, stream)
     rc = _lib.w4_linear(w._at, x.data_ptr(), xd, m, ldx, b, r, ldr, out.data_ptr(), _step_dtype(out, "out"), ldo,
                         work.data_ptr() if work is not None else None, _stream_on(stream, dev))
     if rc:
@@ -614,7 +622,7 @@ def w4_gated(gate: W4, up: W4, x, out, stream=None) -> None:
     m = x.shape[0]
     ldo = _rows(out, dev, "out", m, gate.n)
     xd = _step_dtype(x, "x")
-    work = _scratch(gate, x, xd, m, ldx, stream)
+    work = _scratch(gate, x, xd, m, ldx, 1, stream)
     rc = _lib.w4_gated(gate._at, up._at, x.data_ptr(), xd, m, ldx, out.data_ptr(), _step_dtype(out, "out"), ldo,
                        work.data_ptr() if work is not None else None, _stream_on(stream, dev))
     if rc:

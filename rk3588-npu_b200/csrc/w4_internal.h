@@ -147,9 +147,13 @@ inline W4TcPlan w4_tc_plan(int M, int T, int S, int pieces, int nw) {
 // 8 rows 7.8 / 12; 2048 x 1536, 48 rows 11.1 / 10.5, 32 rows 6.3 / 9.7; 8960 x 1536
 // gated, 24 rows 15.9 / 13.4, 16 rows 10.6 / 13.3; the same in groups of 32, 48 rows
 // 30.5 / 19.5, 32 rows 18.9 / 19.3; 151936 x 1536, 48 rows 158 / 127, 32 rows 96 / 125.
+// The parts of an fp32 x take a launch of their own first, so they need five rows
+// (15 of parts): 4 and 5 rows of fp32, 1536 x 8960 16.6 / 13.5 and 25.1 / 13.5, 4096 x 4096
+// 10.2 / 12.3 and 14.0 / 12.4, gated 13.6 / 20.0 and 16.8 / 20.0, 1536 x 8960 gated in groups of
+// 32 22.3 / 28.7 and 31.2 / 28.7.
 inline bool w4_use_tc(int M, int T, int S, int pieces, int nw, int group) {
     const int tiles = (T + 7) / 8 * nw, rows = M * pieces;
-    if (tiles <= kSms && S >= 32) return rows > (group == 32 ? 10 : 8);
+    if (tiles <= kSms && S >= 32) return rows > (pieces == 3 ? 14 : group == 32 ? 10 : 8);
     if (tiles <= kSms && nw == 2) return rows > (group == 32 ? 32 : 20);
     return rows > 40;
 }

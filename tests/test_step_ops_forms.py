@@ -10,6 +10,35 @@ import torch
 from test_step_ops import dbl, fill, half_step, need_gpu, plain_quantize, random_matrix, sum_tol  # noqa: F401
 
 
+def near_linear(kv, w, ref, x, out, group, yd):
+    """out = x W^T within test_step_ops.py's bound."""
+    want = dbl(x) @ ref.T
+    tol = sum_tol(dbl(x), ref, group) + 2.0**-23 * np.abs(want)
+    tol = tol + half_step(np.abs(want) + tol, yd)
+    assert np.all(np.abs(dbl(out) - want) <= tol), np.max(np.abs(dbl(out) - want) / tol)
+
+
+# --------------------------------------------- rows at the borders between the kernels
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,group", [(96, 4096, 32), (200, 4100, 128), (1500, 640, 64)])
+@pytest.mark.parametrize("xd", ["f32", "bf16"])
+def test_linear_from_few_to_many_rows(kv, n, k, group, xd):
+    """Every count of rows from 1 to 24, and around a tile of columns: with the scratch that the planner asks for,
+    where the parts of five fp32 rows go to the tensor-memory form, and without any."""
+    need_gpu()
+    rng = np.random.default_rng(k)
+    w, ref = random_matrix(kv, rng, n, k, group, True)
+    for m in (*range(1, 25), 41, 43, 64, 65, 85, 86):
+        x, out = fill(rng, (m, k), xd), torch.empty(m, n, device="cuda")
+        kv.w4_linear(w, x, out)
+        near_linear(kv, w, ref, x, out, group, "f32")
+        out.fill_(0)
+        kv.call("w4_linear", w._at, x.data_ptr(), kv.STEP_F32 if xd == "f32" else kv.STEP_BF16, m, k, None, None, 0,
+                out.data_ptr(), kv.STEP_F32, n, None, torch.cuda.current_stream().cuda_stream)
+        near_linear(kv, w, ref, x, out, group, "f32")
+    assert kv.step_ops_status() == kv.KV_OK
+
+
 # ------------------------------------------------------------------ streams
 @pytest.mark.gpu
 @pytest.mark.parametrize("op", ["linear", "gated"])

@@ -190,3 +190,39 @@ def test_gathered_rows_belong_to_the_calls_stream(kv, streams, stream):
     P.h = None
     assert all(t.home == at and (at == HERE or HERE in t.used) for t in rows)
     assert [(name, a[-1]) for name, a in streams["calls"]] == [("kvp_gather", at), ("kvp_gather_i8", at)]
+
+
+# (n, k, group): few tiles of long rows, where few operand rows take the tcgen05 form; short rows; many tiles
+SCRATCH = [(1536, 8960, 128), (1536, 8960, 32), (100, 4000, 64), (100, 4096, 32), (2048, 1536, 128), (8960, 1536, 32),
+           (40000, 1536, 128), (40000, 5000, 64), (33, 257, 64)]
+
+
+@pytest.mark.parametrize("n,k,group", SCRATCH)
+@pytest.mark.parametrize("xd", ["f32", "f16"])
+def test_scratch_is_what_the_call_asks_for(kv, streams, n, k, group, xd):
+    """w4_linear and w4_gated hand over scratch where w4_work_bytes says that rows of x go through it, of that size at
+    least, and none where it says 0: 1 to 48 rows, and many; 16-bit rows that TMA can address never need any."""
+    import torch
+    w, size = w4_of(kv, n, k, group), C.c_size_t()
+    dtype, code = (torch.float32, kv.STEP_F32) if xd == "f32" else (torch.float16, kv.STEP_F16)
+    some = 0
+    for m in (*range(1, 49), 100, 1000):
+        for gated in (0, 1):
+            kv.call("w4_work_bytes", n, k, group, code, m, gated, C.byref(size))
+            x, out = Tensor((m, k), dtype), Tensor((m, n), torch.float32)
+            for misaligned in (0, 2):
+                if misaligned and xd == "f32":
+                    continue
+                x.data_ptr = lambda: 0x100000 + misaligned
+                want = 0 if xd == "f16" and k % 8 == 0 and not misaligned else size.value
+                streams["made"].clear()
+                if gated:
+                    kv.w4_gated(w, w, x, out)
+                else:
+                    kv.w4_linear(w, x, out)
+                work = streams["calls"][-1][1][-2]
+                made = [t.nbytes for t in streams["made"]]
+                assert (work is not None) == (want > 0) == (len(made) == 1), (m, gated)
+                assert sum(made) >= want, (m, gated)
+                some += want > 0
+    assert some
