@@ -58,7 +58,7 @@ int kv_kernel_count(long long* n) {
 namespace {
 
 int cuda_fail(cudaError_t e, const char* what) {
-    return fail(KV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    return fail(KV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(taken(e)));
 }
 
 #define KV_CUDA(call)                                   \

@@ -302,6 +302,13 @@ cudaError_t launch_f16_to_f32_exact(const uint16_t* y16, long n, float* y, cudaS
 // the reference's float libm calls.
 const float2* pool_rope_table(const ::kvp_pool* p);
 
+// An error that goes to the caller, taken from the runtime, which would hold it for
+// the next launch that asks for the last one.
+inline cudaError_t taken(cudaError_t e) {
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e;
+}
+
 // Sets a device for the scope of a call and restores the caller's.
 struct DeviceGuard {
     int prev = -1;
@@ -309,7 +316,7 @@ struct DeviceGuard {
     explicit DeviceGuard(int dev) {
         if (dev < 0) return;  // host-only object: no device calls
         if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
+        if (prev != dev) ok = taken(cudaSetDevice(dev)) == cudaSuccess;
         else prev = -1;  // nothing to restore
     }
     ~DeviceGuard() {
@@ -343,7 +350,7 @@ int set_error(int status, const char* msg);
 void count_launch();
 inline cudaError_t counted(cudaError_t e) {
     if (e == cudaSuccess) count_launch();
-    return e;
+    return taken(e);
 }
 
 }  // namespace kvattn

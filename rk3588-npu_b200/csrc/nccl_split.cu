@@ -87,7 +87,7 @@ int nccl_gather_combine(::kvn_comm* c, int rows, float* out, cudaStream_t st) {
     if (r != ncclSuccess) return nccl_fail(r, "ncclAllGather");
     const float* pk = c->recv;
     cudaError_t e = launch_combine(c->world, rows, kHeadDim, pk, pk + rows, pk + 2 * (size_t)rows, per, per, out, st);
-    if (e != cudaSuccess) return set_error(KV_ERR_CUDA, cudaGetErrorString(e));
+    if (e != cudaSuccess) return set_error(KV_ERR_CUDA, cudaGetErrorString(taken(e)));
     return KV_OK;
 }
 
@@ -121,8 +121,8 @@ int kvn_create(int device, int rank, int world, const void* id, int max_rows, kv
     c->world = world;
     c->max_rows = max_rows;
     const size_t per = (size_t)max_rows * (2 + kHeadDim);
-    if (cudaMalloc((void**)&c->send, per * sizeof(float)) != cudaSuccess ||
-        cudaMalloc((void**)&c->recv, per * world * sizeof(float)) != cudaSuccess) {
+    if (taken(cudaMalloc((void**)&c->send, per * sizeof(float))) != cudaSuccess ||
+        taken(cudaMalloc((void**)&c->recv, per * world * sizeof(float))) != cudaSuccess) {
         cudaFree(c->send);
         cudaFree(c->recv);
         delete c;

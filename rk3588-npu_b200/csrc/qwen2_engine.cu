@@ -56,7 +56,7 @@ int qfail(int status, const char* fmt, ...) {
 #define QW_CUDA(call)                                                                             \
     do {                                                                                          \
         cudaError_t e_ = (call);                                                                  \
-        if (e_ != cudaSuccess) return qfail(KV_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); \
+        if (e_ != cudaSuccess) return qfail(KV_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(taken(e_))); \
     } while (0)
 
 #define QW_OK(call)                \
@@ -207,7 +207,7 @@ struct qw2_model {
 
     int alloc(void** p, size_t bytes) {
         cudaError_t e = cudaMalloc(p, bytes);
-        if (e != cudaSuccess) return qfail(KV_ERR_OOM, "cudaMalloc(%zu): %s", bytes, cudaGetErrorString(e));
+        if (e != cudaSuccess) return qfail(KV_ERR_OOM, "cudaMalloc(%zu): %s", bytes, cudaGetErrorString(taken(e)));
         allocs.push_back(*p);
         return KV_OK;
     }
@@ -1646,7 +1646,7 @@ int qw2_quantize_weights(qw2_model* m, int group, int zero_points) {
     }
     if (rc == KV_OK) {
         const cudaError_t e = cudaStreamSynchronize(m->st);
-        if (e != cudaSuccess) rc = qfail(KV_ERR_CUDA, "quantising the weights: %s", cudaGetErrorString(e));
+        if (e != cudaSuccess) rc = qfail(KV_ERR_CUDA, "quantising the weights: %s", cudaGetErrorString(taken(e)));
     }
     if (rc != KV_OK) {
         cudaStreamSynchronize(m->st);

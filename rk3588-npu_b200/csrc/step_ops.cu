@@ -107,7 +107,7 @@ int check_work(const w4_matrix& w, const void* x, int x_dtype, int m, long long 
 
 int launched(cudaError_t e, const char* what) {
     if (e == cudaSuccess) return KV_OK;
-    return sfail(KV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    return sfail(KV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(taken(e)));
 }
 
 }  // namespace

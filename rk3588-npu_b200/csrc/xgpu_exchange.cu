@@ -240,7 +240,7 @@ struct DevGuard {
 
 int cuda_err(cudaError_t e, const char* what) {
     char buf[256];
-    snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
+    snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(taken(e)));
     return set_error(KV_ERR_CUDA, buf);
 }
 

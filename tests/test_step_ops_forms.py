@@ -3,10 +3,13 @@ rows at the borders between the kernels, special values in each of them,
 waits that run out.  Tolerances are those of test_step_ops.py."""
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
+from test_model_sessions import q2
 from test_step_ops import dbl, fill, half_step, need_gpu, plain_quantize, random_matrix, sum_tol  # noqa: F401
 
 
@@ -99,3 +102,31 @@ def test_results_on_another_stream_leave_pending_work_alone(kv):
         torch.cuda.synchronize()
         assert [int(t) for t in sums] == sizes
         assert torch.equal(got.codes, want.codes) and torch.equal(read, values)
+
+
+# ---------------------------------------------------------- after an error
+@pytest.mark.gpu
+def test_a_refused_call_leaves_no_error_behind(kv):
+    """A device that is not there and memory that is not there are reported once, by the call that asked for them."""
+    need_gpu()
+    w = fill(np.random.default_rng(1), (64, 64), "f16")
+    m = kv.w4_quantize(w, 32)
+    values = m.dequantize()
+
+    def fine():
+        assert torch.equal(kv.w4_quantize(w, 32).codes, m.codes) and torch.equal(m.dequantize(), values)
+
+    with pytest.raises(kv.KVError):
+        kv.step_ops_status(999)
+    fine()
+    far = kv._W4Matrix(999, 64, 64, 32, m.codes.data_ptr(), m.scales.data_ptr(), None)
+    out = torch.empty(2, 64, device="cuda")
+    for name, args in (("w4_quantize", (w.data_ptr(), 0, 64)), ("w4_dequantize", (values.data_ptr(), 64)),
+                       ("w4_linear", (w.data_ptr(), 0, 2, 64, None, None, 0, out.data_ptr(), 2, 64, None))):
+        with pytest.raises(kv.KVError):
+            kv.call(name, C.addressof(far), *args, None)
+        fine()
+    cfg = dict(q2().QWEN2_1_5B, hidden=4096, q_heads=32, kv_heads=32, vocab=2**30, layers=1)  # 8 TB of embedding
+    with pytest.raises(kv.KVError):
+        q2().Model(0, cfg)
+    fine()
