@@ -209,7 +209,9 @@ int qw2_cancel(qw2_model* m, int session);
  * multiply the 4-bit values with the same fp16 inputs, fp32 sums and
  * epilogues.  KV_ERR_STATE while a request runs, a second time, or together
  * with qw2_set_exact; matrices cannot be set afterwards.  On failure (no
- * memory) the model is unchanged. */
+ * memory) the model is unchanged.  A forward in which a bounded wait of the
+ * projections ran out (step_ops_wait_limit) returns KV_ERR_TIMEOUT, as one of
+ * the attention's does: what its sessions' caches hold of it is unspecified. */
 int qw2_quantize_weights(qw2_model* m, int group, int zero_points);
 
 /* ------------------------------------------------------------ controls

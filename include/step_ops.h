@@ -97,9 +97,16 @@ int w4_gated(const w4_matrix* gate, const w4_matrix* up, const void* x, int x_dt
 int w4_work_bytes(int n, int k, int group, int x_dtype, int m, int gated, size_t* bytes);
 
 /* The waits inside the kernels for many rows are bounded (about a second):
- * *status is KV_OK, or KV_ERR_TIMEOUT if one has run out on `device` since the
- * last call (that launch's outputs are not written).  Synchronises the device. */
+ * *status is KV_OK, or KV_ERR_TIMEOUT if one has run out in a call on `device`
+ * since the last step_ops_status (what that call's out holds is then
+ * unspecified: some of it may be written, some of that from unfinished sums).
+ * Synchronises the device.  A model's forwards report their own (KV_ERR_TIMEOUT
+ * from the forward), and not here. */
 int step_ops_status(int device, int* status);
+
+/* The limit of those waits, in SM clocks, for every launch of this process from
+ * now on: 0 gives up wherever something is not ready yet, < 0 is the default. */
+int step_ops_wait_limit(long long clocks);
 
 /* Penalties, biases, a mask and the greedy choice on `rows` rows of logits.
  * For row r and token t, in fp32, each step rounded by itself:

@@ -118,6 +118,7 @@ _SIGS.update({
     "w4_work_bytes": [C.c_int] * 6 + [C.POINTER(C.c_size_t)],
     "logits_adjust": [C.POINTER(_LogitsCall), _vp],
     "step_ops_status": [C.c_int, _ip],
+    "step_ops_wait_limit": [C.c_longlong],
 })
 _RESTYPE = {"kv_last_error": C.c_char_p, "kv_status_str": C.c_char_p, "kv_version": C.c_char_p}
 
@@ -634,6 +635,11 @@ def step_ops_status(device: int = 0) -> int:
     s = C.c_int()
     call("step_ops_status", device, C.byref(s))
     return s.value
+
+
+def step_ops_wait_limit(clocks: int = -1) -> None:
+    """The limit of those waits in SM clocks for launches from now on (0: what is not ready has run out; < 0: about a second)."""
+    call("step_ops_wait_limit", clocks)
 
 
 def logits_adjust(logits, out, pick=None, hist=None, hist_off=None, gen_from=None, repetition=None, presence=None,

@@ -179,6 +179,7 @@ struct kvp_pool {
 };
 
 const float2* kvattn::pool_rope_table(const kvp_pool* p) { return p ? p->d_rope : nullptr; }
+int* kvattn::pool_status(const kvp_pool* p) { return p ? p->d_status : nullptr; }
 
 namespace {
 

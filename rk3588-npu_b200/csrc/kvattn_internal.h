@@ -301,6 +301,8 @@ cudaError_t launch_f16_to_f32_exact(const uint16_t* y16, long n, float* y, cudaS
 // The pool's device RoPE table [max_seq_len][64] (cos, sin), host-built with
 // the reference's float libm calls.
 const float2* pool_rope_table(const ::kvp_pool* p);
+// The pool's device status words (kvp_device_status reads and clears them).
+int* pool_status(const ::kvp_pool* p);
 
 // An error that goes to the caller, taken from the runtime, which would hold it for
 // the next launch that asks for the last one.

@@ -615,6 +615,7 @@ cudaError_t project(const qw2_model* m, int mode, int in, const GemvArgs& a, con
     }
     w.mode = mode;  // the launch_gemv modes
     w.g = a;
+    w.status = pool_status(m->pool);  // read with the pool's own, at the forward's end
     w.early = true;
     return launch_w4(w, q.group, /*bf16*/ false, q2 ? 2 : 1, st);
 }

@@ -214,6 +214,11 @@ int step_ops_status(int device, int* status) {
     return launched(e, "step_ops_status");
 }
 
+int step_ops_wait_limit(long long clocks) {
+    set_wait_limit(clocks);
+    return KV_OK;
+}
+
 int logits_adjust(const logits_call* c, void* stream) {
     if (!c) return sfail(KV_ERR_INVAL, "NULL call");
     ST_OK(check_dtype(c->dtype, "logits"));

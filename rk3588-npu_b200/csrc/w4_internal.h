@@ -50,6 +50,8 @@ struct W4Args {
     int chunk = 0;            // spans of x staged at a time
     int batches = 2;    // of codes per warp in shared memory
     int last_groups = 0;      // groups of a row's last span
+    int* status = nullptr;    // where a wait of the tcgen05 form that runs out is noted: a pool's status words, or NULL, the public calls'
+    long long wait_limit = 0; // SM clocks; 0: what is not ready has run out
     bool early = false;       // the weights may be read before the previous kernel of the stream ends
 
     void set_matrix(int i, const w4_matrix& w) {
@@ -65,6 +67,7 @@ struct W4Args {
 };
 
 constexpr int kSms = 148;
+constexpr long long kW4WaitLimit = 2000000000LL;  // SM clocks: about a second
 constexpr int kW4MaxSmem = 227 * 1024;
 // Floats of a warp's partial tile: 20 per column (16 rows, padded against bank
 // conflicts), 4 more so that the warps' tiles start in different banks.
@@ -168,8 +171,10 @@ cudaError_t launch_w4(W4Args a, int group, bool bf, int nw, cudaStream_t st);
 inline size_t w4_rows_bytes(int M, int K, int pieces) { return (size_t)pieces * M * ((K + 7) / 8 * 8) * 2; }
 cudaError_t launch_rows(bool f32, const void* x, long long ldx, int M, int K, void* to, cudaStream_t st);
 cudaError_t launch_w4_tc(W4Args a, int group, bool bf, int nw, cudaStream_t st);
-// The status of the waits in launch_w4_tc's kernels on the current device
-// (0, or KV_ERR_TIMEOUT), cleared by reading it.
+// The limit of the waits in launch_w4_tc's kernels from now on (< 0: kW4WaitLimit).
+void set_wait_limit(long long clocks);
+// The status of those waits in the public calls' launches on the current
+// device (0, or KV_ERR_TIMEOUT), cleared by reading it.
 cudaError_t step_status(int* status);
 cudaError_t launch_w4_quantize(const w4_matrix& m, const void* w, int dtype, long long ldw, cudaStream_t st);
 cudaError_t launch_w4_dequantize(const w4_matrix& m, float* out, long long ldo, cudaStream_t st);

@@ -29,6 +29,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "device_common.cuh"
 #include "kvattn.h"
 #include "kvattn_internal.h"
@@ -56,7 +58,6 @@ constexpr int kCodes = 2 * 1024 + 128;  // a span of a warp's two tiles, and the
 constexpr int kThreads = 16 * 32;
 constexpr int kMmaWarp = 7;
 constexpr int kHalfA = 128 * 128;  // 64 inputs of 128 rows
-constexpr long long kWaitLimit = 2000000000LL;  // SM clocks: about a second
 
 template <int NB>
 struct Smem {
@@ -70,22 +71,28 @@ struct Smem {
 
 struct Bars {
     uint64_t full_a[kStagesA], empty_a[kStagesA], full_b[4], empty_b[4], sum_full[4], sum_empty[4];
+    uint64_t done;  // the MMAs in flight where a wait gave up
     uint32_t tmem;
     int failed;
 };
 
-__device__ int g_step_status;  // KV_ERR_TIMEOUT once a wait has run out
+// The public calls' status words, as a pool's: KV_ERR_TIMEOUT once a wait has run out, its CTA, where.
+__device__ int g_step_status[3];
 
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Bars* b) {
-    if (mbar_wait_bounded(bar, parity, kWaitLimit)) return true;
-    atomicCAS(&g_step_status, 0, KV_ERR_TIMEOUT);
+__device__ __noinline__ void gave_up(const W4Args& a, Bars* b) {
+    int* const status = a.status ? a.status : g_step_status;
+    if (atomicCAS(status, 0, KV_ERR_TIMEOUT) == 0) {
+        status[1] = blockIdx.x;
+        status[2] = 800;
+    }
     *reinterpret_cast<volatile int*>(&b->failed) = 1;
-    return false;
 }
 
-// The same for a whole warp: all of its lanes, or none, go on.
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Bars* b) {
-    const bool ok = wait(bar, parity, b) && !*reinterpret_cast<volatile int*>(&b->failed);
+// A whole warp's wait: all of its lanes, or none, go on.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Bars* b, const W4Args& a) {
+    bool ok = a.wait_limit > 0 ? mbar_wait_bounded(bar, parity, a.wait_limit) : mbar_test_wait(bar, parity);
+    if (!ok) gave_up(a, b);
+    ok = ok && !*reinterpret_cast<volatile int*>(&b->failed);
     return __all_sync(0xffffffffu, ok);
 }
 
@@ -147,6 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&bars.sum_full[i], 1);
             mbar_init(&bars.sum_empty[i], 8);
         }
+        mbar_init(&bars.done, 1);
         bars.failed = 0;
     }
     fence_mbar_init();
@@ -216,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             cp_wait<kAhead - 2>();
             __syncwarp();  // zero points came by other lanes; the slot refilled next was read by all of them
             fetch();
-            if (sp - s0 >= kStagesA && !wait_warp(&bars.empty_a[st], ph, &bars)) break;
+            if (sp - s0 >= kStagesA && !wait_warp(&bars.empty_a[st], ph, &bars, a)) break;
             const uint8_t* from = ring + slot * kCodes;
             uint8_t* to = smem + st * (2 * kHalfA) + row0 + chunk0;
 #pragma unroll 1
@@ -251,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == 4) {
             int st = 0, ph = 1, sp = s0;
             for (; sp < s1; ++sp) {
-                if (sp - s0 >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], ph, &bars)) break;
+                if (sp - s0 >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], ph, &bars, a)) break;
                 if (lane == 0) {
                     const uint32_t dst = smem_u32(smem) + SM::kB + st * (2 * SM::kHalfB);
                     mbar_arrive_expect_tx(&bars.full_b[st], 2 * SM::kHalfB);
@@ -263,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // no copy outlives the CTA, wherever another warp gave up
             for (int i = max(sp - s0 - kStagesB<NB>, 0); i < sp - s0; ++i)
-                mbar_wait_bounded(&bars.full_b[i % kStagesB<NB>], (i / kStagesB<NB>) & 1, kWaitLimit);
+                mbar_wait_bounded(&bars.full_b[i % kStagesB<NB>], (i / kStagesB<NB>) & 1, kW4WaitLimit);
         }
     } else if (warp == kMmaWarp) {
         // ----------------------------------------------------------- MMA issue
@@ -277,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int f = 0, sta = 0, stb = 0, pha = 0, phb = 0;  // units so far; stages and their phases
         bool ok = true;
         for (int sp = s0; ok && sp < s1; ++sp) {
-            ok = wait_warp(&bars.full_b[stb], phb, &bars) && wait_warp(&bars.full_a[sta], pha, &bars);
+            ok = wait_warp(&bars.full_b[stb], phb, &bars, a) && wait_warp(&bars.full_a[sta], pha, &bars, a);
             if (!ok) break;
             tc_fence_after();
             const int ua = __shfl_sync(0xffffffffu, sta, 0), ub = __shfl_sync(0xffffffffu, stb, 0);
@@ -288,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (q0 >= nf) break;
                 const int unit = __shfl_sync(0xffffffffu, f % kN, 0);
                 if (f >= kN) {
-                    ok = wait_warp(&bars.sum_empty[unit], (f / kN - 1) & 1, &bars);
+                    ok = wait_warp(&bars.sum_empty[unit], (f / kN - 1) & 1, &bars, a);
                     if (!ok) break;
                     tc_fence_after();
                 }
@@ -345,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int q0 = 0; q0 < GP; q0 += kG) {
                 if (q0 >= nf) break;
                 const int unit = f % kN;
-                ok = wait_warp(&bars.sum_full[unit], (f / kN) & 1, &bars);
+                ok = wait_warp(&bars.sum_full[unit], (f / kN) & 1, &bars, a);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(unit * kG * NB + half * (NB / 2));
@@ -388,10 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool failed = *reinterpret_cast<volatile int*>(&bars.failed) != 0;
     if (warp == kMmaWarp) {
         if (failed && elect_one()) {  // MMAs in flight end before their memory goes
-            mbar_init(&bars.full_a[0], 1);
-            fence_mbar_init();
-            tc_commit(&bars.full_a[0]);
-            mbar_wait_bounded(&bars.full_a[0], 0, kWaitLimit);
+            tc_commit(&bars.done);
+            mbar_wait_bounded(&bars.done, 0, kW4WaitLimit);
         }
         __syncwarp();
         tmem_dealloc(tmem, kUnits<NB, GP> * kUnit<NB, GP> * NB);
@@ -511,11 +517,17 @@ cudaError_t launch_group(const W4Args& a, int group, int nb, bool gated, int gx,
 
 }  // namespace
 
+// The limit of the waits in launches from now on.
+static std::atomic<long long> g_wait_limit{kW4WaitLimit};
+
+void set_wait_limit(long long clocks) { g_wait_limit.store(clocks < 0 ? kW4WaitLimit : clocks); }
+
 cudaError_t launch_w4_tc(W4Args a, int group, bool bf, int nw, cudaStream_t st) {
     const W4TcPlan p = w4_tc_plan(a.M, a.T, a.S, a.pieces, nw);
     a.rows = p.rows;
     a.cs = p.cs;
     a.last_groups = a.Q - (a.S - 1) * (128 / group);
+    a.wait_limit = g_wait_limit.load();
     return bf ? launch_group<1>(a, group, p.nb, nw == 2, p.gx, p.gy, st)
               : launch_group<0>(a, group, p.nb, nw == 2, p.gx, p.gy, st);
 }
@@ -579,8 +591,8 @@ cudaError_t launch_rows(bool f32, const void* x, long long ldx, int M, int K, vo
 cudaError_t step_status(int* status) {
     cudaError_t e = cudaMemcpyFromSymbol(status, g_step_status, sizeof(int));
     if (e != cudaSuccess) return e;
-    const int zero = 0;
-    if (*status) e = cudaMemcpyToSymbol(g_step_status, &zero, sizeof(int));
+    const int zeros[3] = {};
+    if (*status) e = cudaMemcpyToSymbol(g_step_status, zeros, sizeof zeros);
     return e;
 }
 

@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_model_sessions import q2
+from test_model_sessions import SMALL, prompt, q2
 from test_step_ops import dbl, fill, half_step, need_gpu, plain_quantize, random_matrix, sum_tol  # noqa: F401
 
 
@@ -130,3 +130,74 @@ def test_a_refused_call_leaves_no_error_behind(kv):
     with pytest.raises(kv.KVError):
         q2().Model(0, cfg)
     fine()
+
+
+# ------------------------------------------------------- waits that run out
+@pytest.fixture
+def no_waiting(kv):
+    """Launches give up wherever something is not ready, from its call on; the default limit afterwards."""
+    yield lambda: kv.step_ops_wait_limit(0)
+    kv.step_ops_wait_limit()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,xd", [(20, 200, 4096, "f16"), (100, 200, 4096, "bf16"), (300, 200, 4096, "f16"),
+                                      (70, 20000, 260, "f16"), (60, 500, 700, "f32")])
+@pytest.mark.parametrize("group", [32, 128])
+def test_a_wait_that_runs_out_is_reported(kv, no_waiting, m, n, k, xd, group):
+    """By step_ops_status, once; the device works on and the next call is right."""
+    need_gpu()
+    rng = np.random.default_rng(m + n)
+    w, ref = random_matrix(kv, rng, n, k, group, True)
+    x, out = fill(rng, (m, k), xd), torch.empty(m, n, device="cuda")
+    assert kv.step_ops_status() == kv.KV_OK
+    for op in (lambda: kv.w4_linear(w, x, out), lambda: kv.w4_gated(w, w, x, out)):
+        no_waiting()
+        op()
+        assert kv.step_ops_status() == kv.KV_ERR_TIMEOUT
+        assert kv.step_ops_status() == kv.KV_OK
+        kv.step_ops_wait_limit()
+        kv.w4_linear(w, x, out)
+        near_linear(kv, w, ref, x, out, group, "f32")
+        assert kv.step_ops_status() == kv.KV_OK
+
+
+@pytest.fixture(scope="module")
+def model4():
+    """The small model on 4-bit weights."""
+    need_gpu()
+    M = q2().Model(0, SMALL, max_sessions=8)
+    for name, a in q2().synth_weights(SMALL, seed=21):
+        M.set_tensor(name, a)
+    M.quantize_weights(64)
+    yield M
+    M.close()
+
+
+@pytest.mark.gpu
+def test_a_forwards_wait_that_runs_out_fails_the_forward(kv, no_waiting, model4):
+    """KV_ERR_TIMEOUT from the model's own call, nothing for step_ops_status to find; other sessions go on."""
+    need_gpu()
+    M = model4
+    a, b = M.create_session(), M.create_session()
+    M.forward_session(a, prompt(20, 1))
+    want, pick = M.forward_session(b, prompt(130, 2))
+    M.destroy_session(b)
+    b = M.create_session()
+    no_waiting()
+    with pytest.raises(q2().KVError) as e:
+        M.forward_session(b, prompt(130, 2))
+    assert e.value.status == kv.KV_ERR_TIMEOUT
+    with pytest.raises(q2().KVError) as e:
+        M.generate_session(b, prompt(130, 3), 3)
+    assert e.value.status == kv.KV_ERR_TIMEOUT
+    kv.step_ops_wait_limit()
+    assert kv.step_ops_status() == kv.KV_OK
+    M.destroy_session(b)
+    b = M.create_session()
+    got, again = M.forward_session(b, prompt(130, 2))
+    assert np.array_equal(got, want) and again == pick
+    logits, _ = M.forward_session(a, [3])
+    assert np.all(np.isfinite(logits))
+    for s in (a, b):
+        M.destroy_session(s)
