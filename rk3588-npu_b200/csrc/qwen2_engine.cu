@@ -475,12 +475,15 @@ int guarded(F f) {
 }
 
 // After a forward: the groups' ids join their sessions' histories.
-void note_ids(qw2_model* m, const std::vector<Group>& gs) {
-    for (const Group& g : gs) {
-        std::vector<int>& h = m->session_ids[g.session];
-        h.insert(h.end(), g.tokens, g.tokens + g.n);
-        if (g.n > 1) m->session_gen[g.session] = (int)h.size();
-    }
+int note_ids(qw2_model* m, const std::vector<Group>& gs) {
+    return guarded([&] {
+        for (const Group& g : gs) {
+            std::vector<int>& h = m->session_ids[g.session];
+            h.insert(h.end(), g.tokens, g.tokens + g.n);
+            if (g.n > 1) m->session_gen[g.session] = (int)h.size();
+        }
+        return KV_OK;
+    });
 }
 
 // The choices of the groups whose session has controls, in place of the plain
@@ -746,11 +749,11 @@ int forward_exact(qw2_model* m, std::vector<Group>& gs) {
     QW_CUDA(cudaMemcpyAsync(keys.data(), m->best, sizeof(unsigned long long) * G, cudaMemcpyDeviceToHost, st));
     int status = 0;
     QW_OK(kvp_device_status(m->pool, st, &status));  // synchronises the stream
+    QW_OK(note_ids(m, gs));
     if (status != 0) return status;
     for (int g = 0; g < G; ++g)
         gs[g].argmax = keys[g] ? (int)(0xFFFFFFFFu - (uint32_t)(keys[g] & 0xFFFFFFFFu)) : 0;
     return guarded([&] {
-        note_ids(m, gs);
         std::vector<int> order(G);
         for (int g = 0; g < G; ++g) order[g] = g;
         return choose_controlled(m, gs, order);
@@ -906,15 +909,13 @@ int forward_groups(qw2_model* m, std::vector<Group>& gs) {
                                     sizeof(float) * (size_t)c.vocab, cudaMemcpyDeviceToHost, st));
     int status = 0;
     QW_OK(kvp_device_status(m->pool, st, &status));  // synchronises the stream
+    QW_OK(note_ids(m, gs));                          // in the caches by now, whatever the status
     if (status != 0) return status;
     for (int i = 0; i < G; ++i) {
         const unsigned long long key = keys[i];
         gs[order[i]].argmax = key ? (int)(0xFFFFFFFFu - (uint32_t)(key & 0xFFFFFFFFu)) : 0;
     }
-    return guarded([&] {
-        note_ids(m, gs);
-        return choose_controlled(m, gs, order);
-    });
+    return guarded([&] { return choose_controlled(m, gs, order); });
 }
 
 using Clock = std::chrono::steady_clock;

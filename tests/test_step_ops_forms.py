@@ -201,3 +201,20 @@ def test_a_forwards_wait_that_runs_out_fails_the_forward(kv, no_waiting, model4)
     assert np.all(np.isfinite(logits))
     for s in (a, b):
         M.destroy_session(s)
+
+
+@pytest.mark.gpu
+def test_a_failed_forwards_ids_stay_in_the_history(kv, no_waiting, model4):
+    """The history that controls see is the ids in the cache, those of a forward that failed on the way included."""
+    need_gpu()
+    M, seen = model4, []
+    s = M.create_session()
+    M.set_controls(s, mask=lambda session, ids, gen_from: seen.append((list(ids), gen_from)))
+    first = prompt(130, 5)
+    no_waiting()
+    with pytest.raises(q2().KVError):
+        M.forward_session(s, first)
+    kv.step_ops_wait_limit()
+    M.forward_session(s, [9])
+    assert seen == [(first + [9], 130)]
+    M.destroy_session(s)
