@@ -58,6 +58,10 @@ constexpr int kCodes = 2 * 1024 + 128;  // a span of a warp's two tiles, and the
 constexpr int kThreads = 16 * 32;
 constexpr int kMmaWarp = 7;
 constexpr int kHalfA = 128 * 128;  // 64 inputs of 128 rows
+// Registers of a thread of the unpacking, the copying and issuing and the two
+// scaling warpgroups where a tile has 256 columns: what the launch has, dealt anew.
+constexpr int kLaunchRegs = 65536 / kThreads, kRegs[3] = {104, 56, 176};
+static_assert(kRegs[0] + kRegs[1] + 2 * kRegs[2] <= 4 * kLaunchRegs, "the scaling warps would wait for registers for good");
 
 template <int NB>
 struct Smem {
@@ -88,9 +92,11 @@ __device__ __noinline__ void gave_up(const W4Args& a, Bars* b) {
     *reinterpret_cast<volatile int*>(&b->failed) = 1;
 }
 
-// A whole warp's wait: all of its lanes, or none, go on.
+// A whole warp's wait: all of its lanes, or none, go on.  The test without a
+// suspend stands alone in front, as most waits end there: 512 gated rows 45.4 us,
+// 48.5 with it behind the choice by the limit, 51.5 with the rest in a call.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Bars* b, const W4Args& a) {
-    bool ok = a.wait_limit > 0 ? mbar_wait_bounded(bar, parity, a.wait_limit) : mbar_test_wait(bar, parity);
+    bool ok = mbar_test_wait(bar, parity) || (a.wait_limit > 0 && mbar_wait_bounded(bar, parity, a.wait_limit));
     if (!ok) gave_up(a, b);
     ok = ok && !*reinterpret_cast<volatile int*>(&b->failed);
     return __all_sync(0xffffffffu, ok);
@@ -135,7 +141,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     __shared__ Bars bars;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // from lane 0, so that the roles part by uniform branches
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int cs = a.cs, rank = (int)blockIdx.x % cs;
     const int tile0 = (int)blockIdx.x / cs * (GATED ? 4 : 8);  // first 16-row tile
     const int m0 = blockIdx.y * a.rows, mrows = min(a.rows, a.M - m0);
@@ -175,8 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp < 4) {
         // ---------------------------------------------------- A: unpack codes
-        // 512 threads of 128 registers: warpgroups of 104 + 56 + 2 x 176
-        if (NB == 256) regs_down<104>();
+        if (NB == 256) regs_down<kRegs[0]>();
         // A short loop on purpose: sixteen warps of four roles share the
         // instruction caches, and unrolling this role starved the others.
         const int g = lane >> 2, c = lane & 3, odd = g & 1;
@@ -253,10 +259,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             slot = slot + 1 == kAhead ? 0 : slot + 1;
         }
         cp_wait<0>();
-    } else if (warp < kMmaWarp) {
-        // ------------------------------------------- B: rows of x (warp 4; 5 and 6 idle)
-        if (NB == 256) regs_down<56>();
+    } else if (warp < 8) {
+        if (NB == 256) regs_down<kRegs[1]>();  // by the whole warpgroup, before its warps' roles part
         if (warp == 4) {
+            // --------------------------------------- B: rows of x (5 and 6 idle)
             int st = 0, ph = 1, sp = s0;
             for (; sp < s1; ++sp) {
                 if (sp - s0 >= kStagesB<NB> && !wait_warp(&bars.empty_b[st], ph, &bars, a)) break;
@@ -272,61 +278,60 @@ __global__ void __launch_bounds__(kThreads, 1)
             // no copy outlives the CTA, wherever another warp gave up
             for (int i = max(sp - s0 - kStagesB<NB>, 0); i < sp - s0; ++i)
                 mbar_wait_bounded(&bars.full_b[i % kStagesB<NB>], (i / kStagesB<NB>) & 1, kW4WaitLimit);
-        }
-    } else if (warp == kMmaWarp) {
-        // ----------------------------------------------------------- MMA issue
-        if (NB == 256) regs_down<56>();
-        // The whole warp runs the loop and one lane issues: the operands of an
-        // MMA live in uniform registers, which only uniform control flow fills
-        // directly.
-        constexpr uint32_t idesc = idesc_f16(BF, 128, NB, 0);
-        const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0), d0 = __shfl_sync(0xffffffffu, tmem, 0);
-        constexpr int kG = kUnit<NB, GP>, kN = kUnits<NB, GP>;
-        int f = 0, sta = 0, stb = 0, pha = 0, phb = 0;  // units so far; stages and their phases
-        bool ok = true;
-        for (int sp = s0; ok && sp < s1; ++sp) {
-            ok = wait_warp(&bars.full_b[stb], phb, &bars, a) && wait_warp(&bars.full_a[sta], pha, &bars, a);
-            if (!ok) break;
-            tc_fence_after();
-            const int ua = __shfl_sync(0xffffffffu, sta, 0), ub = __shfl_sync(0xffffffffu, stb, 0);
-            const uint64_t da = sdesc(base + ua * (2 * kHalfA), 16, 1024), db = sdesc(base + SM::kB + ub * (2 * SM::kHalfB), 16, 1024);
-            const int nf = flushes(sp);
+        } else if (warp == kMmaWarp) {
+            // ------------------------------------------------------- MMA issue
+            // The whole warp runs the loop and one lane issues: the operands of an
+            // MMA live in uniform registers, which only uniform control flow fills
+            // directly.
+            constexpr uint32_t idesc = idesc_f16(BF, 128, NB, 0);
+            const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0), d0 = __shfl_sync(0xffffffffu, tmem, 0);
+            constexpr int kG = kUnit<NB, GP>, kN = kUnits<NB, GP>;
+            int f = 0, sta = 0, stb = 0, pha = 0, phb = 0;  // units so far; stages and their phases
+            bool ok = true;
+            for (int sp = s0; ok && sp < s1; ++sp) {
+                ok = wait_warp(&bars.full_b[stb], phb, &bars, a) && wait_warp(&bars.full_a[sta], pha, &bars, a);
+                if (!ok) break;
+                tc_fence_after();
+                const int ua = __shfl_sync(0xffffffffu, sta, 0), ub = __shfl_sync(0xffffffffu, stb, 0);
+                const uint64_t da = sdesc(base + ua * (2 * kHalfA), 16, 1024), db = sdesc(base + SM::kB + ub * (2 * SM::kHalfB), 16, 1024);
+                const int nf = flushes(sp);
 #pragma unroll
-            for (int q0 = 0; q0 < GP; q0 += kG) {
-                if (q0 >= nf) break;
-                const int unit = __shfl_sync(0xffffffffu, f % kN, 0);
-                if (f >= kN) {
-                    ok = wait_warp(&bars.sum_empty[unit], (f / kN - 1) & 1, &bars, a);
-                    if (!ok) break;
-                    tc_fence_after();
-                }
-                if (elect_one()) {
+                for (int q0 = 0; q0 < GP; q0 += kG) {
+                    if (q0 >= nf) break;
+                    const int unit = __shfl_sync(0xffffffffu, f % kN, 0);
+                    if (f >= kN) {
+                        ok = wait_warp(&bars.sum_empty[unit], (f / kN - 1) & 1, &bars, a);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    if (elect_one()) {
 #pragma unroll
-                    for (int q = q0; q < q0 + kG; ++q) {
-                        if (q >= nf) break;
+                        for (int q = q0; q < q0 + kG; ++q) {
+                            if (q >= nf) break;
 #pragma unroll
-                        for (int i = 0; i < 8 / GP; ++i) {
-                            const int kk = q * (8 / GP) + i;  // 16 inputs: 32 bytes on (the descriptors count 16)
-                            mma_ss(d0 + (unit * kG + q - q0) * NB, da + ((kk >> 2) * kHalfA + (kk & 3) * 32) / 16,
-                                   db + ((kk >> 2) * SM::kHalfB + (kk & 3) * 32) / 16, idesc, i != 0);
+                            for (int i = 0; i < 8 / GP; ++i) {
+                                const int kk = q * (8 / GP) + i;  // 16 inputs: 32 bytes on (the descriptors count 16)
+                                mma_ss(d0 + (unit * kG + q - q0) * NB, da + ((kk >> 2) * kHalfA + (kk & 3) * 32) / 16,
+                                       db + ((kk >> 2) * SM::kHalfB + (kk & 3) * 32) / 16, idesc, i != 0);
+                            }
+                        }
+                        tc_commit(&bars.sum_full[unit]);
+                        if (q0 + kG >= nf) {
+                            tc_commit(&bars.empty_a[ua]);
+                            tc_commit(&bars.empty_b[ub]);
                         }
                     }
-                    tc_commit(&bars.sum_full[unit]);
-                    if (q0 + kG >= nf) {
-                        tc_commit(&bars.empty_a[ua]);
-                        tc_commit(&bars.empty_b[ub]);
-                    }
+                    __syncwarp();
+                    ++f;
                 }
-                __syncwarp();
-                ++f;
+                if (++sta == kStagesA) sta = 0, pha ^= 1;
+                if (++stb == kStagesB<NB>) stb = 0, phb ^= 1;
             }
-            if (++sta == kStagesA) sta = 0, pha ^= 1;
-            if (++stb == kStagesB<NB>) stb = 0, phb ^= 1;
+            __syncwarp();
         }
-        __syncwarp();
     } else {
         // -------------------------------------------------- scale and accumulate
-        if (NB == 256) regs_up<176>();
+        if (NB == 256) regs_up<kRegs[2]>();
         const int quarter = warp & 3, half = (warp - 8) >> 2;
         const int r = quarter * 32 + lane;  // weight row of the CTA
         const __half* sc = a.scales[mat_of(r >> 4)] + (size_t)tile_of(r >> 4) * a.Q * 16 + (r & 7) * 2 + ((r >> 3) & 1);
@@ -390,8 +395,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     if (NB == 256) {  // every warp goes on with the registers of the launch
-        if (warp >= 8) regs_down<128>();
-        else regs_up<128>();
+        if (warp >= 8) regs_down<kLaunchRegs>();
+        else regs_up<kLaunchRegs>();
     }
     const bool failed = *reinterpret_cast<volatile int*>(&bars.failed) != 0;
     if (warp == kMmaWarp) {
@@ -477,6 +482,14 @@ cudaError_t launch_inst(const W4Args& a, int gx, int gy, cudaStream_t st) {
     static SmemGrant grant;
     cudaError_t e = grant.raise(reinterpret_cast<const void*>(fn), Smem<NB>::kBytes);
     if (e != cudaSuccess) return e;
+    if (NB == 256) {
+        // built with fewer registers, the scaling warps' share would never come free
+        static const int regs = [&] {
+            cudaFuncAttributes f = {};
+            return cudaFuncGetAttributes(&f, fn) == cudaSuccess ? f.numRegs : 0;
+        }();
+        if (regs < kLaunchRegs) return cudaErrorInvalidConfiguration;
+    }
     CUtensorMap map = {};
     if ((e = x_map(a, BF != 0, NB, &map)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

@@ -3,10 +3,13 @@ a GPU: what crosses the C boundary and when.  The C library's calls are stood in
 from __future__ import annotations
 
 import ctypes as C
+import os
+import re
 
 import numpy as np
 import pytest
 
+from conftest import PKG_DIR
 from test_model_sessions import q2
 
 
@@ -226,3 +229,19 @@ def test_scratch_is_what_the_call_asks_for(kv, streams, n, k, group, xd):
                 assert sum(made) >= want, (m, gated)
                 some += want > 0
     assert some
+
+
+def test_register_splits_are_changed_by_whole_warpgroups():
+    """setmaxnreg in w4_tc_kernel: one change per warpgroup and split, on conditions that do not part its four warps
+    (warp 7 issues, 4 to 6 copy: one warpgroup), and no more registers asked for than the launch brings."""
+    with open(os.path.join(PKG_DIR, "csrc", "w4_tc_kernel.cu")) as f:
+        src = f.read()
+    kernel = src[src.index("    w4_tc_kernel("):src.index("// x as TMA sees it")]
+    changes = [(m.group(1), m.start()) for m in re.finditer(r"regs_(?:up|down)<([^>]*)>\(\)", kernel)]
+    assert [c for c, _ in changes] == ["kRegs[0]", "kRegs[1]", "kRegs[2]", "kLaunchRegs", "kLaunchRegs"]
+    # the roles of warps 4 to 7 part inside their warpgroup's branch, after its change
+    branch = [kernel.index("if (warp < 4) {"), kernel.index("} else if (warp < 8) {"), kernel.index("} else if (warp == kMmaWarp) {")]
+    assert branch[0] < changes[0][1] < branch[1] < changes[1][1] < branch[2] < changes[2][1]
+    threads = int(re.search(r"kThreads = 16 \* (\d+)", src).group(1)) * 16
+    a, b, c = (int(v) for v in re.search(r"kRegs\[3\] = \{(\d+), (\d+), (\d+)\}", src).groups())
+    assert threads == 512 and 128 * (a + b + 2 * c) <= 65536 // threads * threads
