@@ -79,7 +79,9 @@ int w4_dequantize(const w4_matrix* m, float* out, long long ldo, void* stream);
  * itself.  Sums are fp32; an fp32 x keeps all its bits (three bf16 parts);
  * the result is rounded once.  A group's sum of (code - zero) * x is formed
  * before its scale, so that sum has to stay within fp32 (|x| below 1e35 does).
- * out must not overlap x.
+ * out must not overlap x; they may be columns of one buffer (rows the same
+ * distance apart in bytes: otherwise spans that meet are refused).  The same
+ * holds for residual and out, and for the rows of logits_adjust.
  * work: w4_work_bytes() of scratch, 16-byte aligned, overlapping nothing else,
  * or NULL: many rows of an x that is fp32, or not in 16-byte aligned rows, go
  * through it, and take longer without it. */
@@ -128,7 +130,8 @@ int step_ops_wait_limit(long long clocks);
  * of the row's ld_mask words, 1 = allowed; bits from vocab on are not read
  * as tokens.  hist, bias_ids, mask, pick and the penalties may be NULL (none;
  * repetition 1).  out may be logits itself (same ld); another overlap is
- * refused. */
+ * refused.  Rows of out that start at another distance from a 16-byte boundary
+ * than those of logits are written value by value, which takes longer. */
 typedef struct logits_call {
     int device, rows, vocab, dtype;
     const void* logits;

@@ -3,6 +3,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <algorithm>
+
 #include "kvattn.h"
 #include "kvattn_internal.h"
 #include "step_ops.h"
@@ -50,12 +52,24 @@ int check_matrix(const w4_matrix* m, const char* what) {
     return KV_OK;
 }
 
-// The bytes that `rows` rows of `n` elements, `ld` apart, span.
+// `rows` rows of `n` elements, `ld` apart: the bytes that they span, and whether
+// any of them are another's.  Rows of one pitch may lie between the other's
+// (columns of one buffer); where the pitches differ, spans that meet count as shared.
 struct Range {
     size_t a, b;
+    long long rows, width, pitch;
     Range(const void* p, long long rows, long long n, long long ld, size_t es)
-        : a(reinterpret_cast<size_t>(p)), b(a + (rows > 0 ? (size_t)((rows - 1) * ld + n) * es : 0)) {}
-    bool meets(const Range& o) const { return a < o.b && o.a < b; }
+        : a(reinterpret_cast<size_t>(p)), b(a + (rows > 0 ? (size_t)((rows - 1) * ld + n) * es : 0)), rows(rows),
+          width(n * (long long)es), pitch(ld * (long long)es) {}
+    bool meets(const Range& o) const {
+        if (a >= o.b || o.a >= b) return false;
+        if (pitch != o.pitch || pitch <= 0) return true;
+        // row i here and row j there meet where t = i - j has  t pitch < d + o.width  and  t pitch > d - width
+        const long long d = (long long)(o.a - a);
+        auto below = [&](long long v) { return v >= 0 ? v / pitch : -((-v + pitch - 1) / pitch); };  // floor(v / pitch)
+        const long long first = std::max(below(d - width) + 1, 1 - o.rows), last = std::min(-below(-(d + o.width)) - 1, rows - 1);
+        return first <= last;
+    }
 };
 
 int check_dtype(int dtype, const char* what) {

@@ -245,3 +245,37 @@ def test_register_splits_are_changed_by_whole_warpgroups():
     threads = int(re.search(r"kThreads = 16 \* (\d+)", src).group(1)) * 16
     a, b, c = (int(v) for v in re.search(r"kRegs\[3\] = \{(\d+), (\d+), (\d+)\}", src).groups())
     assert threads == 512 and 128 * (a + b + 2 * c) <= 65536 // threads * threads
+
+
+def brute(a, rows_a, width_a, b, rows_b, width_b, pitch):
+    one = {a + i * pitch + k for i in range(rows_a) for k in range(width_a)}
+    return any(b + j * pitch + k in one for j in range(rows_b) for k in range(width_b))
+
+
+def test_columns_of_one_buffer_do_not_overlap(kv):
+    """x, out and residual, logits and out with the same distance between rows: refused where they share a byte, and
+    only there (what is accepted gets as far as the device, which is not there)."""
+    rng = np.random.default_rng(0)
+    A = 0x100000
+    codes = kv._W4Matrix(999, 3, 4, 32, 0x900000, 0x900000, None)
+    seen = set()
+
+    def outcome(fn, *args):
+        with pytest.raises(kv.KVError) as e:
+            kv.call(fn, *args, None)
+        assert "overlap" in str(e.value) or "no CUDA device 999" in str(e.value), str(e.value)
+        return "overlap" in str(e.value)
+
+    for _ in range(3000):
+        m, ld = int(rng.integers(1, 5)), int(rng.integers(4, 14))  # rows of 2-byte elements: 4 of x, 3 of out
+        at, res = A + 2 * int(rng.integers(-40, 41)), A + 2 * int(rng.integers(-40, 41))
+        # x of another pitch far away, so that only residual and out may meet
+        got = (outcome("w4_linear", C.addressof(codes), A, 0, m, ld, None, None, 0, at, 0, ld, None),
+               outcome("w4_linear", C.addressof(codes), 0x500000, 0, m, 4, None, res, ld, at, 0, ld, None),
+               outcome("logits_adjust", C.byref(kv._LogitsCall(device=999, rows=m, vocab=3, dtype=0, logits=A, ld_logits=ld,
+                                                               out=at, ld_out=ld))))
+        want = (brute(A, m, 8, at, m, 6, 2 * ld), res != at and brute(res, m, 6, at, m, 6, 2 * ld),
+                A != at and brute(A, m, 6, at, m, 6, 2 * ld))
+        assert got == want, (m, ld, at - A, res - A)
+        seen.update(enumerate(got))
+    assert len(seen) == 6
