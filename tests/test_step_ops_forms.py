@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from test_model_sessions import SMALL, prompt, q2
-from test_step_ops import dbl, fill, half_step, need_gpu, plain_quantize, random_matrix, sum_tol  # noqa: F401
+from test_step_ops import dbl, fill, flat, half_step, logits_inputs, mask_words, need_gpu, plain_logits, random_matrix, sum_tol
 
 
 def near_linear(kv, w, ref, x, out, group, yd):
@@ -218,3 +218,151 @@ def test_a_failed_forwards_ids_stay_in_the_history(kv, no_waiting, model4):
     M.forward_session(s, [9])
     assert seen == [(first + [9], 130)]
     M.destroy_session(s)
+
+
+# ---------------------------------------------------------- special values
+@pytest.mark.gpu
+@pytest.mark.parametrize("xd", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m,n,k,group", [(20, 100, 4100, 32), (100, 70, 700, 64), (300, 40, 333, 128)])
+def test_non_finite_rows_among_many(kv, m, n, k, group, xd):
+    """Infinity, NaN and large values in rows of the tensor-memory form and of the copies that it reads: every column
+    tile; a row's value stays in its row, and what it makes of the row is what the products say."""
+    need_gpu()
+    rng = np.random.default_rng(m)
+    w, ref = random_matrix(kv, rng, n, k, group, True)
+    x = fill(rng, (m, k), xd)
+    rows = [0, m // 3, m // 2, m - 1]
+    top = min(torch.finfo(x.dtype).max, 1e34)
+    for row, value in zip(rows, (float("inf"), float("-inf"), float("nan"), top)):
+        x[row, (7 * row + k - 1) % k] = value
+    out = torch.empty(m, n, device="cuda")
+    kv.w4_linear(w, x, out)
+    got, want = dbl(out), (x.cpu().double() @ torch.from_numpy(ref).T).numpy()
+    for row in rows[:3]:
+        assert np.array_equal(np.isnan(got[row]), np.isnan(want[row]))
+        f = ~np.isnan(want[row])
+        assert np.array_equal(got[row][f], want[row][f])
+    others = np.setdiff1d(np.arange(m), rows[:3])
+    y = dbl(x)[others]
+    tol = sum_tol(y, ref, group) + 2.0**-23 * np.abs(want[others])
+    assert np.all(np.abs(got[others] - want[others]) <= tol)
+    gate = torch.empty(m, n, device="cuda")
+    kv.w4_gated(w, w, x, gate)
+    assert np.all(np.isfinite(dbl(gate)[np.setdiff1d(np.arange(m), rows)]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,xd,yd", [(300, "f16", "f16"), (64, "f32", "bf16"), (30, "bf16", "f32")])
+def test_many_rows_in_place(kv, m, xd, yd):
+    """The residual is out itself, rows apart, and out's rows start anywhere."""
+    need_gpu()
+    rng = np.random.default_rng(m)
+    n, k = 333, 4104
+    w, ref = random_matrix(kv, rng, n, k, 64, False)
+    x, wide = fill(rng, (m, k), xd), fill(rng, (m, n + 9), yd)
+    before = wide.clone()
+    out = wide[:, 5:5 + n]
+    kv.w4_linear(w, x, out, residual=out)
+    res = dbl(before[:, 5:5 + n])
+    want = dbl(x) @ ref.T + res
+    tol = sum_tol(dbl(x), ref, 64) + 2.0**-22 * np.abs(want) + 2.0**-23 * np.abs(res)
+    tol = tol + half_step(np.abs(want) + tol, yd)
+    assert np.all(np.abs(dbl(out) - want) <= tol)
+    assert torch.equal(wide[:, :5], before[:, :5]) and torch.equal(wide[:, 5 + n:], before[:, 5 + n:])
+
+
+# ------------------------------------------------------------- offsets past 32 bits
+@pytest.mark.gpu
+def test_a_matrix_past_32_bits(kv):
+    """600000 x 8192: the codes pass 2^31 bytes and the values 2^32 elements.  Its last rows give what they give alone."""
+    need_gpu()
+    n, k, group = 600000, 8192, 64
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    w = torch.empty(n, k, dtype=torch.float16, device="cuda").normal_(std=0.02, generator=gen)
+    big = kv.w4_quantize(w, group, zero_points=True)
+    spans = (0, 299984, n - 48)
+    small = [kv.w4_quantize(w[a:a + 48].clone(), group, zero_points=True) for a in spans]
+    del w
+    rng = np.random.default_rng(5)
+    for m, xd in ((1, "f32"), (7, "bf16"), (48, "f16")):
+        x = fill(rng, (m, k), xd)
+        out = torch.empty(m, n, device="cuda")
+        kv.w4_linear(big, x, out)
+        for a, s in zip(spans, small):
+            near_linear(kv, s, dbl(s.dequantize()), x, out[:, a:a + 48], group, "f32")
+    values = big.dequantize()
+    for a, s in zip(spans, small):
+        assert torch.equal(values[a:a + 48], s.dequantize())
+
+
+@pytest.mark.gpu
+def test_rows_further_apart_than_32_bits(kv):
+    """Rows of x, out, residual and logits more than 2^31 elements from the first."""
+    need_gpu()
+    rng = np.random.default_rng(6)
+    far = 2**31 // 32 + 8
+    room = torch.empty(34 * far, dtype=torch.float16, device="cuda")
+    w, ref = random_matrix(kv, rng, 40, 264, 32, False)
+    for m in (3, 34):  # both forms
+        x = torch.as_strided(room, (m, 264), (far * (33 // (m - 1)), 1))
+        x.copy_(fill(rng, (m, 264), "f16"))
+        out = torch.as_strided(room, (m, 40), (far * (33 // (m - 1)), 1), 512)
+        out.zero_()
+        kv.w4_linear(w, x, out, residual=out)
+        near_linear(kv, w, ref, x, out, 32, "f16")
+    logits = torch.as_strided(room, (34, 1000), (far, 1), 2048)
+    logits.copy_(fill(rng, (34, 1000), "f16"))
+    near, pick, want = torch.empty(34, 1000, dtype=torch.float16, device="cuda"), *(
+        torch.empty(34, dtype=torch.int32, device="cuda") for _ in range(2))
+    kw = dict(hist=torch.arange(34, dtype=torch.int32, device="cuda"), hist_off=torch.arange(35, dtype=torch.int32, device="cuda"),
+              presence=torch.ones(34, device="cuda"))
+    kv.logits_adjust(logits.contiguous(), near, pick=want, **kw)
+    kv.logits_adjust(logits, logits, pick=pick, **kw)
+    assert torch.equal(logits, near) and torch.equal(pick, want)
+
+
+# --------------------------------------------------------------------- logits
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,vocab,hist,bias", [(3, 50257, 900, 40), (1, 160001, 300, 20), (20, 160001, 40, 5), (2, 700, 60, 70000)])
+def test_logits_into_rows_aligned_otherwise(kv, dtype, rows, vocab, hist, bias):
+    """out off the 16-byte boundaries that logits stands on, and rows of odd length: bit for bit what aligned rows give."""
+    need_gpu()
+    rng = np.random.default_rng(vocab + rows)
+    x, hs, bs, gen, rep, pres, freq, ok = logits_inputs(rng, rows, vocab, dtype, hist, bias, True)
+    args = dict(mask=mask_words(ok), gen_from=torch.tensor(gen, dtype=torch.int32, device="cuda"))
+    args["hist"], args["hist_off"] = flat(hs)
+    args["bias_ids"], args["bias_off"] = flat(bs, lambda v: v[0])
+    args["bias"], _ = flat(bs, lambda v: v[1], torch.float32)
+    for name, v in (("repetition", rep), ("presence", pres), ("frequency", freq)):
+        args[name] = torch.from_numpy(v).cuda()
+    want, pick = torch.empty_like(x), torch.empty(rows, dtype=torch.int32, device="cuda")
+    kv.logits_adjust(x, want, pick=pick, **args)
+    for a, b in ((0, 1), (1, 0), (3, 3), (5, 2)):  # elements before the rows of logits and of out
+        src = torch.full((rows, vocab + 7), 9.0, dtype=x.dtype, device="cuda")
+        dst = torch.full((rows, vocab + 8), 9.0, dtype=x.dtype, device="cuda")
+        src[:, a:a + vocab] = x
+        got = torch.empty_like(pick)
+        kv.logits_adjust(src[:, a:a + vocab], dst[:, b:b + vocab], pick=got, **args)
+        assert torch.equal(dst[:, b:b + vocab], want) and torch.equal(got, pick)
+        assert torch.all(dst[:, :b] == 9.0) and torch.all(dst[:, b + vocab:] == 9.0)
+
+
+@pytest.mark.gpu
+def test_controls_in_the_reference_order_forward():
+    """qw2_set_exact: the same controls on the logits of that forward."""
+    need_gpu()
+    M = q2().Model(0, SMALL, max_sessions=2)
+    for name, a in q2().synth_weights(SMALL, seed=22):
+        M.set_tensor(name, a)
+    M.set_exact(True)
+    s = M.create_session()
+    M.set_controls(s, repetition_penalty=1.5, presence_penalty=0.25, frequency_penalty=0.5, bias={3: 1.0, 17: -2.0})
+    history = prompt(9, 4)
+    logits, am = M.forward_session(s, history)
+    for _ in range(6):
+        y, _ = plain_logits(logits.astype(np.float64), history, 9, 1.5, 0.25, 0.5, [(3, 1.0), (17, -2.0)], None)
+        assert am == int(np.argmax(y))
+        history = history + [am]
+        logits, am = M.forward_session(s, [am])
+    M.close()
