@@ -206,6 +206,11 @@ struct qw2_model {
     std::vector<void*> allocs;
 
     int alloc(void** p, size_t bytes) {
+        try {  // room for its entry first
+            if (allocs.size() == allocs.capacity()) allocs.reserve(2 * allocs.size() + 64);
+        } catch (const std::exception& e) {
+            return qfail(KV_ERR_OOM, "host memory: %s", e.what());
+        }
         cudaError_t e = cudaMalloc(p, bytes);
         if (e != cudaSuccess) return qfail(KV_ERR_OOM, "cudaMalloc(%zu): %s", bytes, cudaGetErrorString(taken(e)));
         allocs.push_back(*p);
@@ -1624,6 +1629,10 @@ int qw2_quantize_weights(qw2_model* m, int group, int zero_points) {
         int n, k;
     };
     std::vector<Item> items;
+    QW_OK(guarded([&] {
+        items.reserve(5 * m->L.size() + 1);
+        return KV_OK;
+    }));
     for (auto& Ly : m->L) {
         items.push_back({&Ly.qqkv, &Ly.wqkv, H + 2 * kvd, H});
         items.push_back({&Ly.qo, &Ly.wo, H, H});

@@ -4,6 +4,9 @@ waits that run out.  Tolerances are those of test_step_ops.py."""
 from __future__ import annotations
 
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -366,3 +369,67 @@ def test_controls_in_the_reference_order_forward():
         history = history + [am]
         logits, am = M.forward_session(s, [am])
     M.close()
+
+
+FIRST = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import numpy as np, torch
+from conftest import load_pkg
+from test_step_ops import fill, random_matrix
+kv = load_pkg()
+kv.load()
+rng = np.random.default_rng(3)
+w, _ = random_matrix(kv, rng, 300, 1000, 32, True)
+calls = []
+for m, xd in ((1, "f32"), (300, "f32"), (300, "f16"), (20, "bf16")):
+    x, out = fill(rng, (m, 1000), xd), torch.zeros(m, 300, device="cuda")
+    calls.append((lambda x=x, out=out: kv.w4_linear(w, x, out), out))
+    out = torch.zeros(m, 300, device="cuda")
+    calls.append((lambda x=x, out=out: kv.w4_gated(w, w, x, out), out))
+logits, out = fill(rng, (3, 5000), "f32"), torch.zeros(3, 5000, device="cuda")
+calls.append((lambda: kv.logits_adjust(logits, out, presence=torch.ones(3, device="cuda")), out))
+half, values = fill(rng, (64, 200), "f16"), torch.zeros(64, 200, device="cuda")
+calls.append((lambda: kv.w4_quantize(half, 64).dequantize(out=values), values))
+got = []
+for f, out in calls:
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        f()
+    graph.replay()
+    torch.cuda.synchronize()
+    got.append((graph, out.clone()))
+    out.zero_()
+for (f, out), (graph, was) in zip(calls, got):
+    f()
+    torch.cuda.synchronize()
+    assert out.abs().sum() > 0 and torch.equal(out, was)
+# two graphs and an eager call at once, the default stream by its address
+s = torch.cuda.Stream()
+for _ in range(3):
+    for (f, out), (graph, was) in zip(calls, got):
+        graph.replay()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        got[2][0].replay()
+    got[4][0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, was) for (f, out), (graph, was) in zip(calls, got))
+x, out = fill(rng, (64, 1000), "f32"), [torch.zeros(64, 300, device="cuda") for _ in range(2)]
+kv.w4_linear(w, x, out[0])
+kv.w4_linear(w, x, out[1], stream=0)
+assert torch.equal(kv.w4_quantize(half, 64, stream=0).dequantize(stream=0), values)
+torch.cuda.synchronize()
+assert torch.equal(*out)
+print("fine")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_are_captured():
+    """Every operator's first call of a process inside a capture, graphs replayed side by side, the default stream
+    given by its address."""
+    need_gpu()
+    r = subprocess.run([sys.executable, "-c", FIRST, os.path.dirname(os.path.abspath(__file__))], capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stdout + r.stderr
