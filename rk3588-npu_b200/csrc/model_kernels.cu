@@ -64,13 +64,6 @@ __device__ __forceinline__ float dot8h(const uint4& w, const uint4& x, float acc
 
 constexpr int kStageU = 2;  // 16-byte fp32 input chunks per thread in flight while staging
 
-// 1 / rms of an fp32 row of H values (op_rmsnorm.cpp:12-15) by a 256-thread
-// block: thread t sums the rounded squares of its float4 chunks t, t + 256,
-// ... (components in order), then a warp tree, then the 8 warps in order.
-// Every caller (the standalone kernel and the fused projections) runs this
-// same order, so all of them get the same value.  All loads of a thread are
-// issued before any is used.
-
 // Finish 1/rms from each thread's partial sum (warp tree, then the 8 warps in
 // order; every thread of the 256 gets the value).
 __device__ __forceinline__ float block_inv_rms_from(float s, int H, float eps, float* part) {
@@ -85,6 +78,11 @@ __device__ __forceinline__ float block_inv_rms_from(float s, int H, float eps, f
     return __fdiv_rn(1.0f, rms);
 }
 
+// 1 / rms of an fp32 row of H values (op_rmsnorm.cpp:12-15) by a 256-thread
+// block: thread t sums the rounded squares of its float4 chunks t, t + 256,
+// ... (components in order), then a warp tree, then the 8 warps in order.
+// (Where a warp stages a row by itself, here and in the 4-bit projections, its
+// lanes sum in another order: the values may differ in their last bit.)
 __device__ __forceinline__ float block_inv_rms(const float* __restrict__ xr, int H, float eps, float* part) {
     const float4* src = reinterpret_cast<const float4*>(xr);
     const int n4 = H >> 2;

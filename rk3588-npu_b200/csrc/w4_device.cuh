@@ -28,7 +28,8 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
 }
 
 // Eight codes minus their zero point as four pairs of fp16 / bf16 values, in
-// input order.
+// input order.  The way of setting integers under a fixed exponent is that of
+// Kim, Henry, Fahim and Hassan Awadalla, "Who Says Elephants Can't Run" (2022).
 template <int BF>
 __device__ __forceinline__ void unpack(uint32_t w, uint2 zc, uint32_t (&p)[4]) {
     if (BF) {

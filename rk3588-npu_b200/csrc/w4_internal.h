@@ -66,6 +66,8 @@ struct W4Args {
     }
 };
 
+// The part that the plans below are made for.  On fewer SMs their grids run in
+// more turns than planned: slower, and nothing else, as a CTA waits for none but its cluster's.
 constexpr int kSms = 148;
 constexpr long long kW4WaitLimit = 2000000000LL;  // SM clocks: about a second
 constexpr int kW4MaxSmem = 227 * 1024;
