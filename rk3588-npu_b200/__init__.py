@@ -489,7 +489,7 @@ def _on_stream(stream, device, make):
     """make()'s tensors, allocated for the stream that a call runs on: a block of
     the current stream's may still be in use by that stream's pending work,
     which `stream` does not wait for."""
-    if stream is None:
+    if stream is None or _stream_on(stream, device.index) == _stream_on(None, device.index):
         return make()
     import torch
     s = torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream

@@ -279,3 +279,16 @@ def test_columns_of_one_buffer_do_not_overlap(kv):
         assert got == want, (m, ld, at - A, res - A)
         seen.update(enumerate(got))
     assert len(seen) == 6
+
+
+@pytest.mark.parametrize("stream", [Stream(HERE), HERE], ids=["object", "address"])
+def test_the_current_stream_by_name_is_the_current_stream(kv, streams, monkeypatch, stream):
+    import torch
+
+    def never(s):
+        raise AssertionError("a change of stream for the current one")
+
+    monkeypatch.setattr(torch.cuda, "stream", never)
+    w = w4_of(kv, 64, 512, 64)
+    kv.w4_linear(w, Tensor((64, 512), torch.float32), Tensor((64, 64), torch.float32), stream=stream)
+    assert [t.home for t in streams["made"]] == [HERE]
